@@ -220,6 +220,111 @@ yl_status yl_attention_noalloc(float *out, const float *q, const float *key_cach
 yl_status yl_swiglu_quantize(const float *gate, const float *up, size_t hidden, size_t batch,
                              float *h, int32_t qfmt, int8_t *q, float *scale, void *stream);
 
+/* --------------------------------------------------- paged cache, scoring
+ * No counterparts in the reference, which holds one conversation: ops for
+ * programs that serve many conversations from one pool of cache pages.
+ * Activations are f32 as in the ops above; results differ from a serial f32
+ * evaluation in rounding only (f32 sums in another order).  Everything is
+ * enqueued on `stream` and not waited for, nothing is allocated and the host
+ * reads no device memory, so calls can be captured into a graph; lengths and
+ * page tables are read when the work runs, so a replay sees their new values. */
+
+typedef enum { YL_T_F32 = 0, YL_T_F16 = 1, YL_T_BF16 = 2 } yl_dtype;
+
+/* One layer's pool of pages (device): keys and values, each
+ * [n_pages][n_kv_heads][page_size][head_size] of `dtype`, 16-byte aligned.
+ * head_size 32, 64 or 128; page_size 16, 32, 64, 128 or 256 positions;
+ * n_pages * page_size below 2^31. */
+typedef struct {
+    void *keys, *values;
+    int32_t dtype;               /* yl_dtype */
+    uint32_t n_pages, page_size, n_kv_heads, head_size;
+} yl_paged_cache;
+
+/* The rows of one call and the sequences they belong to.  Sequence s owns
+ * rows row_start[s] .. row_start[s + 1] - 1 (row_start ascends; rows outside
+ * every sequence are left as they were), the last of them at position
+ * kv_len[s] - 1, the others at the positions before it.  row_start NULL: row
+ * s is sequence s's only one (n_rows == n_seqs).
+ * Positions 0 .. prefix_len - 1 are every sequence's and lie on prefix_pages;
+ * position prefix_len + i of sequence s lies on page
+ * page_table[s][i / page_size].  An entry that names no page (negative, or not
+ * below n_pages) and a position past the table hold nothing: they are not
+ * written and nothing attends to them. */
+typedef struct {
+    uint32_t n_seqs, n_rows;
+    uint32_t max_pages;            /* entries of a sequence in page_table */
+    uint32_t max_len;              /* an upper bound of kv_len (0: what prefix and table hold): it
+                                      decides how the work is split; longer ones are right, slower */
+    const int32_t *page_table;     /* device [n_seqs][max_pages] */
+    const uint32_t *kv_len;        /* device [n_seqs] */
+    const uint32_t *row_start;     /* device [n_seqs + 1], or NULL */
+    uint32_t prefix_len;
+    const int32_t *prefix_pages;   /* device [ceil(prefix_len / page_size)]; unused without a prefix */
+} yl_paged_batch;
+
+/* Which elements of a head a rotation turns together: (2i, 2i + 1), as
+ * yl_rope_gguf; (i, i + head_size / 2), the HF layout; none. */
+#define YL_ROPE_NONE     -1
+#define YL_ROPE_ADJACENT  0
+#define YL_ROPE_HALF      1
+
+/* The tables that the rotations read, on the host: cos_t and sin_t
+ * [rows][head_size / 2] for positions 0 .. rows - 1.  YL_ROPE_ADJACENT:
+ * rope_gguf's angles (util.rs:653-718) with p's scaling; YL_ROPE_HALF:
+ * util::rope's (util.rs:589-635), of which p gives head_size, rope_theta and,
+ * as original_ctx_len, the model's context length. */
+yl_status yl_rope_table(const yl_rope_params *p, int32_t pairs, uint32_t rows, float *cos_t, float *sin_t);
+
+/* Rotates the rows' queries and keys to their positions, writes the queries
+ * to q_out and the keys and values, rounded to the cache's type, to their
+ * pages.  q, q_out [n_rows] rows of n_heads * head_size floats, k and v
+ * [n_rows] rows of n_kv_heads * head_size (device), rows q_ld, q_out_ld, k_ld,
+ * v_ld floats apart: q, k and v may be parts of one fused row.  q_out may be
+ * q (with q_ld) but not overlap the inputs otherwise; q and q_out NULL: keys
+ * and values only.  cos_t and sin_t (device, [rope_rows][head_size / 2]): a
+ * pair (a, b) becomes (a cos - b sin, a sin + b cos), each product and sum
+ * rounded on its own, the same bits as yl_rope_gguf's; YL_ROPE_NONE: copied
+ * as it is.  A row at a negative position, or at one not below rope_rows
+ * while there is a rotation, is passed over; one below prefix_len writes q_out
+ * only (prefix pages are shared).  No two rows of a call may hold the same
+ * slot of a page. */
+yl_status yl_paged_append(const yl_paged_cache *cache, const yl_paged_batch *batch, uint32_t n_heads, float *q_out,
+                          size_t q_out_ld, const float *q, size_t q_ld, const float *k, size_t k_ld, const float *v,
+                          size_t v_ld, int32_t pairs, const float *cos_t, const float *sin_t, uint32_t rope_rows,
+                          void *stream);
+
+/* Causal attention over the pages: a row of position p attends to positions
+ * 0 .. p that its sequence or the prefix holds, query head h to kv head
+ * h / (n_heads / n_kv_heads); out = sum_j e_j v_j / sum_j e_j with
+ * e_j = exp(attn_scale q . k_j - max).  A row that has nothing to attend to
+ * gets zeros.  Whatever lies at positions a row does not attend to takes no
+ * part.  q, out: [n_rows] rows of n_heads * head_size floats (device), q_ld
+ * and out_ld floats apart; out may be q (with q_ld) but not overlap it
+ * otherwise.  A prefix is read once for all sequences.  workspace (device,
+ * 16-byte aligned): yl_paged_attention_workspace bytes, its contents of no
+ * matter before and after; calls that may run at the same time need one each.
+ * Smaller: YL_ERR_RANGE. */
+size_t yl_paged_attention_workspace(const yl_paged_cache *cache, const yl_paged_batch *batch, uint32_t n_heads);
+yl_status yl_paged_attention(float *out, size_t out_ld, const float *q, size_t q_ld, const yl_paged_cache *cache,
+                             const yl_paged_batch *batch, uint32_t n_heads, float attn_scale, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
+/* Scores rows of logits [rows][vocab] of `dtype` (device, ld elements apart):
+ *   logprob[r] = x[tokens[r]] - log sum_i exp(x[i])  (-inf for an id that is
+ *                not below vocab); tokens and logprob both NULL: not wanted
+ *   entropy[r] = -sum_i p_i log p_i (nullable)
+ *   top_ids[r][j], top_logprobs[r][j]: the `top` (0 .. 32, at most vocab) most
+ *                probable ids in falling order, equal values by rising id
+ * Logits of -inf have probability 0.  A row of nothing else: logprob and
+ * top_logprobs -inf, entropy 0, ids from 0 on.  A row that holds NaN or +inf:
+ * NaN in all of them, ids with NaN last.  workspace as above, of
+ * yl_token_logprobs_workspace bytes. */
+size_t yl_token_logprobs_workspace(size_t rows, size_t vocab, uint32_t top);
+yl_status yl_token_logprobs(const void *logits, int32_t dtype, size_t rows, size_t vocab, size_t ld,
+                            const uint32_t *tokens, float *logprob, float *entropy, uint32_t top, uint32_t *top_ids,
+                            float *top_logprobs, void *workspace, size_t workspace_bytes, void *stream);
+
 /* --------------------------------------------------- model and session */
 
 typedef struct {                 /* TransformerShape, base_transformer.rs:25-44 */

@@ -9,10 +9,12 @@ reference's API over it:
                                                        base_transformer.rs
   load_transformer, load_transformer_ffi, infer_ffi    lib.rs, README.md
   Tokenizer, Sampler                                   tokenizer.rs, sampler.rs
-  ops.*                                                util.rs, forward.rs
+  ops.*                                                util.rs, forward.rs, and the paged
+                                                       cache and scoring ops, which the
+                                                       reference does not have
   synth                                                seeded GGUF models
 """
-from ._lib import LIB_PATH, YlError, check, lib
+from ._lib import DTYPES, LIB_PATH, ROPE_PAIRS, PagedBatchDesc, PagedCacheDesc, YlError, check, lib
 from .device import DeviceBuffer, device_count
 from .tokenizer import Sampler, Tokenizer, pretokenize
 from .transformer import (InferenceSession, Transformer, TransformerLlamaGguf, infer_ffi, infer_reset,
@@ -23,5 +25,5 @@ __all__ = [
     "LIB_PATH", "YlError", "check", "lib", "DeviceBuffer", "device_count", "InferenceSession", "Transformer",
     "TransformerLlamaGguf", "infer_ffi", "load_transformer", "load_transformer_ffi", "QuantizedWeight",
     "WeightFormat", "matmul", "matmul_device", "quantize", "quantize_device", "Sampler", "Tokenizer", "pretokenize",
-    "infer_reset", "infer_set_max_tokens",
+    "infer_reset", "infer_set_max_tokens", "DTYPES", "ROPE_PAIRS", "PagedBatchDesc", "PagedCacheDesc",
 ]

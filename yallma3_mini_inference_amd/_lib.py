@@ -32,7 +32,13 @@ EXPORTS = [
     "yl_infer_reset", "yl_tokenizer_load", "yl_tokenizer_free", "yl_model_tokenizer", "yl_tokenizer_vocab_size",
     "yl_tokenize", "yl_detokenize", "yl_chat_template", "yl_chat_prompt", "yl_pretokenize", "yl_sampler_new",
     "yl_sampler_sample", "yl_sampler_free", "yl_generate_text", "yl_weight_upload_f16", "yl_matmul_f32",
+    "yl_rope_table", "yl_paged_append", "yl_paged_attention_workspace", "yl_paged_attention",
+    "yl_token_logprobs_workspace", "yl_token_logprobs",
 ]
+
+# yl_dtype, and which elements of a head a rotation turns together (YL_ROPE_*)
+DTYPES = {"f32": 0, "f16": 1, "bf16": 2}
+ROPE_PAIRS = {"none": -1, "adjacent": 0, "half": 1}
 
 
 class YlError(RuntimeError):
@@ -56,6 +62,19 @@ class Shape(C.Structure):
                 ("rope_ext_factor", C.c_float), ("rope_attn_factor", C.c_float),
                 ("rope_original_ctx_len", C.c_uint32), ("attention_scale", C.c_float),
                 ("weight_format", C.c_int32)]
+
+
+class PagedCacheDesc(C.Structure):
+    """yl_paged_cache: a pool of pages, keys and values [n_pages][n_kv_heads][page_size][head_size]."""
+    _fields_ = [("keys", C.c_void_p), ("values", C.c_void_p), ("dtype", C.c_int32), ("n_pages", C.c_uint32),
+                ("page_size", C.c_uint32), ("n_kv_heads", C.c_uint32), ("head_size", C.c_uint32)]
+
+
+class PagedBatchDesc(C.Structure):
+    """yl_paged_batch: the rows of one call and their sequences (device arrays)."""
+    _fields_ = [("n_seqs", C.c_uint32), ("n_rows", C.c_uint32), ("max_pages", C.c_uint32), ("max_len", C.c_uint32),
+                ("page_table", C.c_void_p), ("kv_len", C.c_void_p), ("row_start", C.c_void_p),
+                ("prefix_len", C.c_uint32), ("prefix_pages", C.c_void_p)]
 
 
 class SynthConfig(C.Structure):
@@ -161,6 +180,14 @@ def lib():
         "yl_generate_text": (st, [vp, vp, vp, vp, sz, u32, C.POINTER(vp), vp, sz, C.POINTER(sz)]),
         "yl_weight_upload_f16": (vp, [vp, sz, sz]),
         "yl_matmul_f32": (st, [vp, vp, sz, vp, sz, sz, vp]),
+        "yl_rope_table": (st, [C.POINTER(RopeParams), st, u32, vp, vp]),
+        "yl_paged_append": (st, [C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), u32, vp, sz, vp, sz, vp, sz, vp, sz,
+                                 st, vp, vp, u32, vp]),
+        "yl_paged_attention_workspace": (sz, [C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), u32]),
+        "yl_paged_attention": (st, [vp, sz, vp, sz, C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), u32, f32, vp,
+                                    sz, vp]),
+        "yl_token_logprobs_workspace": (sz, [sz, sz, u32]),
+        "yl_token_logprobs": (st, [vp, st, sz, sz, sz, vp, vp, vp, u32, vp, vp, vp, sz, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

@@ -26,6 +26,7 @@
 #include <algorithm>
 #include <memory>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -1634,6 +1635,21 @@ yl_status yl_rope_gguf(const yl_rope_params* p, float* q, float* k, size_t batch
     if (ds) hipFree(ds);
     if (dst) hipFree(dst);
     return e == hipSuccess ? YL_OK : hip_fail(e, "rope");
+}
+
+yl_status yl_rope_table(const yl_rope_params* p, int32_t pairs, uint32_t rows, float* cos_t, float* sin_t) {
+    if (!p || !p->head_size || p->head_size % 2 || p->head_size > 1024 || (rows && (!cos_t || !sin_t)) ||
+        (pairs != YL_ROPE_ADJACENT && pairs != YL_ROPE_HALF)) {
+        set_error("rope_table: an even head size (at most 1024), pairs adjacent or half, and tables to fill");
+        return YL_ERR_ARG;
+    }
+    try {
+        if (pairs == YL_ROPE_ADJACENT) rope_table(*p, 0, rows, cos_t, sin_t);
+        else rope_table_hf(p->rope_theta, (int)p->head_size, p->original_ctx_len, rows, cos_t, sin_t);
+    } catch (const std::bad_alloc&) {
+        return YL_ERR_NOMEM;
+    }
+    return YL_OK;
 }
 
 }  // extern "C"
