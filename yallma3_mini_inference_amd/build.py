@@ -20,7 +20,7 @@ OBJ = os.path.join(PKG, "_build")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIB_DIR, "libyallma3_amd.so")
 
-SOURCES = ["yl_kernels.hip", "yl_gemv.hip", "yl_gemm.hip", "yl_attn.hip", "yl_attn_split.hip", "yl_pattn.hip", "yl_logits.hip", "yl_f16.hip", "yl_q8g.hip", "yl_paged.hip", "yl_logprobs.hip", "yl_model.hip",
+SOURCES = ["yl_kernels.hip", "yl_gemv.hip", "yl_gemm.hip", "yl_attn.hip", "yl_attn_split.hip", "yl_pattn.hip", "yl_logits.hip", "yl_f16.hip", "yl_q8g.hip", "yl_paged.hip", "yl_paged_attn.hip", "yl_logprobs.hip", "yl_model.hip",
            "yl_gguf.cpp", "yl_synth.cpp", "yl_tokenizer.cpp", "yl_jinja.cpp", "yl_loaders.cpp"]
 ARCH = os.environ.get("YL_OFFLOAD_ARCH", "gfx950")
 

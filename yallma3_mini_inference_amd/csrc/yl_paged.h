@@ -84,4 +84,9 @@ YL_HD bool paged_place(const PagedArgs& a, int s, int64_t pos, int* page, int* s
     return *page >= 0;
 }
 
+#if defined(YALLMA3_H)
+// The kernels' arguments from a caller's descriptions; YL_OK, or the refusal.
+yl_status paged_args(const yl_paged_cache* c, const yl_paged_batch* b, uint32_t n_heads, PagedArgs* a);
+#endif
+
 }  // namespace yl

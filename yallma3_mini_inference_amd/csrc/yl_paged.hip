@@ -1,5 +1,5 @@
 // yl_paged.hip -- a K/V cache in pages that many sequences share: appending
-// rows to it with the position rotation on the way, and attention over it.
+// rows to it with the position rotation on the way (yl_paged_attn.hip reads it).
 // No counterpart in the reference, which holds one conversation.
 #include <hip/hip_runtime.h>
 
@@ -65,68 +65,6 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
             static_cast<C*>(a.p.values)[paged_offset(a.p, page, i / hd, slot) + i % hd] = (C)a.v[(size_t)row * a.v_ld + i];
 }
 
-// ---------------------------------------------------------------- attention
-
-// One workgroup per (row, query head): scores of 256 positions at a time, a
-// position per thread, and the running maximum, sum and output.
-template <typename C, int HD>
-__global__ __launch_bounds__(256) void k_paged_attention(PagedArgs a, float* out, size_t out_ld, const float* q,
-                                                         size_t q_ld, float scale) {
-    constexpr int NP = 256 / HD;     // positions whose values are added at once
-    __shared__ float qs[HD], e[256], red[4], acc[NP][HD];
-    __shared__ int pg[256];
-    const int row = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int s = paged_seq_of_row(a, row);
-    if (s < 0) return;
-    int first, end;
-    paged_rows(a, s, &first, &end);
-    if (row < first || row >= end) return;
-    const int limit = paged_limit(a, paged_row_pos(a.kv_len[s], end, row));
-    const int kvh = h / (a.n_heads / a.n_kv), slots = (1 << a.page_shift) - 1;
-    if (tid < HD) qs[tid] = q[(size_t)row * q_ld + (size_t)h * HD + tid] * scale;
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (int p0 = 0; p0 < limit; p0 += 256) {
-        int page = -1, slot = 0;
-        const bool held = p0 + tid < limit && paged_place(a, s, p0 + tid, &page, &slot);
-        pg[tid] = held ? page : -1;
-        float sc = -INFINITY;
-        if (held) {
-            const C* k = static_cast<const C*>(a.keys) + paged_offset(a, page, kvh, slot);
-            sc = 0.0f;
-            for (int d = 0; d < HD; d++) sc = fmaf(qs[d], (float)k[d], sc);
-        }
-        float mx = sc;
-        for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-        if (lane == 0) red[wave] = mx;
-        __syncthreads();
-        mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.0f : m_new;
-        const float alpha = expf(m - base);
-        e[tid] = held ? expf(sc - base) : 0.0f;
-        __syncthreads();
-        float sum = 0.0f, add = 0.0f;
-        for (int j = tid / HD; j < 256; j += NP) {
-            if (pg[j] < 0) continue;
-            const int pos = p0 + j, i = pos < a.prefix_len ? pos : pos - a.prefix_len;
-            add = fmaf(e[j], (float)static_cast<const C*>(a.values)[paged_offset(a, pg[j], kvh, i & slots) + tid % HD], add);
-            sum += e[j];
-        }
-        l = l * alpha + sum;
-        o = o * alpha + add;
-        m = m_new;
-        __syncthreads();
-    }
-    acc[tid / HD][tid % HD] = o;
-    if (tid % HD == 0) e[tid / HD] = l;
-    __syncthreads();
-    if (tid < HD) {
-        float sum = 0.0f, add = 0.0f;
-        for (int j = 0; j < NP; j++) { sum += e[j]; add += acc[j][tid]; }
-        out[(size_t)row * out_ld + (size_t)h * HD + tid] = limit > 0 && sum != 0.0f ? add / sum : 0.0f;
-    }
-}
-
 // ------------------------------------------------------------- host entries
 
 namespace {
@@ -136,7 +74,8 @@ yl_status refuse(const char* what, yl_status st = YL_ERR_ARG) {
     return st;
 }
 
-// Fills `a` from the caller's descriptions; YL_OK or the refusal.
+}  // namespace
+
 yl_status paged_args(const yl_paged_cache* c, const yl_paged_batch* b, uint32_t n_heads, PagedArgs* a) {
     if (!c || !b) return refuse("paged: no cache or no batch");
     if (c->dtype != YL_T_F32 && c->dtype != YL_T_F16 && c->dtype != YL_T_BF16)
@@ -149,9 +88,9 @@ yl_status paged_args(const yl_paged_cache* c, const yl_paged_batch* b, uint32_t 
         return refuse("paged: n_heads (at most 1024) is a multiple of n_kv_heads");
     if (!c->keys || !c->values || ((uintptr_t)c->keys | (uintptr_t)c->values) % 16)
         return refuse("paged: keys and values have to be there, 16-byte aligned");
-    if ((uint64_t)b->n_rows * n_heads >= (1ull << 31) || b->n_seqs >= (1u << 24) ||
+    if ((uint64_t)b->n_rows * n_heads >= (1ull << 24) || (uint64_t)b->n_seqs * n_heads >= (1ull << 24) ||
         (uint64_t)b->prefix_len + (uint64_t)b->max_pages * c->page_size >= (1ull << 31))
-        return refuse("paged: n_rows * n_heads and a sequence's capacity below 2^31, n_seqs below 2^24", YL_ERR_RANGE);
+        return refuse("paged: n_rows * n_heads and n_seqs * n_heads below 2^24, a sequence's capacity below 2^31", YL_ERR_RANGE);
     if (!b->row_start && b->n_rows != b->n_seqs) return refuse("paged: without row_start there is one row per sequence");
     if (b->n_rows && b->n_seqs && (!b->kv_len || (b->max_pages && !b->page_table)))
         return refuse("paged: kv_len and page_table have to be there");
@@ -162,11 +101,7 @@ yl_status paged_args(const yl_paged_cache* c, const yl_paged_batch* b, uint32_t 
     return YL_OK;
 }
 
-template <typename C>
-void launch_attention_hd(const PagedArgs& a, float* out, size_t out_ld, const float* q, size_t q_ld, float scale, hipStream_t s) {
-    auto k = a.hd == 32 ? k_paged_attention<C, 32> : a.hd == 64 ? k_paged_attention<C, 64> : k_paged_attention<C, 128>;
-    hipLaunchKernelGGL(k, dim3(a.n_rows, a.n_heads), dim3(256), 0, s, a, out, out_ld, q, q_ld, scale);
-}
+namespace {
 
 yl_status launched(const char* what) {
     const hipError_t e = hipGetLastError();
@@ -203,31 +138,6 @@ yl_status yl_paged_append(const yl_paged_cache* cache, const yl_paged_batch* bat
     auto kern = cache->dtype == YL_T_F32 ? k_paged_append<float> : cache->dtype == YL_T_F16 ? k_paged_append<_Float16> : k_paged_append<__bf16>;
     hipLaunchKernelGGL(kern, dim3(batch->n_rows), dim3(256), 0, (hipStream_t)stream, a);
     return launched("paged_append launch");
-}
-
-size_t yl_paged_attention_workspace(const yl_paged_cache* cache, const yl_paged_batch* batch, uint32_t n_heads) {
-    return 0;
-}
-
-yl_status yl_paged_attention(float* out, size_t out_ld, const float* q, size_t q_ld, const yl_paged_cache* cache,
-                             const yl_paged_batch* batch, uint32_t n_heads, float attn_scale, void* workspace,
-                             size_t workspace_bytes, void* stream) {
-    PagedArgs a{};
-    const yl_status st = paged_args(cache, batch, n_heads, &a);
-    if (st != YL_OK) return st;
-    const size_t need = yl_paged_attention_workspace(cache, batch, n_heads);
-    if (!batch->n_rows || !batch->n_seqs) return YL_OK;
-    if (!out || !q) return refuse("paged_attention: no q or no out");
-    const size_t att = (size_t)n_heads * cache->head_size;
-    if (q_ld < att || out_ld < att) return refuse("paged_attention: rows further apart than they are long");
-    if (q == out && q_ld != out_ld) return refuse("paged_attention: in place, q_ld and out_ld are the same");
-    if (need && (!workspace || (uintptr_t)workspace % 16)) return refuse("paged_attention: the workspace has to be there, 16-byte aligned");
-    if (workspace_bytes < need) return refuse("paged_attention: the workspace is smaller than yl_paged_attention_workspace says", YL_ERR_RANGE);
-    hipStream_t s = (hipStream_t)stream;
-    if (cache->dtype == YL_T_F32) launch_attention_hd<float>(a, out, out_ld, q, q_ld, attn_scale, s);
-    else if (cache->dtype == YL_T_F16) launch_attention_hd<_Float16>(a, out, out_ld, q, q_ld, attn_scale, s);
-    else launch_attention_hd<__bf16>(a, out, out_ld, q, q_ld, attn_scale, s);
-    return launched("paged_attention launch");
 }
 
 }  // extern "C"
