@@ -58,16 +58,19 @@ template <> struct Type<_Float16> {
     // two values -> their parts, packed
     static __device__ __forceinline__ void cut(float a, float b, uint32_t part[2]) {
         const h2 hi = __builtin_convertvector(vf2{a, b}, h2);
-        const h2 lo = __builtin_convertvector((vf2{a - (float)hi[0], b - (float)hi[1]}), h2);
         part[0] = __builtin_bit_cast(uint32_t, hi);
-        part[1] = __builtin_bit_cast(uint32_t, lo);
+        // a - hi, b - hi rounded to f16: one mixed-precision fma each
+        asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]\n\tv_fma_mixhi_f16 %0, %1, -1.0, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+            : "=&v"(part[1]) : "v"(part[0]), "v"(a), "v"(b));
     }
     // the power of two that brings a row of q to [2^9, 2^10)
     static __device__ __forceinline__ int exponent(float amax) {
         return amax > 0.0f && amax < INFINITY ? min(9 - __builtin_amdgcn_frexp_expf(amax), 110) : 0;
     }
-    static __device__ __forceinline__ bool finite(uint32_t two) { return (two & 0x7c00u) != 0x7c00u && (two & 0x7c000000u) != 0x7c000000u; }
-    static __device__ __forceinline__ float widen(uint32_t two, int half) { return f16_to_f32((uint16_t)(half ? two >> 16 : two)); }
+    // all bits of the halves that are no numbers
+    static __device__ __forceinline__ uint32_t not_finite(uint32_t two) {
+        return ((two & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((two & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
+    }
 };
 template <> struct Type<__bf16> {
     static constexpr int kParts = 3, kTiles = 2;
@@ -87,12 +90,14 @@ template <> struct Type<__bf16> {
         }
     }
     static __device__ __forceinline__ int exponent(float) { return 0; }
-    static __device__ __forceinline__ bool finite(uint32_t two) { return (two & 0x7f80u) != 0x7f80u && (two & 0x7f800000u) != 0x7f800000u; }
-    static __device__ __forceinline__ float widen(uint32_t two, int half) { return __uint_as_float(half ? two & 0xffff0000u : two << 16); }
+    static __device__ __forceinline__ uint32_t not_finite(uint32_t two) {
+        return ((two & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((two & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+    }
 };
 template <> struct Type<float> {
     static constexpr int kParts = 1, kTiles = 1;
     static constexpr float kBias = 0.0f;
+    static __device__ __forceinline__ uint32_t not_finite(uint32_t x) { return (x & 0x7f800000u) == 0x7f800000u ? ~0u : 0u; }
     static __device__ __forceinline__ int exponent(float) { return 0; }
 };
 
@@ -138,10 +143,14 @@ struct PagedAttn {
     float scale_log2;                // attn_scale * log2(e)
     int group;                       // query heads per kv head
     int parts, part0;                // partial results per row and head; the first of this launch's
+    int per_seq;                     // their rows: so many for each sequence, 0: the batch's rows
     int chunk;                       // positions of a split at least
     int splits;
-    float* po;                       // [n_rows * n_heads][parts][hd], unnormalised
-    float2* pml;                     // [n_rows * n_heads][parts]: maximum (base 2), sum; maximum -inf: nothing there
+    int direct;                      // this launch sees all that its rows attend to: it writes `out`
+    int per;                         // row kernel: slots of a sequence, 0: as its rows need
+    int both;                        // sequences are divided between the row kernel and the tile kernel
+    float* po;                       // [row][n_heads][parts][hd], unnormalised
+    float2* pml;                     // [row][n_heads][parts]: maximum (base 2), sum; maximum -inf: nothing there
 };
 
 // A tile of the stacked rows that attend to the same pages.
@@ -154,16 +163,17 @@ struct RowSet {
 // The tile of slot `slot`: sequence s takes slots from floor(row_start[s] *
 // group / 16) + s on, of which it uses one per 16 stacked rows: a sequence's
 // slots always suffice, and are found by a search over row_start alone (64
-// starts per step, one per lane).  False: a slot that nothing uses.
-__device__ __forceinline__ bool tile_of_slot(const PagedAttn& a, int slot, int rows_log2, RowSet* set, int* tile) {
+// starts per step, one per lane).  `per`: that many slots for every sequence
+// instead.  False: a slot that nothing uses.
+__device__ __forceinline__ bool tile_of_slot(const PagedAttn& a, int slot, int rows_log2, int per, RowSet* set, int* tile) {
     const PagedArgs& p = a.p;
     set->entries = p.max_pages;
-    if (!p.row_start) {
-        const int per = (a.group + (1 << rows_log2) - 1) >> rows_log2;
+    if (per) {
         set->seq = slot / per;
         *tile = slot - set->seq * per;
-        set->first = set->seq;
-        set->rows = 1;
+        int end;
+        paged_rows(p, set->seq, &set->first, &end);
+        set->rows = end - set->first;
     } else {
         const int lane = threadIdx.x & 63;
         const auto base = [&](int s) {
@@ -206,83 +216,81 @@ __device__ __forceinline__ int limit_of_row(const PagedAttn& a, const RowSet& se
 
 constexpr int kRowTile = 16;
 
-// One tile of 16 stacked rows over one split of the positions, the positions
-// dealt to four wavefronts in steps of 16 kTiles.  K and V go from memory to
-// registers in the operands' order; the next step's keys are loaded while
-// this one is computed.  Bound by memory: with few rows per kv head a byte of
-// the cache meets about as many operations as the matrix cores need.
+// Stacked rows of a sequence (tokens times heads per kv head) up to which the
+// row kernel takes it.
+constexpr int kRowKernelRows = 32;
+__device__ __forceinline__ bool row_kernel_takes(int rows, int group) { return (int64_t)rows * group <= kRowKernelRows; }
+inline int row_kernel_tokens(int group) { return std::max(1, kRowKernelRows / group); }
+
+// 16 stacked rows in a wavefront: lane (c, g) holds of row c the query parts,
+// the sums of dimensions (4g + i) NJ + j and those of its positions.
 template <typename C, int HD>
-__global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int prefix) {
+struct Tile {
     using T = Type<C>;
-    constexpr int NT = T::kTiles, NP = T::kParts, STEP = 16 * NT;
-    constexpr bool F32 = sizeof(C) == 4;
-    constexpr int NJ = HD / 16;                       // dimensions per lane of V, tiles of O^T
-    constexpr int NK = F32 ? HD / 16 : HD / 32;       // 16-byte loads of a key per lane
-    constexpr int VW = NJ * (int)sizeof(C) / 4;       // words of a V row per lane
-    constexpr int LD = HD + 4;
-    __shared__ __align__(16) float so[4][kRowTile][LD];
-    __shared__ float sm[4][kRowTile], sl[4][kRowTile];
+    static constexpr bool F32 = sizeof(C) == 4;
+    static constexpr int NT = T::kTiles, NP = T::kParts, STEP = 16 * NT;
+    static constexpr int NJ = HD / 16;                       // dimensions per lane of V, tiles of O^T
+    static constexpr int NK = F32 ? HD / 16 : HD / 32;       // 16-byte pieces of a key per lane
+    static constexpr int KD = F32 ? 16 : 32, KE = F32 ? 4 : 8;   // dimensions per piece of all lane groups, of one
+    static constexpr int VW = NJ * (int)sizeof(C) / 4;       // words of a V row per lane
+    typedef Words<VW> Value;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int c = lane & 15, g = lane >> 4;
-    const int kvh = blockIdx.x % a.p.n_kv, slot = blockIdx.x / a.p.n_kv, split = blockIdx.y;
-    RowSet set;
-    int tile;
-    if (prefix) {
-        set = RowSet{a.p.prefix_pages, (a.p.prefix_len + (1 << a.p.page_shift) - 1) >> a.p.page_shift, 0, a.p.n_rows, -1};
-        tile = slot;
-    } else if (!tile_of_slot(a, slot, 4, &set, &tile)) {
-        return;
-    }
-
-    // this lane's row: stacked row tile * 16 + c
-    const int stacked = tile * kRowTile + c;
-    const bool live = stacked < set.rows * a.group;
-    const int row = set.first + (live ? stacked / a.group : 0), head = kvh * a.group + (live ? stacked % a.group : 0);
-    int lim = live ? limit_of_row(a, set, row) : 0;
-    int most = lim;                                   // the tile's longest row
-    for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor(most, o, 64));
-    most = __builtin_amdgcn_readfirstlane(min((int64_t)most, (int64_t)set.entries << a.p.page_shift));
-    const bool whole = a.splits == 1 && a.parts == 1;   // this workgroup sees all there is
-    int lo = 0, hi = most;
-    if (a.splits > 1) {
-        const int even = (most + a.splits - 1) / a.splits;
-        const int chunk = max(a.chunk, (even + 127) & ~127);
-        lo = (int)min((int64_t)split * chunk, (int64_t)most);
-        hi = min(lo + chunk, most);
-    }
-    const size_t part_at = ((size_t)row * a.p.n_heads + head) * a.parts + a.part0 + split;
-    if (lo >= hi && !whole) {
-        if (live && wave == 0 && g == 0) a.pml[part_at] = make_float2(-INFINITY, 0.0f);
-        return;
-    }
-    if (!live) lim = most;                            // (spare rows follow the longest, so that they need no masks)
-    int least = lim;
-    for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o, 64));
-    least = __builtin_amdgcn_readfirstlane(least);
-
-    // q of the lane's row, cut into parts, in the order of the keys' loads
+    int row, head, lim;              // lim: positions below it are attended to
+    bool live;
+    float m, l, unscale;
     u4 qf[NP][NK];
-    float unscale = a.scale_log2;
-    {
-        const float* qr = a.q + (size_t)row * a.q_ld + (size_t)head * HD + (F32 ? 4 * g : 8 * g);
-        f4u v[NK][F32 ? 1 : 2];
+    vf4 acc[NJ];
+
+    // Places the tile at stacked rows from `stacked` on.
+    __device__ __forceinline__ void place(const PagedAttn& a, const RowSet& set, int stacked, int kvh, int c) {
+        const int r = stacked + c;
+        live = r < set.rows * a.group;
+        row = set.first + (live ? r / a.group : 0);
+        head = kvh * a.group + (live ? r % a.group : 0);
+        lim = live ? limit_of_row(a, set, row) : 0;
+        if (live) lim = (int)min((int64_t)lim, (int64_t)set.entries << a.p.page_shift);
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NJ; j++) acc[j] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // The tile's longest and shortest rows (spare rows follow the longest, so that they need no masks).
+    __device__ __forceinline__ void reach(int* most, int* least) {
+        int x = lim;
+        for (int o = 1; o < 16; o <<= 1) x = max(x, __shfl_xor(x, o, 64));
+        *most = __builtin_amdgcn_readfirstlane(x);
+        if (!live) lim = *most;
+        x = lim;
+        for (int o = 1; o < 16; o <<= 1) x = min(x, __shfl_xor(x, o, 64));
+        *least = __builtin_amdgcn_readfirstlane(x);
+    }
+    // q of the lane's row, cut into parts, in the order of the keys' pieces
+    __device__ __forceinline__ void load_q(const PagedAttn& a, int g) {
+        const float* qr = a.q + (size_t)row * a.q_ld + (size_t)head * HD + KE * g;
+        f4u v[NK][KE / 4];
         float amax = 0.0f;
 #pragma unroll
         for (int k = 0; k < NK; k++)
 #pragma unroll
-            for (int e = 0; e < (F32 ? 1 : 2); e++) {
-                v[k][e] = *reinterpret_cast<const f4u*>(qr + k * (F32 ? 16 : 32) + 4 * e);
+            for (int e = 0; e < KE / 4; e++) {
+                v[k][e] = *reinterpret_cast<const f4u*>(qr + k * KD + 4 * e);
                 if (!live) v[k][e] = f4u{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int i = 0; i < 4; i++) amax = fmaxf(amax, fabsf(v[k][e][i]));
             }
+        // scores times `unscale` > 0 are the exponents: q takes the sign (or the zero) of the scale
+        const float sign = a.scale_log2 < 0.0f ? -1.0f : a.scale_log2 == 0.0f ? 0.0f : 1.0f;
+        unscale = a.scale_log2 == 0.0f ? 1.0f : fabsf(a.scale_log2);
+#pragma unroll
+        for (int k = 0; k < NK; k++)
+#pragma unroll
+            for (int e = 0; e < KE / 4; e++) v[k][e] *= sign;
         if constexpr (F32) {
 #pragma unroll
             for (int k = 0; k < NK; k++) qf[0][k] = __builtin_bit_cast(u4, v[k][0]);
         } else {
             const int ex = T::exponent(group_max16(amax));
-            if (ex) unscale = __builtin_amdgcn_ldexpf(a.scale_log2, -ex);
+            if (ex) unscale = __builtin_amdgcn_ldexpf(unscale, -ex);
 #pragma unroll
             for (int k = 0; k < NK; k++)
 #pragma unroll
@@ -294,101 +302,49 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
                 }
         }
     }
-
-    vf4 acc[NJ];
+    // scores of the step's positions, before `unscale` (the tiles' chains of products side by side)
+    __device__ __forceinline__ void scores(const u4 kc[NT][NK], float s[NT][4]) const {
+        vf4 d[NT];
 #pragma unroll
-    for (int j = 0; j < NJ; j++) acc[j] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f;                    // l: this lane's positions only
-
-    const C* keys = static_cast<const C*>(a.p.keys);
-    const C* values = static_cast<const C*>(a.p.values);
-    const int slots = (1 << a.p.page_shift) - 1;
-    const int steps = (hi - lo + STEP - 1) / STEP;
-    // Pages of this wavefront's next 64 tiles, one per lane (-1: none, or past hi).
-    const auto pages_from = [&](int step) {
-        const int at = lo + STEP * (step + 4 * (lane / NT)) + 16 * (lane % NT);
-        return at < hi ? paged_page(set.pages[at >> a.p.page_shift], a.p.n_pages) : -1;
-    };
-    int page_reg = pages_from(wave), page_n = 0;
-    const auto tile_page = [&](int t) { return __builtin_amdgcn_readlane(page_reg, page_n * NT + t); };
-    u4 kf[2][NT][NK];
-    const auto load_keys = [&](int step, int page[NT], u4 f[NT][NK]) {
+        for (int t = 0; t < NT; t++) d[t] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (F32) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            page[t] = tile_page(t);
-            const C* k = keys + paged_offset(a.p, max(page[t], 0), kvh, (lo + STEP * step + 16 * t) & slots) + (size_t)c * HD + (F32 ? 4 * g : 8 * g);
+            for (int k = 0; k < NK; k++)
 #pragma unroll
-            for (int i = 0; i < NK; i++) f[t][i] = *reinterpret_cast<const u4*>(k + i * (F32 ? 16 : 32));
-        }
-    };
-
-    int page[NT], next_page[NT] = {};
-    const auto step_on = [&](int step, u4 (&kc)[NT][NK], u4 (&kn)[NT][NK]) {
-        // values of this step, keys of the next
-        Words<VW> vr[NT][4];
+                for (int e = 0; e < 4; e++)
+                    d[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kc[0][k][e]), __uint_as_float(qf[0][k][e]), d[0], 0, 0, 0);
+        } else {
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const C* v = values + paged_offset(a.p, max(page[t], 0), kvh, ((lo + STEP * step + 16 * t) & slots) + 4 * g) + (size_t)c * NJ;
-#pragma unroll
-            for (int i = 0; i < 4; i++) vr[t][i] = load_words<VW>(v + (size_t)i * HD);
-        }
-        if (step + 4 < steps) {
-            if (++page_n == 64 / NT) {
-                page_n = 0;
-                page_reg = pages_from(step + 4);
-            }
-            load_keys(step + 4, next_page, kn);
-        }
-        // scores
-        float s[NT][4];
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-            vf4 d = {0.0f, 0.0f, 0.0f, 0.0f};
-            if constexpr (F32) {
+            for (int p = NP - 1; p >= 0; p--)
 #pragma unroll
                 for (int k = 0; k < NK; k++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        d = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kc[t][k][e]), __uint_as_float(qf[0][k][e]), d, 0, 0, 0);
-            } else {
+                    for (int t = 0; t < NT; t++) d[t] = T::mul(kc[t][k], qf[p][k], d[t]);
+        }
 #pragma unroll
-                for (int p = NP - 1; p >= 0; p--)
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int k = 0; k < NK; k++) d = T::mul(kc[t][k], qf[p][k], d);
+            for (int i = 0; i < 4; i++) s[t][i] = d[t][i];
+    }
+    // Takes positions that are not there, or past the row, out of the scores.
+    __device__ __forceinline__ void mask(float s[NT][4], int p0, int hi, const int page[NT], int g) const {
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int pos = p0 + 16 * t + 4 * g + i;
+                if (page[t] < 0 || pos >= min(lim, hi)) s[t][i] = -INFINITY;
             }
-#pragma unroll
-            for (int i = 0; i < 4; i++) s[t][i] = d[i] * unscale;
-        }
-        // positions that some row does not attend to
-        const int p0 = lo + STEP * step;
-        bool edge = p0 + STEP > min(least, hi);
-#pragma unroll
-        for (int t = 0; t < NT; t++) edge = edge || page[t] < 0;
-        bool odd = false;      // a value that is no number at a position that some rows attend to
-        if (edge) {
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int pos = p0 + 16 * t + 4 * g + i;
-                    const bool held = page[t] >= 0 && pos < hi;
-                    if (!held || pos >= lim) s[t][i] = -INFINITY;
-#pragma unroll
-                    for (int w = 0; w < VW; w++) {
-                        if (!held) vr[t][i].w[w] = 0u;
-                        if constexpr (F32) odd = odd || (vr[t][i].w[w] & 0x7f800000u) == 0x7f800000u;
-                        else odd = odd || !T::finite(vr[t][i].w[w]);
-                    }
-                }
-            odd = __ballot(odd) != 0 && p0 + STEP > least;
-        }
+    }
+    // scores -> weights, under a maximum that is raised where it has to be
+    __device__ __forceinline__ void weigh(float s[NT][4]) {
         float mx = s[0][0];
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[t][i]);
-        if (__ballot(mx > m + kSlack)) {              // (m = -inf: any score raises it)
-            const float m_new = fmaxf(m, group_max16(mx));
+        if (__ballot(mx * unscale > m + kSlack)) {    // (m = -inf: any score raises it)
+            const float m_new = fmaxf(m, group_max16(mx) * unscale);
             const float alpha = m_new == m ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
             l *= alpha;
 #pragma unroll
@@ -400,33 +356,22 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
         for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                s[t][i] = __builtin_amdgcn_exp2f(s[t][i] + back);
+                s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], unscale, back));
                 l += s[t][i];
             }
-        if (odd) {
-            // one position after the other, each only for the rows that attend to it
-            for (int pos = 0; pos < STEP; pos++) {
-                const int t = pos >> 4, from = ((pos >> 2) & 3) * 16 + c, i = pos & 3;
-                float w = 0.0f;
+    }
+    // V^T's operands: of f16 and bf16, dimension j's halves of the 8 positions
+    static __device__ __forceinline__ u4 operand(const Value vr[NT][4], int j) {
+        u4 f;
 #pragma unroll
-                for (int tt = 0; tt < NT; tt++)
-#pragma unroll
-                    for (int ii = 0; ii < 4; ii++) {
-                        const float got = __shfl(s[tt][ii], from, 64);
-                        if (tt == t && ii == i) w = got;
-                    }
-                int pg = page[0];
-#pragma unroll
-                for (int tt = 1; tt < NT; tt++)
-                    if (t == tt) pg = page[tt];
-                if (pg < 0 || p0 + pos >= lim || p0 + pos >= hi) continue;
-                const C* v = values + paged_offset(a.p, pg, kvh, (p0 + pos) & slots) + (size_t)4 * g * NJ;
-#pragma unroll
-                for (int ii = 0; ii < 4; ii++)
-#pragma unroll
-                    for (int j = 0; j < NJ; j++) acc[j][ii] = fmaf(w, (float)v[ii * NJ + j], acc[j][ii]);
-            }
-        } else if constexpr (F32) {
+        for (int d = 0; d < 4; d++)
+            f[d] = __builtin_amdgcn_perm(vr[d >> 1][2 * (d & 1) + 1].w[j >> 1], vr[d >> 1][2 * (d & 1)].w[j >> 1],
+                                         j & 1 ? 0x07060302 : 0x05040100);
+        return f;
+    }
+    // adds the weighted values
+    __device__ __forceinline__ void add(const float s[NT][4], const Value vr[NT][4]) {
+        if constexpr (F32) {
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -441,17 +386,179 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
 #pragma unroll
                 for (int p = 0; p < NP; p++) pf[p][d] = part[p];
             }
+            u4 vf[NJ];
 #pragma unroll
-            for (int j = 0; j < NJ; j++) {
-                u4 vf;
+            for (int j = 0; j < NJ; j++) vf[j] = operand(vr, j);
 #pragma unroll
-                for (int d = 0; d < 4; d++)
-                    vf[d] = __builtin_amdgcn_perm(vr[d >> 1][2 * (d & 1) + 1].w[j >> 1], vr[d >> 1][2 * (d & 1)].w[j >> 1],
-                                                  j & 1 ? 0x07060302 : 0x05040100);
+            for (int p = NP - 1; p >= 0; p--)
 #pragma unroll
-                for (int p = NP - 1; p >= 0; p--) acc[j] = T::mul(vf, pf[p], acc[j]);
+                for (int j = 0; j < NJ; j++) acc[j] = T::mul(vf[j], pf[p], acc[j]);
+        }
+    }
+    // Adds the values that are no numbers (clear_values has taken them out)
+    // where rows differ in what they attend to: as 0 times one of them is no
+    // number either, only to the rows that attend to its position.
+    __device__ __forceinline__ void add_odd(const PagedAttn& a, const float s[NT][4], int p0, int hi, const int page[NT], int kvh, int c, int g) {
+        const int slots = (1 << a.p.page_shift) - 1;
+        for (int pos = 0; pos < STEP; pos++) {
+            const int t = pos >> 4, from = ((pos >> 2) & 3) * 16 + c, i = pos & 3;
+            float w = 0.0f;
+#pragma unroll
+            for (int tt = 0; tt < NT; tt++)
+#pragma unroll
+                for (int ii = 0; ii < 4; ii++) {
+                    const float got = __shfl(s[tt][ii], from, 64);
+                    if (tt == t && ii == i) w = got;
+                }
+            int pg = page[0];
+#pragma unroll
+            for (int tt = 1; tt < NT; tt++)
+                if (t == tt) pg = page[tt];
+            if (pg < 0 || p0 + pos >= min(lim, hi)) continue;
+            const C* v = static_cast<const C*>(a.p.values) + paged_offset(a.p, pg, kvh, (p0 + pos) & slots) + (size_t)4 * g * NJ;
+#pragma unroll
+            for (int ii = 0; ii < 4; ii++)
+#pragma unroll
+                for (int j = 0; j < NJ; j++) {
+                    const float x = (float)v[ii * NJ + j];
+                    if (!(fabsf(x) < INFINITY)) acc[j][ii] = fmaf(w, x, acc[j][ii]);
+                }
+        }
+    }
+};
+
+// Clears values that are not there, and among positions that not every row
+// attends to those that are no numbers; true if there was one of the latter.
+template <typename C, int HD>
+__device__ __forceinline__ bool clear_values(typename Tile<C, HD>::Value vr[Tile<C, HD>::NT][4], int p0, int hi, bool differ, const int page[], int g) {
+    using R = Tile<C, HD>;
+    uint32_t odd = 0;
+#pragma unroll
+    for (int t = 0; t < R::NT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const bool held = page[t] >= 0 && p0 + 16 * t + 4 * g + i < hi;
+#pragma unroll
+            for (int w = 0; w < R::VW; w++) {
+                uint32_t x = held ? vr[t][i].w[w] : 0u;
+                if (differ) {
+                    const uint32_t bad = R::T::not_finite(x);
+                    odd |= bad;
+                    x &= ~bad;
+                }
+                vr[t][i].w[w] = x;
             }
         }
+    return __ballot(odd != 0) != 0;
+}
+
+// The stretch [lo, hi) of positions that a split covers, of the `most` that a tile attends to.
+__device__ __forceinline__ void split_range(const PagedAttn& a, int split, int most, int* lo, int* hi) {
+    *lo = 0;
+    *hi = most;
+    if (a.splits > 1) {
+        const int even = (most + a.splits - 1) / a.splits;
+        const int chunk = max(a.chunk, (even + 127) & ~127);
+        *lo = (int)min((int64_t)split * chunk, (int64_t)most);
+        *hi = most - *lo < chunk ? most : *lo + chunk;
+    }
+}
+
+// The prefix as every row's pages.
+__device__ __forceinline__ RowSet prefix_set(const PagedAttn& a) {
+    return RowSet{a.p.prefix_pages, (a.p.prefix_len + (1 << a.p.page_shift) - 1) >> a.p.page_shift, 0, a.p.n_rows, -1};
+}
+
+// Where one row's part of the partial results stands.
+__device__ __forceinline__ size_t part_of(const PagedAttn& a, const RowSet& set, int row, int head, int split) {
+    const int at = a.per_seq ? set.seq * a.per_seq + (row - set.first) : row;
+    return ((size_t)at * a.p.n_heads + head) * a.parts + a.part0 + split;
+}
+
+// One tile of 16 stacked rows over one split of the positions, the positions
+// dealt to four wavefronts in steps of 16 NT.  K and V go from memory to
+// registers in the operands' order; the next step's keys are loaded while
+// this one is computed.  Bound by memory: with few rows per kv head a byte of
+// the cache meets about as many operations as the matrix cores need.
+template <typename C, int HD>
+__global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int prefix) {
+    using R = Tile<C, HD>;
+    constexpr int NT = R::NT, NK = R::NK, NJ = R::NJ, STEP = R::STEP, LD = HD + 4;
+    __shared__ __align__(16) float so[4][kRowTile][LD];
+    __shared__ float sm[4][kRowTile], sl[4][kRowTile];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int kvh = blockIdx.x % a.p.n_kv, slot = blockIdx.x / a.p.n_kv, split = blockIdx.y;
+    RowSet set;
+    int tile;
+    if (prefix) {
+        set = prefix_set(a);
+        tile = slot;
+    } else if (!tile_of_slot(a, slot, 4, a.per, &set, &tile) || (a.both && !row_kernel_takes(set.rows, a.group))) {
+        return;
+    }
+    R r;
+    r.place(a, set, tile * kRowTile, kvh, c);
+    int most, least, lo, hi;
+    r.reach(&most, &least);
+    split_range(a, split, most, &lo, &hi);
+    if (lo >= hi && !a.direct) {
+        if (r.live && wave == 0 && g == 0) a.pml[part_of(a, set, r.row, r.head, split)] = make_float2(-INFINITY, 0.0f);
+        return;
+    }
+    r.load_q(a, g);
+
+    const C* keys = static_cast<const C*>(a.p.keys);
+    const C* values = static_cast<const C*>(a.p.values);
+    const int slots = (1 << a.p.page_shift) - 1;
+    const int steps = (hi - lo + STEP - 1) / STEP;
+    // Pages of this wavefront's next 64 tiles, one per lane (-1: none, or past hi).
+    const auto pages_from = [&](int step) {
+        const int at = lo + STEP * (step + 4 * (lane / NT)) + 16 * (lane % NT);
+        return at < hi ? paged_page(set.pages[at >> a.p.page_shift], a.p.n_pages) : -1;
+    };
+    int page_reg = pages_from(wave), page_n = 0;
+    u4 kf[2][NT][NK];
+    const auto load_keys = [&](int step, int page[NT], u4 f[NT][NK]) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            page[t] = __builtin_amdgcn_readlane(page_reg, page_n * NT + t);
+            const C* k = keys + paged_offset(a.p, max(page[t], 0), kvh, (lo + STEP * step + 16 * t) & slots) + (size_t)c * HD + R::KE * g;
+#pragma unroll
+            for (int i = 0; i < NK; i++) f[t][i] = *reinterpret_cast<const u4*>(k + i * R::KD);
+        }
+    };
+    int page[NT], next_page[NT] = {};
+    const auto step_on = [&](int step, u4 (&kc)[NT][NK], u4 (&kn)[NT][NK]) {
+        // values of this step, keys of the next
+        typename R::Value vr[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const C* v = values + paged_offset(a.p, max(page[t], 0), kvh, ((lo + STEP * step + 16 * t) & slots) + 4 * g) + (size_t)c * NJ;
+#pragma unroll
+            for (int i = 0; i < 4; i++) vr[t][i] = load_words<R::VW>(v + (size_t)i * HD);
+        }
+        if (step + 4 < steps) {
+            if (++page_n == 64 / NT) {
+                page_n = 0;
+                page_reg = pages_from(step + 4);
+            }
+            load_keys(step + 4, next_page, kn);
+        }
+        float s[NT][4];
+        r.scores(kc, s);
+        const int p0 = lo + STEP * step;
+        bool edge = p0 + STEP > min(least, hi), odd = false;
+#pragma unroll
+        for (int t = 0; t < NT; t++) edge = edge || page[t] < 0;
+        if (edge) {
+            r.mask(s, p0, hi, page, g);
+            odd = clear_values<C, HD>(vr, p0, hi, p0 + STEP > least, page, g);
+        }
+        r.weigh(s);
+        r.add(s, vr);
+        if (odd) r.add_odd(a, s, p0, hi, page, kvh, c, g);
 #pragma unroll
         for (int t = 0; t < NT; t++) page[t] = next_page[t];
     };
@@ -464,36 +571,36 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
     }
 
     // the four wavefronts' results together
-    l = group_sum16(l);
-    if (g == 0) { sm[wave][c] = m; sl[wave][c] = l; }
+    const float l = group_sum16(r.l);
+    if (g == 0) { sm[wave][c] = r.m; sl[wave][c] = l; }
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < NJ; j++) so[wave][c][(4 * g + i) * NJ + j] = acc[j][i];
+        for (int j = 0; j < NJ; j++) so[wave][c][(4 * g + i) * NJ + j] = r.acc[j][i];
     __syncthreads();
-    const int r = tid >> 4, e0 = (tid & 15) * NJ;      // row of the tile, NJ neighbouring dimensions
+    const int tr = tid >> 4, e0 = (tid & 15) * NJ;      // row of the tile, NJ neighbouring dimensions
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; w++) M = fmaxf(M, sm[w][r]);
+    for (int w = 0; w < 4; w++) M = fmaxf(M, sm[w][tr]);
     float L = 0.0f, o[NJ] = {};
 #pragma unroll
     for (int w = 0; w < 4; w++) {
         // (a wavefront without positions: weight 0; its sums are 0 or, with NaN scores only, NaN)
-        const float f = sm[w][r] == M ? 1.0f : __builtin_amdgcn_exp2f(sm[w][r] - M);
-        L = fmaf(sl[w][r], f, L);
+        const float f = sm[w][tr] == M ? 1.0f : __builtin_amdgcn_exp2f(sm[w][tr] - M);
+        L = fmaf(sl[w][tr], f, L);
 #pragma unroll
-        for (int k = 0; k < NJ; k++) o[k] = fmaf(so[w][r][e0 + k], f, o[k]);
+        for (int k = 0; k < NJ; k++) o[k] = fmaf(so[w][tr][e0 + k], f, o[k]);
     }
-    const int sr = tile * kRowTile + r;
+    const int sr = tile * kRowTile + tr;
     if (sr >= set.rows * a.group) return;
-    const int orow = set.first + sr / a.group, ohead = kvh * a.group + sr % a.group;
-    if (whole) {
+    const int row = set.first + sr / a.group, head = kvh * a.group + sr % a.group;
+    if (a.direct) {
         const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-        float* dst = a.out + (size_t)orow * a.out_ld + (size_t)ohead * HD + e0;
+        float* dst = a.out + (size_t)row * a.out_ld + (size_t)head * HD + e0;
 #pragma unroll
         for (int k = 0; k < NJ; k++) dst[k] = o[k] * inv;
     } else {
-        const size_t at = ((size_t)orow * a.p.n_heads + ohead) * a.parts + a.part0 + split;
+        const size_t at = part_of(a, set, row, head, split);
         float* dst = a.po + at * HD + e0;
 #pragma unroll
         for (int k = 0; k < NJ; k++) dst[k] = o[k];
@@ -502,38 +609,236 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
     }
 }
 
+// Many rows over the same pages (prompts, a prefix under a batch): eight
+// wavefronts of MT row tiles each share tiles of K and V in LDS, which LDS
+// DMA brings in while the tile before is computed.  In LDS a row's 16-byte
+// pieces are permuted by the row (piece ^ row), so that the 16 rows that a key
+// operand reads at one piece lie in different banks.
+constexpr int kTileThreads = 512;
+// 16 bytes per lane from `src` to LDS at `dst` + 16 lane
+__device__ __forceinline__ void load_to_lds(const char* src, char* dst) { __builtin_amdgcn_global_load_lds(src, dst, 16, 0, 0); }
+template <typename C, int HD, int MT>
+__global__ __launch_bounds__(kTileThreads, HD == 128 ? 2 : 4) void k_paged_attn_tile(PagedAttn a, int prefix) {
+    using R = Tile<C, HD>;
+    constexpr int NT = R::NT, NK = R::NK, NJ = R::NJ, STEP = R::STEP;
+    constexpr int RB = HD * (int)sizeof(C), PIECES = RB / 16;          // bytes and pieces of a row
+    constexpr int POS = sizeof(C) == 4 ? 32 : 64;                      // positions of a tile
+    constexpr int PER = PIECES >= 16 ? 1 : 16 / PIECES;                // rows of 256 bytes
+    constexpr int SWZ = PIECES >= 16 ? 15 : PIECES - 1;
+    constexpr int ROWS = 8 * 16 * MT;
+    __shared__ __align__(16) char lds[2][2][POS * RB];                 // [buffer][keys, values]
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int kvh = blockIdx.x % a.p.n_kv, split = blockIdx.y;
+    const int slot = (int)(gridDim.x / a.p.n_kv) - 1 - (int)(blockIdx.x / a.p.n_kv);    // a sequence's last rows, the longest, first
+    RowSet set;
+    int tile;
+    if (prefix) {
+        set = prefix_set(a);
+        tile = slot;
+    } else if (!tile_of_slot(a, slot, __builtin_ctz(ROWS), 0, &set, &tile) || row_kernel_takes(set.rows, a.group)) {
+        return;
+    }
+    R r[MT];
+    int most[MT], least[MT], wave_most = 0, wave_least = 0x7fffffff;
+#pragma unroll
+    for (int k = 0; k < MT; k++) {
+        r[k].place(a, set, tile * ROWS + (wave * MT + k) * 16, kvh, c);
+        r[k].reach(&most[k], &least[k]);
+        wave_most = max(wave_most, most[k]);
+        wave_least = min(wave_least, least[k]);
+    }
+    // the longest row of the workgroup
+    int* reach = reinterpret_cast<int*>(lds);
+    if (lane == 0) reach[wave] = wave_most;
+    __syncthreads();
+    int all = reach[0];
+#pragma unroll
+    for (int w = 1; w < 8; w++) all = max(all, reach[w]);
+    __syncthreads();
+    int lo, hi;
+    split_range(a, split, all, &lo, &hi);
+    if (lo >= hi && !a.direct) {
+#pragma unroll
+        for (int k = 0; k < MT; k++)
+            if (r[k].live && g == 0) a.pml[part_of(a, set, r[k].row, r[k].head, split)] = make_float2(-INFINITY, 0.0f);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < MT; k++) r[k].load_q(a, g);
+
+    const int slots = (1 << a.p.page_shift) - 1;
+    const int tiles = (hi - lo + POS - 1) / POS;
+    // Pages of the next 64 16-position stretches, one per lane; of the tile being computed and the one on its way.
+    const auto pages_from = [&](int at) { return at < hi ? paged_page(set.pages[at >> a.p.page_shift], a.p.n_pages) : -1; };
+    constexpr int S = POS / 16;
+    int page_reg = pages_from(lo + 16 * lane), next_reg = page_reg;
+    // Brings a tile's keys and values into a buffer: RB bytes per position, 1024 per instruction.
+    const auto fetch = [&](int t, int reg, int buffer) {
+        constexpr int PI = 1024 / RB, N = POS / PI;            // positions per instruction, instructions
+        const int prow = lane / PIECES, piece = lane % PIECES;
+#pragma unroll
+        for (int n = 0; n < (2 * N + 7) / 8; n++) {
+            const int i = wave + 8 * n;
+            if (i < 2 * N) {
+                const int k = i < N ? i : i - N, row = k * PI + prow;
+                const int page = __builtin_amdgcn_readlane(reg, (t % (64 / S)) * S + k * PI / 16);
+                const char* src = static_cast<const char*>(i < N ? a.p.keys : a.p.values) +
+                                  paged_offset(a.p, max(page, 0), kvh, (lo + POS * t + row) & slots) * sizeof(C) + 16 * (piece ^ ((row / PER) & SWZ));
+                load_to_lds(src, &lds[buffer][i < N ? 0 : 1][k * 1024]);
+            }
+        }
+    };
+    // where a lane's pieces of a key, and of a value at each of its four
+    // positions, stand in a stretch of 16 positions (the permutation repeats)
+    static_assert((16 / PER) % (SWZ + 1) == 0, "16 positions hold whole permutations");
+    constexpr int VB = 4 * R::VW, VH = VB > 16 ? VB / 16 : 1;
+    int k_at[NK], v_at[4][VH];
+#pragma unroll
+    for (int i = 0; i < NK; i++) k_at[i] = c * RB + 16 * ((4 * i + g) ^ ((c / PER) & SWZ));
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int h = 0; h < VH; h++) {
+            const int row = 4 * g + i, at = c * VB + 16 * h;
+            v_at[i][h] = row * RB + 16 * ((at / 16) ^ ((row / PER) & SWZ)) + at % 16;
+        }
+    fetch(0, page_reg, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
+    for (int t = 0; t < tiles; t++) {
+        const int buffer = t & 1;
+        if (t + 1 < tiles) {
+            next_reg = (t + 1) % (64 / S) ? page_reg : pages_from(lo + POS * (t + 1) + 16 * lane);
+            fetch(t + 1, next_reg, buffer ^ 1);
+        }
+        const char* kt = lds[buffer][0];
+        const char* vt = lds[buffer][1];
+#pragma unroll
+        for (int st = 0; st < POS / STEP; st++) {
+            const int p0 = lo + POS * t + STEP * st;
+            if (p0 >= min(wave_most, hi)) break;
+            int page[NT];
+            u4 kc[NT][NK];
+            typename R::Value vr[NT][4];
+#pragma unroll
+            for (int u = 0; u < NT; u++) {
+                page[u] = __builtin_amdgcn_readlane(page_reg, (t % (64 / S)) * S + st * NT + u);
+#pragma unroll
+                for (int i = 0; i < NK; i++) kc[u][i] = *reinterpret_cast<const u4*>(kt + (STEP * st + 16 * u) * RB + k_at[i]);
+            }
+#pragma unroll
+            for (int u = 0; u < NT; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const char* v = vt + (STEP * st + 16 * u) * RB;
+                    if constexpr (VB <= 16) {
+                        vr[u][i] = load_words<R::VW>(v + v_at[i][0]);
+                    } else {
+#pragma unroll
+                        for (int h = 0; h < VH; h++) {
+                            const Words<4> w = load_words<4>(v + v_at[i][h]);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) vr[u][i].w[4 * h + e] = w.w[e];
+                        }
+                    }
+                }
+            bool edge = p0 + STEP > min(wave_least, hi), odd = false;
+#pragma unroll
+            for (int u = 0; u < NT; u++) edge = edge || page[u] < 0;
+            if (edge) odd = clear_values<C, HD>(vr, p0, hi, p0 + STEP > wave_least, page, g);
+#pragma unroll
+            for (int k = 0; k < MT; k++) {
+                float s[NT][4];
+                r[k].scores(kc, s);
+                if (edge) r[k].mask(s, p0, hi, page, g);
+                r[k].weigh(s);
+                r[k].add(s, vr);
+                if (odd) r[k].add_odd(a, s, p0, hi, page, kvh, c, g);
+            }
+        }
+        page_reg = next_reg;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // the next tile is there
+        lds_barrier();
+    }
+
+#pragma unroll
+    for (int k = 0; k < MT; k++) {
+        const float L = group_sum16(r[k].l);
+        if (!r[k].live) continue;
+        float f = 1.0f;
+        float* dst;
+        if (a.direct) {
+            f = L != 0.0f ? 1.0f / L : 0.0f;
+            dst = a.out + (size_t)r[k].row * a.out_ld + (size_t)r[k].head * HD;
+        } else {
+            const size_t at = part_of(a, set, r[k].row, r[k].head, split);
+            dst = a.po + at * HD;
+            if (g == 0) a.pml[at] = make_float2(r[k].m == -INFINITY && L != 0.0f ? 0.0f : r[k].m, L);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float* d = dst + (4 * g + i) * NJ;
+            if constexpr (NJ >= 4) {
+#pragma unroll
+                for (int j = 0; j < NJ; j += 4)
+                    *reinterpret_cast<f4u*>(d + j) = f4u{r[k].acc[j][i] * f, r[k].acc[j + 1][i] * f, r[k].acc[j + 2][i] * f, r[k].acc[j + 3][i] * f};
+            } else {
+#pragma unroll
+                for (int j = 0; j < NJ; j++) d[j] = r[k].acc[j][i] * f;
+            }
+        }
+    }
+}
+
+// Partial results of rows, `n` of them per row and head (0: none).
+struct Parts {
+    const float* po; const float2* pml;
+    int stride, first, n;
+};
+
 // Joins the partial results of one row and head: weights 2^(m - max), a
 // quarter of the parts per wavefront, HD / 64 (or one) dimensions per lane.
+// A row's own parts come from the kernel that took its sequence, the
+// prefix's stand with those of the tile kernel.
 template <int HD>
-__global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttn a) {
+__global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttn a, Parts rows, Parts tile, Parts prefix) {
     constexpr int E = HD < 64 ? 1 : HD / 64;
     __shared__ float so[4][HD], sl[4], sm[4];
-    const int row = blockIdx.x / a.p.n_heads, head = blockIdx.x % a.p.n_heads;
+    const int unit = blockIdx.x / a.p.n_heads, head = blockIdx.x % a.p.n_heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (a.p.row_start) {
-        const int s = paged_seq_of_row(a.p, row);
-        if (s < 0) return;
-        int first, end;
-        paged_rows(a.p, s, &first, &end);
-        if (row < first || row >= end) return;
-    }
-    const float2* ml = a.pml + (size_t)blockIdx.x * a.parts;
-    const float* po = a.po + (size_t)blockIdx.x * a.parts * HD;
+    // the row: of the batch, or only of what the row kernel took
+    const bool all = tile.n + prefix.n > 0 || !a.per_seq;
+    const int s = all ? paged_seq_of_row(a.p, unit) : unit / a.per_seq;
+    if (s < 0) return;
+    int first, end;
+    paged_rows(a.p, s, &first, &end);
+    const int row = all ? unit : first + unit % a.per_seq;
+    if (row < first || row >= end) return;
+    const bool by_rows = !a.both || row_kernel_takes(end - first, a.group);
+    const Parts own = by_rows ? rows : tile;
+    if (own.n + prefix.n == 0) return;         // written by its kernel
+    const size_t oat = ((size_t)(by_rows && a.per_seq ? s * a.per_seq + (row - first) : row) * a.p.n_heads + head) * own.stride + own.first;
+    const size_t pat = ((size_t)row * a.p.n_heads + head) * prefix.stride + prefix.first;
+    const int parts = own.n + prefix.n;
+    const auto ml = [&](int i) { return i < own.n ? own.pml[oat + i] : prefix.pml[pat + (i - own.n)]; };
     float M = -INFINITY;
-    for (int i = tid; i < a.parts; i += 256) M = fmaxf(M, ml[i].x);
-    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    for (int i = tid; i < parts; i += 256) M = fmaxf(M, ml(i).x);
+    M = wave_max(M);
     if (lane == 0) sm[wave] = M;
     __syncthreads();
     M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
     float L = 0.0f, o[E] = {};
-    for (int i = wave; i < a.parts; i += 4) {
-        const float2 v = ml[i];
+    for (int i = wave; i < parts; i += 4) {
+        const float2 v = ml(i);
         if (v.x == -INFINITY) continue;
         const float f = __builtin_amdgcn_exp2f(v.x - M);
+        const float* po = i < own.n ? own.po + (oat + i) * HD : prefix.po + (pat + (i - own.n)) * HD;
         L = fmaf(v.y, f, L);
 #pragma unroll
         for (int e = 0; e < E; e++)
-            if (HD >= 64 || lane < HD) o[e] = fmaf(po[(size_t)i * HD + E * lane + e], f, o[e]);
+            if (HD >= 64 || lane < HD) o[e] = fmaf(po[E * lane + e], f, o[e]);
     }
     if (lane == 0) sl[wave] = L;
 #pragma unroll
@@ -552,45 +857,106 @@ __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttn a) {
 namespace {
 
 // How a call is split, from what the host knows of it.
+struct Launch {
+    int tiles = 0, splits = 0, chunk = 0;
+};
 struct AttnPlan {
-    int slots = 0, splits = 1, chunk = 0;            // own pages
-    int prefix_tiles = 0, prefix_splits = 0, prefix_chunk = 0;
-    int parts = 1;
-    size_t bytes = 0;
+    Launch rows, tile, prefix;       // own pages: short sequences, long ones; the prefix
+    int per = 0;                     // slots of a sequence in the row kernel (0: as its rows need)
+    bool prefix_by_tile = false;
+    int per_seq = 0, rows_parts = 0, tile_parts = 0;
+    size_t row_units = 0, all_units = 0, bytes = 0;
 };
 
-AttnPlan plan_attention(const PagedArgs& p, uint32_t max_len) {
+// Row tiles of 16 per wavefront in the tile kernel: as the registers allow.
+template <typename C> constexpr int tile_mt(int hd) { return 1; }
+int tile_rows(int dtype, int hd) { return 128 * (dtype == YL_T_F32 ? tile_mt<float>(hd) : dtype == YL_T_F16 ? tile_mt<_Float16>(hd) : tile_mt<__bf16>(hd)); }
+
+AttnPlan plan_attention(const PagedArgs& p, int dtype, uint32_t max_len) {
     AttnPlan r;
-    const int group = p.n_heads / p.n_kv;
-    const int64_t cap = paged_capacity(p);
+    const int group = p.n_heads / p.n_kv, R = tile_rows(dtype, p.hd);
+    const int64_t cap = paged_capacity(p), stacked = (int64_t)p.n_rows * group;
     const int64_t longest = max_len && max_len < cap ? max_len : cap;
     const int own = (int)std::max<int64_t>(longest - p.prefix_len, 0);
-    r.slots = p.row_start ? (int)(((int64_t)p.n_rows * group) / kRowTile) + p.n_seqs : p.n_seqs * ((group + kRowTile - 1) / kRowTile);
-    const auto split = [&](int64_t tiles, int positions, int* splits, int* chunk) {
-        const int64_t want = std::max<int64_t>(2048 / std::max<int64_t>(tiles, 1), 1);
-        *splits = (int)std::clamp<int64_t>(want, 1, std::max(1, (positions + 255) / 256));
-        *chunk = ((positions + *splits - 1) / *splits + 127) & ~127;
+    const auto split = [&](Launch* l, int positions, int wanted, int least) {
+        const int64_t want = std::max<int64_t>(wanted / std::max<int64_t>((int64_t)l->tiles * p.n_kv, 1), 1);
+        l->splits = (int)std::clamp<int64_t>(want, 1, std::max(1, (positions + least - 1) / least));
+        l->chunk = ((positions + l->splits - 1) / l->splits + 127) & ~127;
     };
-    split((int64_t)r.slots * p.n_kv, own, &r.splits, &r.chunk);
-    r.parts = r.splits;
-    if (p.prefix_len) {
-        r.prefix_tiles = (int)(((int64_t)p.n_rows * group + kRowTile - 1) / kRowTile);
-        split((int64_t)r.prefix_tiles * p.n_kv, p.prefix_len, &r.prefix_splits, &r.prefix_chunk);
-        r.parts += r.prefix_splits;
+    const bool both = p.row_start && stacked > kRowKernelRows;
+    r.per = both ? kRowKernelRows / kRowTile : p.row_start ? 0 : (group + kRowTile - 1) / kRowTile;
+    r.rows.tiles = r.per ? p.n_seqs * r.per : (int)(stacked / kRowTile) + p.n_seqs;
+    split(&r.rows, own, 2048, 256);
+    if (both) {
+        r.tile.tiles = (int)(stacked / R) + p.n_seqs;
+        split(&r.tile, own, 512, 512);
     }
-    if (r.parts > 1) r.bytes = (size_t)p.n_rows * p.n_heads * r.parts * (p.hd + 2) * sizeof(float);
+    if (p.prefix_len) {
+        r.prefix_by_tile = stacked > kRowKernelRows;
+        r.prefix.tiles = (int)((stacked + (r.prefix_by_tile ? R : kRowTile) - 1) / (r.prefix_by_tile ? R : kRowTile));
+        split(&r.prefix, p.prefix_len, r.prefix_by_tile ? 512 : 2048, 256);
+    }
+    // partial results: of the row kernel, for as many rows as it can take of
+    // the sequences if that is less than all; of the others, for every row
+    r.per_seq = row_kernel_tokens(group);
+    if ((int64_t)p.n_seqs * r.per_seq >= p.n_rows) r.per_seq = 0;
+    r.rows_parts = r.rows.splits > 1 || p.prefix_len ? r.rows.splits : 0;
+    r.tile_parts = r.tile.splits > 1 || (p.prefix_len && r.tile.tiles) ? r.tile.splits : 0;
+    r.row_units = (size_t)(r.per_seq ? p.n_seqs * r.per_seq : p.n_rows) * p.n_heads * r.rows_parts;
+    r.all_units = (size_t)p.n_rows * p.n_heads * (r.tile_parts + r.prefix.splits);
+    r.bytes = (r.row_units + r.all_units) * (p.hd + 2) * sizeof(float);
     return r;
 }
 
-template <typename C>
-hipError_t launch_rows(const PagedAttn& a, int tiles, int prefix, hipStream_t s) {
-    auto k = a.p.hd == 32 ? k_paged_attn_rows<C, 32> : a.p.hd == 64 ? k_paged_attn_rows<C, 64> : k_paged_attn_rows<C, 128>;
-    hipLaunchKernelGGL(k, dim3((unsigned)tiles * a.p.n_kv, a.splits), dim3(256), 0, s, a, prefix);
+template <typename C, int HD>
+hipError_t launch_attn_hd(const PagedAttn& a, const dim3& grid, bool by_tile, bool prefix, hipStream_t s) {
+    if (by_tile) hipLaunchKernelGGL((k_paged_attn_tile<C, HD, tile_mt<C>(HD)>), grid, dim3(kTileThreads), 0, s, a, prefix);
+    else hipLaunchKernelGGL((k_paged_attn_rows<C, HD>), grid, dim3(256), 0, s, a, prefix);
     return hipGetLastError();
 }
-hipError_t launch_rows_of(int dtype, const PagedAttn& a, int tiles, int prefix, hipStream_t s) {
-    return dtype == YL_T_F32 ? launch_rows<float>(a, tiles, prefix, s) : dtype == YL_T_F16 ? launch_rows<_Float16>(a, tiles, prefix, s)
-                                                                                          : launch_rows<__bf16>(a, tiles, prefix, s);
+
+template <typename C>
+hipError_t launch_attn(PagedAttn a, const Launch& l, bool by_tile, bool prefix, hipStream_t s) {
+    a.splits = l.splits;
+    a.chunk = l.chunk;
+    const dim3 grid((unsigned)l.tiles * a.p.n_kv, l.splits);
+    return a.p.hd == 32 ? launch_attn_hd<C, 32>(a, grid, by_tile, prefix, s) : a.p.hd == 64 ? launch_attn_hd<C, 64>(a, grid, by_tile, prefix, s)
+                                                                           : launch_attn_hd<C, 128>(a, grid, by_tile, prefix, s);
+}
+
+template <typename C>
+hipError_t launch_all(PagedAttn a, const AttnPlan& plan, float* space, hipStream_t s) {
+    const size_t units = plan.row_units + plan.all_units;
+    float* const all_po = space + plan.row_units * a.p.hd;
+    float2* const ml = reinterpret_cast<float2*>(space + units * a.p.hd);
+    float2* const all_ml = ml + plan.row_units;
+    const int all_parts = plan.tile_parts + plan.prefix.splits;
+    a.both = plan.tile.tiles > 0;
+    a.per = plan.per;
+    a.po = space; a.pml = ml;
+    a.parts = plan.rows_parts; a.per_seq = plan.per_seq;
+    a.direct = !plan.rows_parts;
+    hipError_t e = launch_attn<C>(a, plan.rows, false, false, s);
+    a.po = all_po; a.pml = all_ml;
+    a.parts = all_parts; a.per_seq = 0;
+    if (e == hipSuccess && plan.tile.tiles) {
+        a.direct = !plan.tile_parts;
+        e = launch_attn<C>(a, plan.tile, true, false, s);
+    }
+    if (e == hipSuccess && plan.prefix.tiles) {
+        a.direct = 0;
+        a.part0 = plan.tile_parts;
+        e = launch_attn<C>(a, plan.prefix, plan.prefix_by_tile, true, s);
+    }
+    if (e != hipSuccess || !units) return e;
+    a.per_seq = plan.per_seq;
+    const Parts rows{space, ml, plan.rows_parts, 0, plan.rows_parts}, tile{all_po, all_ml, all_parts, 0, plan.tile_parts};
+    const Parts prefix{all_po, all_ml, all_parts, plan.tile_parts, plan.prefix.splits};
+    const dim3 grid((unsigned)(all_parts || !plan.per_seq ? a.p.n_rows : a.p.n_seqs * plan.per_seq) * a.p.n_heads);
+    if (a.p.hd == 32) hipLaunchKernelGGL(k_paged_attn_join<32>, grid, dim3(256), 0, s, a, rows, tile, prefix);
+    else if (a.p.hd == 64) hipLaunchKernelGGL(k_paged_attn_join<64>, grid, dim3(256), 0, s, a, rows, tile, prefix);
+    else hipLaunchKernelGGL(k_paged_attn_join<128>, grid, dim3(256), 0, s, a, rows, tile, prefix);
+    return hipGetLastError();
 }
 
 yl_status refuse(const char* what, yl_status st = YL_ERR_ARG) {
@@ -608,7 +974,7 @@ extern "C" {
 size_t yl_paged_attention_workspace(const yl_paged_cache* cache, const yl_paged_batch* batch, uint32_t n_heads) {
     PagedArgs p{};
     if (paged_args(cache, batch, n_heads, &p) != YL_OK || !p.n_rows || !p.n_seqs) return 0;
-    return plan_attention(p, batch->max_len).bytes;
+    return plan_attention(p, cache->dtype, batch->max_len).bytes;
 }
 
 yl_status yl_paged_attention(float* out, size_t out_ld, const float* q, size_t q_ld, const yl_paged_cache* cache,
@@ -622,27 +988,16 @@ yl_status yl_paged_attention(float* out, size_t out_ld, const float* q, size_t q
     const size_t att = (size_t)n_heads * cache->head_size;
     if (q_ld < att || out_ld < att) return refuse("paged_attention: rows further apart than they are long");
     if (q == out && q_ld != out_ld) return refuse("paged_attention: in place, q_ld and out_ld are the same");
-    const AttnPlan plan = plan_attention(a.p, batch->max_len);
+    const AttnPlan plan = plan_attention(a.p, cache->dtype, batch->max_len);
     if (plan.bytes && (!workspace || (uintptr_t)workspace % 16)) return refuse("paged_attention: the workspace has to be there, 16-byte aligned");
     if (workspace_bytes < plan.bytes) return refuse("paged_attention: the workspace is smaller than yl_paged_attention_workspace says", YL_ERR_RANGE);
     a.out = out; a.q = q; a.out_ld = out_ld; a.q_ld = q_ld;
     a.scale_log2 = attn_scale * 1.4426950408889634f;
     a.group = a.p.n_heads / a.p.n_kv;
-    a.parts = plan.parts;
-    a.po = static_cast<float*>(workspace);
-    a.pml = reinterpret_cast<float2*>(a.po + (size_t)a.p.n_rows * a.p.n_heads * plan.parts * a.p.hd);
     hipStream_t s = (hipStream_t)stream;
-    a.splits = plan.splits; a.chunk = plan.chunk; a.part0 = 0;
-    hipError_t e = launch_rows_of(cache->dtype, a, plan.slots, 0, s);
-    if (e == hipSuccess && plan.prefix_tiles) {
-        a.splits = plan.prefix_splits; a.chunk = plan.prefix_chunk; a.part0 = plan.splits;
-        e = launch_rows_of(cache->dtype, a, plan.prefix_tiles, 1, s);
-    }
-    if (e == hipSuccess && plan.parts > 1) {
-        auto k = a.p.hd == 32 ? k_paged_attn_join<32> : a.p.hd == 64 ? k_paged_attn_join<64> : k_paged_attn_join<128>;
-        hipLaunchKernelGGL(k, dim3((unsigned)a.p.n_rows * a.p.n_heads), dim3(256), 0, s, a);
-        e = hipGetLastError();
-    }
+    float* space = static_cast<float*>(workspace);
+    const hipError_t e = cache->dtype == YL_T_F32 ? launch_all<float>(a, plan, space, s) : cache->dtype == YL_T_F16 ? launch_all<_Float16>(a, plan, space, s)
+                                                                                                                  : launch_all<__bf16>(a, plan, space, s);
     if (e == hipSuccess) return YL_OK;
     set_error(std::string("paged_attention launch: ") + hipGetErrorString(e));
     return YL_ERR_HIP;
