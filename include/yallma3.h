@@ -251,7 +251,8 @@ typedef struct {
  * page_table[s][i / page_size].  An entry that names no page (negative, or not
  * below n_pages) and a position past the table hold nothing: they are not
  * written and nothing attends to them.  prefix_len + max_pages * page_size is
- * below 2^30, n_rows and n_seqs times a call's n_heads below 2^24. */
+ * below 2^30, n_rows times a call's n_heads below 2^24, n_seqs times them
+ * below 2^22. */
 typedef struct {
     uint32_t n_seqs, n_rows;
     uint32_t max_pages;            /* entries of a sequence in page_table */

@@ -88,9 +88,9 @@ yl_status paged_args(const yl_paged_cache* c, const yl_paged_batch* b, uint32_t 
         return refuse("paged: n_heads (at most 1024) is a multiple of n_kv_heads");
     if (!c->keys || !c->values || ((uintptr_t)c->keys | (uintptr_t)c->values) % 16)
         return refuse("paged: keys and values have to be there, 16-byte aligned");
-    if ((uint64_t)b->n_rows * n_heads >= (1ull << 24) || (uint64_t)b->n_seqs * n_heads >= (1ull << 24) ||
+    if ((uint64_t)b->n_rows * n_heads >= (1ull << 24) || (uint64_t)b->n_seqs * n_heads >= (1ull << 22) ||
         (uint64_t)b->prefix_len + (uint64_t)b->max_pages * c->page_size >= (1ull << 30))
-        return refuse("paged: n_rows * n_heads and n_seqs * n_heads below 2^24, a sequence's capacity below 2^30", YL_ERR_RANGE);
+        return refuse("paged: n_rows * n_heads below 2^24, n_seqs * n_heads below 2^22, a sequence's capacity below 2^30", YL_ERR_RANGE);
     if (!b->row_start && b->n_rows != b->n_seqs) return refuse("paged: without row_start there is one row per sequence");
     if (b->n_rows && b->n_seqs && (!b->kv_len || (b->max_pages && !b->page_table)))
         return refuse("paged: kv_len and page_table have to be there");

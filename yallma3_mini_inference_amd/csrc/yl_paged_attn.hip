@@ -128,6 +128,13 @@ __device__ __forceinline__ float group_max16(float v) {   // over the lanes of o
     v = fmaxf(v, __shfl_xor(v, 16, 64));
     return fmaxf(v, __shfl_xor(v, 32, 64));
 }
+// the largest of 16 neighbouring lanes (every lane active)
+__device__ __forceinline__ int max16(int v) {
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, false));    // quad_perm [1,0,3,2]
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, false));    // quad_perm [2,3,0,1]
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, false));   // row_half_mirror
+    return max(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, false)); // row_mirror
+}
 __device__ __forceinline__ float group_sum16(float v) {
     v += __shfl_xor(v, 16, 64);
     return v + __shfl_xor(v, 32, 64);
@@ -143,14 +150,20 @@ struct PagedAttn {
     float scale_log2;                // attn_scale * log2(e)
     int group;                       // query heads per kv head
     int parts, part0;                // partial results per row and head; the first of this launch's
-    int per_seq;                     // their rows: so many for each sequence, 0: the batch's rows
     int chunk;                       // positions of a split at least
     int splits;
     int direct;                      // this launch sees all that its rows attend to: it writes `out`
-    int per;                         // row kernel: slots of a sequence, 0: as its rows need
+    // the row kernel's own work: tiles of 16 rows a sequence can have; units
+    // wanted (0: a unit per tile, positions never split) and units there is
+    // room for; what each sequence's units are, for the joining kernel
+    int per, wanted, max_units;
+    int4* units;
     int both;                        // sequences are divided between the row kernel and the tile kernel
-    float* po;                       // [row][n_heads][parts][hd], unnormalised
-    float2* pml;                     // [row][n_heads][parts]: maximum (base 2), sum; maximum -inf: nothing there
+    // partial results, unnormalised, and their maximum (base 2) and sum, maximum
+    // -inf: nothing there.  Of the row kernel's own work [unit][n_kv][16 rows],
+    // of the others [row][n_heads][parts]
+    float* po;
+    float2* pml;
 };
 
 // A tile of the stacked rows that attend to the same pages.
@@ -160,42 +173,39 @@ struct RowSet {
     int seq;                             // sequence, or -1: the whole batch over the prefix
 };
 
+__device__ __forceinline__ RowSet set_of_seq(const PagedArgs& p, int seq) {
+    RowSet set;
+    set.seq = seq;
+    set.entries = p.max_pages;
+    set.pages = p.table + (size_t)seq * p.max_pages;
+    int end;
+    paged_rows(p, seq, &set.first, &end);
+    set.rows = end - set.first;
+    return set;
+}
+
 // The tile of slot `slot`: sequence s takes slots from floor(row_start[s] *
-// group / 16) + s on, of which it uses one per 16 stacked rows: a sequence's
+// group / rows of a tile) + s on, of which it uses one per tile: a sequence's
 // slots always suffice, and are found by a search over row_start alone (64
-// starts per step, one per lane).  `per`: that many slots for every sequence
-// instead.  False: a slot that nothing uses.
-__device__ __forceinline__ bool tile_of_slot(const PagedAttn& a, int slot, int rows_log2, int per, RowSet* set, int* tile) {
+// starts per step, one per lane).  False: a slot that nothing uses.
+__device__ __forceinline__ bool tile_of_slot(const PagedAttn& a, int slot, int rows_log2, RowSet* set, int* tile) {
     const PagedArgs& p = a.p;
-    set->entries = p.max_pages;
-    if (per) {
-        set->seq = slot / per;
-        *tile = slot - set->seq * per;
-        int end;
-        paged_rows(p, set->seq, &set->first, &end);
-        set->rows = end - set->first;
-    } else {
-        const int lane = threadIdx.x & 63;
-        const auto base = [&](int s) {
-            const uint32_t st = p.row_start[s];
-            return (int)(((int64_t)(st < (uint32_t)p.n_rows ? (int)st : p.n_rows) * a.group) >> rows_log2) + s;
-        };
-        int lo = 0, n = p.n_seqs;
-        while (n > 1) {
-            const int step = (n + 63) >> 6;
-            const bool ok = lane * step < n && base(lo + lane * step) <= slot;
-            const int c = max(1, (int)__builtin_popcountll(__ballot(ok))) - 1;
-            lo += c * step;
-            n = min(step, n - c * step);
-        }
-        lo = __builtin_amdgcn_readfirstlane(lo);
-        set->seq = lo;
-        *tile = slot - base(lo);
-        int end;
-        paged_rows(p, lo, &set->first, &end);
-        set->rows = end - set->first;
+    const int lane = threadIdx.x & 63;
+    const auto base = [&](int s) {
+        const uint32_t st = p.row_start[s];
+        return (int)(((int64_t)(st < (uint32_t)p.n_rows ? (int)st : p.n_rows) * a.group) >> rows_log2) + s;
+    };
+    int lo = 0, n = p.n_seqs;
+    while (n > 1) {
+        const int step = (n + 63) >> 6;
+        const bool ok = lane * step < n && base(lo + lane * step) <= slot;
+        const int c = max(1, (int)__builtin_popcountll(__ballot(ok))) - 1;
+        lo += c * step;
+        n = min(step, n - c * step);
     }
-    set->pages = p.table + (size_t)set->seq * p.max_pages;
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    *set = set_of_seq(p, lo);
+    *tile = slot - base(lo);
     return *tile >= 0 && ((int64_t)*tile << rows_log2) < (int64_t)set->rows * a.group;
 }
 
@@ -220,7 +230,79 @@ constexpr int kRowTile = 16;
 // row kernel takes it.
 constexpr int kRowKernelRows = 32;
 __device__ __forceinline__ bool row_kernel_takes(int rows, int group) { return (int64_t)rows * group <= kRowKernelRows; }
-inline int row_kernel_tokens(int group) { return std::max(1, kRowKernelRows / group); }
+
+// A unit of the row kernel's own work: a tile of a sequence's rows over one of
+// `splits` stretches of its positions.  `first`: the sequence's first unit.
+struct Unit {
+    int seq, tile, split, splits, chunk, first;
+};
+
+__device__ __forceinline__ int scan_add(int x) {       // inclusive, over the 64 lanes
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, true);
+    return x;
+}
+
+// Unit `u` of the batch.  All tiles' positions together, divided by the units
+// wanted, are a unit's share: a long sequence becomes many units, a short one
+// one, whatever the lengths are when the work runs.  Every wavefront works
+// this out from the lengths (64 sequences per step, one per lane), alike.
+__device__ __forceinline__ bool unit_of(const PagedAttn& a, int u, Unit* r) {
+    const PagedArgs& p = a.p;
+    const int lane = threadIdx.x & 63;
+    // a sequence's tiles (none where the tile kernel takes it) and its longest row's positions
+    const auto of_seq = [&](int s, int* tiles, int* len) {
+        *tiles = *len = 0;
+        if (s >= p.n_seqs) return;
+        int first, end;
+        paged_rows(p, s, &first, &end);
+        const int n = end - first;
+        if (n == 0 || (a.both && !row_kernel_takes(n, a.group))) return;
+        *tiles = min((n * a.group + kRowTile - 1) / kRowTile, a.per);
+        *len = max(paged_limit(p, (int64_t)p.kv_len[s] - 1) - p.prefix_len, 0);
+    };
+    int tiles, len;
+    of_seq(lane, &tiles, &len);
+    float sum = 0.0f;
+    for (int s0 = 0;;) {
+        float x = (float)tiles * (float)len;
+        x += dpp_mov<0xB1>(x);
+        x += dpp_mov<0x4E>(x);
+        x += dpp_mov<0x141>(x);
+        x += dpp_mov<0x140>(x);
+        sum += (lane_value(x, 0) + lane_value(x, 16)) + (lane_value(x, 32) + lane_value(x, 48));
+        s0 += 64;
+        if (s0 >= p.n_seqs) break;
+        of_seq(s0 + lane, &tiles, &len);
+    }
+    // (rounded up beyond the sum's own rounding, so that the units never are more than there is room for)
+    const float share = sum * 1.001f / (float)a.wanted;
+    const int chunk = share < 1e9f ? (max((int)share + 1, a.chunk) + 63) & ~63 : 1 << 30;
+    int before = 0;
+    for (int s0 = 0; s0 < p.n_seqs; s0 += 64) {
+        if (p.n_seqs > 64) of_seq(s0 + lane, &tiles, &len);
+        const int splits = max(1, (int)(((unsigned)len + (unsigned)chunk - 1u) / (unsigned)chunk));
+        const int mine = tiles * splits, upto = before + scan_add(mine);
+        const auto here = __ballot(u < upto);
+        if (here) {
+            const int l = __builtin_ctzll(here);
+            r->seq = s0 + l;
+            r->splits = __builtin_amdgcn_readlane(splits, l);
+            r->first = __builtin_amdgcn_readlane(upto - mine, l);
+            const int k = u - r->first;
+            r->tile = k / r->splits;
+            r->split = k - r->tile * r->splits;
+            r->chunk = chunk;
+            return true;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
 
 // 16 stacked rows in a wavefront: lane (c, g) holds of row c the query parts,
 // the sums of dimensions (4g + i) NJ + j and those of its positions.
@@ -247,22 +329,18 @@ struct Tile {
         live = r < set.rows * a.group;
         row = set.first + (live ? r / a.group : 0);
         head = kvh * a.group + (live ? r % a.group : 0);
-        lim = live ? limit_of_row(a, set, row) : 0;
-        if (live) lim = (int)min((int64_t)lim, (int64_t)set.entries << a.p.page_shift);
         m = -INFINITY;
         l = 0.0f;
 #pragma unroll
         for (int j = 0; j < NJ; j++) acc[j] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // The tile's longest and shortest rows (spare rows follow the longest, so that they need no masks).
-    __device__ __forceinline__ void reach(int* most, int* least) {
-        int x = lim;
-        for (int o = 1; o < 16; o <<= 1) x = max(x, __shfl_xor(x, o, 64));
-        *most = __builtin_amdgcn_readfirstlane(x);
+    // What the rows attend to, and the longest and the shortest of them
+    // (spare rows follow the longest, so that they need no masks).
+    __device__ __forceinline__ void reach(const PagedAttn& a, const RowSet& set, int* most, int* least) {
+        lim = live ? (int)min((int64_t)limit_of_row(a, set, row), (int64_t)set.entries << a.p.page_shift) : 0;
+        *most = __builtin_amdgcn_readfirstlane(max16(lim));
         if (!live) lim = *most;
-        x = lim;
-        for (int o = 1; o < 16; o <<= 1) x = min(x, __shfl_xor(x, o, 64));
-        *least = __builtin_amdgcn_readfirstlane(x);
+        *least = -__builtin_amdgcn_readfirstlane(max16(-lim));
     }
     // q of the lane's row, cut into parts, in the order of the keys' pieces
     __device__ __forceinline__ void load_q(const PagedAttn& a, int g) {
@@ -458,7 +536,7 @@ __device__ __forceinline__ void split_range(const PagedAttn& a, int split, int m
     *hi = most;
     if (a.splits > 1) {
         const int even = (most + a.splits - 1) / a.splits;
-        const int chunk = max(a.chunk, (even + 127) & ~127);
+        const int chunk = max(a.chunk, (even + 63) & ~63);
         *lo = (int)min((int64_t)split * chunk, (int64_t)most);
         *hi = most - *lo < chunk ? most : *lo + chunk;
     }
@@ -469,10 +547,9 @@ __device__ __forceinline__ RowSet prefix_set(const PagedAttn& a) {
     return RowSet{a.p.prefix_pages, (a.p.prefix_len + (1 << a.p.page_shift) - 1) >> a.p.page_shift, 0, a.p.n_rows, -1};
 }
 
-// Where one row's part of the partial results stands.
-__device__ __forceinline__ size_t part_of(const PagedAttn& a, const RowSet& set, int row, int head, int split) {
-    const int at = a.per_seq ? set.seq * a.per_seq + (row - set.first) : row;
-    return ((size_t)at * a.p.n_heads + head) * a.parts + a.part0 + split;
+// Where a row's partial result of the tile kernel, or over the prefix, stands.
+__device__ __forceinline__ size_t part_of(const PagedAttn& a, int row, int head, int split) {
+    return ((size_t)row * a.p.n_heads + head) * a.parts + a.part0 + split;
 }
 
 // One tile of 16 stacked rows over one split of the positions, the positions
@@ -483,47 +560,72 @@ __device__ __forceinline__ size_t part_of(const PagedAttn& a, const RowSet& set,
 template <typename C, int HD>
 __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int prefix) {
     using R = Tile<C, HD>;
-    constexpr int NT = R::NT, NK = R::NK, NJ = R::NJ, STEP = R::STEP, LD = HD + 4;
+    constexpr int NT = R::NT, NK = R::NK, NJ = R::NJ, STEP = R::STEP, LD = HD + 4, W = 4;
     __shared__ __align__(16) float so[4][kRowTile][LD];
     __shared__ float sm[4][kRowTile], sl[4][kRowTile];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
-    const int kvh = blockIdx.x % a.p.n_kv, slot = blockIdx.x / a.p.n_kv, split = blockIdx.y;
+    const int kvh = blockIdx.x % a.p.n_kv, slot = blockIdx.x / a.p.n_kv;
     RowSet set;
-    int tile;
+    Unit u{0, slot, (int)blockIdx.y, 1, 0, 0};
     if (prefix) {
         set = prefix_set(a);
-        tile = slot;
-    } else if (!tile_of_slot(a, slot, 4, a.per, &set, &tile) || (a.both && !row_kernel_takes(set.rows, a.group))) {
-        return;
+    } else {
+        if (a.wanted) {
+            if (!unit_of(a, slot, &u)) return;
+            if (slot == u.first && kvh == 0 && tid == 0) a.units[u.seq] = make_int4(u.first, u.splits, 0, 0);
+        } else {
+            u.seq = slot / a.per;
+            u.first = u.seq * a.per;
+            u.tile = slot - u.first;
+            u.split = 0;
+        }
+        set = set_of_seq(a.p, u.seq);
+        if (u.tile * kRowTile >= set.rows * a.group || (a.both && !row_kernel_takes(set.rows, a.group))) return;
     }
+    const bool direct = a.direct && u.splits == 1;
     R r;
-    r.place(a, set, tile * kRowTile, kvh, c);
+    r.place(a, set, u.tile * kRowTile, kvh, c);
+    // Pages of this wavefront's next 64 tiles, one per lane (-1: none).  The
+    // first are loaded from where the stretch begins if it begins where the
+    // host's knowledge says, so that they, q and the lengths come in one round trip.
+    const int64_t held = (int64_t)set.entries << a.p.page_shift;
+    const auto pages_from = [&](int begin, int step) {
+        const int64_t at = (int64_t)begin + STEP * (step + W * (lane / NT)) + 16 * (lane % NT);
+        return at < held ? paged_page(set.pages[at >> a.p.page_shift], a.p.n_pages) : -1;
+    };
+    const int begin = (int)min((int64_t)u.split * (prefix ? a.chunk : u.chunk), held);
+    int page_reg = pages_from(begin, wave), page_n = 0;
+    r.load_q(a, g);
     int most, least, lo, hi;
-    r.reach(&most, &least);
-    split_range(a, split, most, &lo, &hi);
-    if (lo >= hi && !a.direct) {
-        if (r.live && wave == 0 && g == 0) a.pml[part_of(a, set, r.row, r.head, split)] = make_float2(-INFINITY, 0.0f);
+    r.reach(a, set, &most, &least);
+    if (prefix) {
+        split_range(a, u.split, most, &lo, &hi);
+    } else {
+        lo = min(begin, most);
+        hi = u.splits > 1 && most - lo > u.chunk ? lo + u.chunk : most;
+    }
+    // where the partial result of the tile's row `k` stands
+    const auto part_at = [&](int k, int row, int head) {
+        return prefix ? part_of(a, row, head, u.split) : ((size_t)slot * a.p.n_kv + kvh) * kRowTile + k;
+    };
+    if (lo >= hi && !direct) {
+        if (r.live && wave == 0 && g == 0) a.pml[part_at(c, r.row, r.head)] = make_float2(-INFINITY, 0.0f);
         return;
     }
-    r.load_q(a, g);
+    if (lo != begin) page_reg = pages_from(lo, wave);
 
     const C* keys = static_cast<const C*>(a.p.keys);
     const C* values = static_cast<const C*>(a.p.values);
     const int slots = (1 << a.p.page_shift) - 1;
     const int steps = (hi - lo + STEP - 1) / STEP;
-    // Pages of this wavefront's next 64 tiles, one per lane (-1: none, or past hi).
-    const auto pages_from = [&](int step) {
-        const int at = lo + STEP * (step + 4 * (lane / NT)) + 16 * (lane % NT);
-        return at < hi ? paged_page(set.pages[at >> a.p.page_shift], a.p.n_pages) : -1;
-    };
-    int page_reg = pages_from(wave), page_n = 0;
     u4 kf[2][NT][NK];
     const auto load_keys = [&](int step, int page[NT], u4 f[NT][NK]) {
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            page[t] = __builtin_amdgcn_readlane(page_reg, page_n * NT + t);
+            const int got = __builtin_amdgcn_readlane(page_reg, page_n * NT + t);
+            page[t] = lo + STEP * step + 16 * t < hi ? got : -1;
             const C* k = keys + paged_offset(a.p, max(page[t], 0), kvh, (lo + STEP * step + 16 * t) & slots) + (size_t)c * HD + R::KE * g;
 #pragma unroll
             for (int i = 0; i < NK; i++) f[t][i] = *reinterpret_cast<const u4*>(k + i * R::KD);
@@ -539,12 +641,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
 #pragma unroll
             for (int i = 0; i < 4; i++) vr[t][i] = load_words<R::VW>(v + (size_t)i * HD);
         }
-        if (step + 4 < steps) {
+        if (step + W < steps) {
             if (++page_n == 64 / NT) {
                 page_n = 0;
-                page_reg = pages_from(step + 4);
+                page_reg = pages_from(lo, step + W);
             }
-            load_keys(step + 4, next_page, kn);
+            load_keys(step + W, next_page, kn);
         }
         float s[NT][4];
         r.scores(kc, s);
@@ -564,13 +666,13 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
     };
     if (wave < steps) {
         load_keys(wave, page, kf[0]);
-        for (int step = wave; step < steps; step += 8) {
+        for (int step = wave; step < steps; step += 2 * W) {
             step_on(step, kf[0], kf[1]);
-            if (step + 4 < steps) step_on(step + 4, kf[1], kf[0]);
+            if (step + W < steps) step_on(step + W, kf[1], kf[0]);
         }
     }
 
-    // the four wavefronts' results together
+    // the wavefronts' results together
     const float l = group_sum16(r.l);
     if (g == 0) { sm[wave][c] = r.m; sl[wave][c] = l; }
 #pragma unroll
@@ -591,16 +693,16 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
 #pragma unroll
         for (int k = 0; k < NJ; k++) o[k] = fmaf(so[w][tr][e0 + k], f, o[k]);
     }
-    const int sr = tile * kRowTile + tr;
+    const int sr = u.tile * kRowTile + tr;
     if (sr >= set.rows * a.group) return;
     const int row = set.first + sr / a.group, head = kvh * a.group + sr % a.group;
-    if (a.direct) {
+    if (direct) {
         const float inv = L != 0.0f ? 1.0f / L : 0.0f;
         float* dst = a.out + (size_t)row * a.out_ld + (size_t)head * HD + e0;
 #pragma unroll
         for (int k = 0; k < NJ; k++) dst[k] = o[k] * inv;
     } else {
-        const size_t at = part_of(a, set, row, head, split);
+        const size_t at = part_at(tr, row, head);
         float* dst = a.po + at * HD + e0;
 #pragma unroll
         for (int k = 0; k < NJ; k++) dst[k] = o[k];
@@ -637,7 +739,7 @@ __global__ __launch_bounds__(kTileThreads, HD == 128 ? 2 : 4) void k_paged_attn_
     if (prefix) {
         set = prefix_set(a);
         tile = slot;
-    } else if (!tile_of_slot(a, slot, __builtin_ctz(ROWS), 0, &set, &tile) || row_kernel_takes(set.rows, a.group)) {
+    } else if (!tile_of_slot(a, slot, __builtin_ctz(ROWS), &set, &tile) || row_kernel_takes(set.rows, a.group)) {
         return;
     }
     R r[MT];
@@ -645,7 +747,7 @@ __global__ __launch_bounds__(kTileThreads, HD == 128 ? 2 : 4) void k_paged_attn_
 #pragma unroll
     for (int k = 0; k < MT; k++) {
         r[k].place(a, set, tile * ROWS + (wave * MT + k) * 16, kvh, c);
-        r[k].reach(&most[k], &least[k]);
+        r[k].reach(a, set, &most[k], &least[k]);
         wave_most = max(wave_most, most[k]);
         wave_least = min(wave_least, least[k]);
     }
@@ -662,7 +764,7 @@ __global__ __launch_bounds__(kTileThreads, HD == 128 ? 2 : 4) void k_paged_attn_
     if (lo >= hi && !a.direct) {
 #pragma unroll
         for (int k = 0; k < MT; k++)
-            if (r[k].live && g == 0) a.pml[part_of(a, set, r[k].row, r[k].head, split)] = make_float2(-INFINITY, 0.0f);
+            if (r[k].live && g == 0) a.pml[part_of(a, r[k].row, r[k].head, split)] = make_float2(-INFINITY, 0.0f);
         return;
     }
 #pragma unroll
@@ -773,7 +875,7 @@ __global__ __launch_bounds__(kTileThreads, HD == 128 ? 2 : 4) void k_paged_attn_
             f = L != 0.0f ? 1.0f / L : 0.0f;
             dst = a.out + (size_t)r[k].row * a.out_ld + (size_t)r[k].head * HD;
         } else {
-            const size_t at = part_of(a, set, r[k].row, r[k].head, split);
+            const size_t at = part_of(a, r[k].row, r[k].head, split);
             dst = a.po + at * HD;
             if (g == 0) a.pml[at] = make_float2(r[k].m == -INFINITY && L != 0.0f ? 0.0f : r[k].m, L);
         }
@@ -792,54 +894,79 @@ __global__ __launch_bounds__(kTileThreads, HD == 128 ? 2 : 4) void k_paged_attn_
     }
 }
 
-// Partial results of rows, `n` of them per row and head (0: none).
+// Where one list of partial results begins and how far its entries are apart.
 struct Parts {
     const float* po; const float2* pml;
-    int stride, first, n;
+    size_t first; int step, n;
 };
 
 // Joins the partial results of one row and head: weights 2^(m - max), a
 // quarter of the parts per wavefront, HD / 64 (or one) dimensions per lane.
-// A row's own parts come from the kernel that took its sequence, the
-// prefix's stand with those of the tile kernel.
+// `per_seq`: rows of every sequence that the row kernel took (that many of
+// each are looked at); 0: all rows.  Their own parts stand at `rows`, those
+// of the tile kernel (tile_parts, 0: it wrote `out`) and over the prefix at a.po.
 template <int HD>
-__global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttn a, Parts rows, Parts tile, Parts prefix) {
+__global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttn a, int per_seq, const float* rows_po, const float2* rows_pml,
+                                                         int tile_parts, int prefix_parts) {
     constexpr int E = HD < 64 ? 1 : HD / 64;
     __shared__ float so[4][HD], sl[4], sm[4];
-    const int unit = blockIdx.x / a.p.n_heads, head = blockIdx.x % a.p.n_heads;
+    const int at = blockIdx.x / a.p.n_heads, head = blockIdx.x % a.p.n_heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    // the row: of the batch, or only of what the row kernel took
-    const bool all = tile.n + prefix.n > 0 || !a.per_seq;
-    const int s = all ? paged_seq_of_row(a.p, unit) : unit / a.per_seq;
+    const int s = per_seq ? at / per_seq : paged_seq_of_row(a.p, at);
     if (s < 0) return;
     int first, end;
     paged_rows(a.p, s, &first, &end);
-    const int row = all ? unit : first + unit % a.per_seq;
+    const int row = per_seq ? first + at % per_seq : at;
     if (row < first || row >= end) return;
-    const bool by_rows = !a.both || row_kernel_takes(end - first, a.group);
-    const Parts own = by_rows ? rows : tile;
-    if (own.n + prefix.n == 0) return;         // written by its kernel
-    const size_t oat = ((size_t)(by_rows && a.per_seq ? s * a.per_seq + (row - first) : row) * a.p.n_heads + head) * own.stride + own.first;
-    const size_t pat = ((size_t)row * a.p.n_heads + head) * prefix.stride + prefix.first;
-    const int parts = own.n + prefix.n;
-    const auto ml = [&](int i) { return i < own.n ? own.pml[oat + i] : prefix.pml[pat + (i - own.n)]; };
+    Parts own{a.po, a.pml, ((size_t)row * a.p.n_heads + head) * a.parts, 1, tile_parts};
+    if (!a.both || row_kernel_takes(end - first, a.group)) {
+        const int k = (row - first) * a.group + head % a.group, tile = k / kRowTile;
+        int4 u = a.wanted ? a.units[s] : make_int4(s * a.per, 1, 0, 0);
+        if (u.y == 1 && !prefix_parts) return;             // written by its kernel
+        const int64_t unit = (int64_t)u.x + (int64_t)tile * u.y;
+        if (u.x < 0 || u.y < 1 || unit + u.y > a.max_units) return;    // (starts that do not ascend)
+        own = Parts{rows_po, rows_pml, ((size_t)unit * a.p.n_kv + head / a.group) * kRowTile + k % kRowTile, a.p.n_kv * kRowTile, u.y};
+    } else if (tile_parts + prefix_parts == 0) {
+        return;
+    }
+    const Parts pre{a.po, a.pml, ((size_t)row * a.p.n_heads + head) * a.parts + tile_parts, 1, prefix_parts};
+    const int parts = own.n + pre.n;
+    const auto index = [&](int i) { return i < own.n ? own.first + (size_t)i * own.step : pre.first + (size_t)(i - own.n); };
+    const auto ml = [&](int i) { return (i < own.n ? own.pml : pre.pml)[index(i)]; };
     float M = -INFINITY;
     for (int i = tid; i < parts; i += 256) M = fmaxf(M, ml(i).x);
     M = wave_max(M);
     if (lane == 0) sm[wave] = M;
     __syncthreads();
     M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+    // 64 parts' weights at a time, one per lane; eight parts' values in flight
+    // (a part that is not there has weight 0, its values are not looked at)
     float L = 0.0f, o[E] = {};
-    for (int i = wave; i < parts; i += 4) {
-        const float2 v = ml(i);
-        if (v.x == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(v.x - M);
-        const float* po = i < own.n ? own.po + (oat + i) * HD : prefix.po + (pat + (i - own.n)) * HD;
-        L = fmaf(v.y, f, L);
+    const int per = (parts + 3) / 4, i0 = wave * per, i1 = min(parts, i0 + per);
+    for (int b = i0; b < i1; b += 64) {
+        const float2 v = b + lane < i1 ? ml(b + lane) : make_float2(-INFINITY, 0.0f);
+        const float w = v.x == -INFINITY ? 0.0f : v.x == M ? 1.0f : __builtin_amdgcn_exp2f(v.x - M);
+        L += w == 0.0f ? 0.0f : w * v.y;
+        const int n = min(64, i1 - b);
+        for (int j = 0; j < n; j += 8) {
+            float x[8][E];
 #pragma unroll
-        for (int e = 0; e < E; e++)
-            if (HD >= 64 || lane < HD) o[e] = fmaf(po[E * lane + e], f, o[e]);
+            for (int k = 0; k < 8; k++) {
+                const int i = b + min(j + k, n - 1);
+                const float* po = (i < own.n ? own.po : pre.po) + index(i) * HD;
+#pragma unroll
+                for (int e = 0; e < E; e++) x[k][e] = po[E * min(lane, HD / E - 1) + e];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float f = j + k < n ? lane_value(w, j + k) : 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (f != 0.0f) o[e] = fmaf(x[k][e], f, o[e]);
+            }
+        }
     }
+    for (int off = 32; off > 0; off >>= 1) L += __shfl_xor(L, off, 64);
     if (lane == 0) sl[wave] = L;
 #pragma unroll
     for (int e = 0; e < E; e++)
@@ -858,13 +985,15 @@ namespace {
 
 // How a call is split, from what the host knows of it.
 struct Launch {
-    int tiles = 0, splits = 0, chunk = 0;
+    int tiles = 0, splits = 1, chunk = 0;
 };
 struct AttnPlan {
-    Launch rows, tile, prefix;       // own pages: short sequences, long ones; the prefix
-    int per = 0;                     // slots of a sequence in the row kernel (0: as its rows need)
+    int per = 1, wanted = 0, max_units = 0;          // row kernel, own pages (PagedAttn)
+    bool join_rows = false, both = false;
+    int per_seq = 0;                                 // joining only what the row kernel took: rows of a sequence
+    Launch tile, prefix;                             // tile kernel, own pages; the prefix
     bool prefix_by_tile = false;
-    int per_seq = 0, rows_parts = 0, tile_parts = 0;
+    int tile_parts = 0;
     size_t row_units = 0, all_units = 0, bytes = 0;
 };
 
@@ -872,39 +1001,48 @@ struct AttnPlan {
 template <typename C> constexpr int tile_mt(int hd) { return 1; }
 int tile_rows(int dtype, int hd) { return 128 * (dtype == YL_T_F32 ? tile_mt<float>(hd) : dtype == YL_T_F16 ? tile_mt<_Float16>(hd) : tile_mt<__bf16>(hd)); }
 
+constexpr int kUnsplit = 640;        // own positions up to which a tile's are not split
+constexpr int kLeastChunk = 128;
+
 AttnPlan plan_attention(const PagedArgs& p, int dtype, uint32_t max_len) {
     AttnPlan r;
     const int group = p.n_heads / p.n_kv, R = tile_rows(dtype, p.hd);
     const int64_t cap = paged_capacity(p), stacked = (int64_t)p.n_rows * group;
     const int64_t longest = max_len && max_len < cap ? max_len : cap;
     const int own = (int)std::max<int64_t>(longest - p.prefix_len, 0);
-    const auto split = [&](Launch* l, int positions, int wanted, int least) {
-        const int64_t want = std::max<int64_t>(wanted / std::max<int64_t>((int64_t)l->tiles * p.n_kv, 1), 1);
-        l->splits = (int)std::clamp<int64_t>(want, 1, std::max(1, (positions + least - 1) / least));
-        l->chunk = ((positions + l->splits - 1) / l->splits + 127) & ~127;
+    // splits the positions of `tiles` tiles so that `wanted` workgroups have work
+    const auto split = [&](Launch* l, int64_t tiles, int positions, int wanted) {
+        const int64_t want = std::max<int64_t>(wanted / std::max<int64_t>(tiles * p.n_kv, 1), 1);
+        l->splits = (int)std::clamp<int64_t>(want, 1, std::max(1, (positions + kLeastChunk - 1) / kLeastChunk));
+        l->chunk = ((positions + l->splits - 1) / l->splits + 63) & ~63;
+        l->splits = std::max(1, (positions + l->chunk - 1) / std::max(l->chunk, 1));
     };
-    const bool both = p.row_start && stacked > kRowKernelRows;
-    r.per = both ? kRowKernelRows / kRowTile : p.row_start ? 0 : (group + kRowTile - 1) / kRowTile;
-    r.rows.tiles = r.per ? p.n_seqs * r.per : (int)(stacked / kRowTile) + p.n_seqs;
-    split(&r.rows, own, 2048, 256);
-    if (both) {
+    const int resident = p.hd == 128 ? 256 : 512;    // workgroups of the tile kernel that run at once
+    r.both = p.row_start && stacked > kRowKernelRows;
+    r.per = p.row_start ? kRowKernelRows / kRowTile : (group + kRowTile - 1) / kRowTile;
+    r.wanted = own > kUnsplit ? std::max(std::max(1, 512 / p.n_kv), 2 * p.n_seqs * r.per) : 0;
+    r.max_units = p.n_seqs * r.per + r.wanted;
+    r.join_rows = r.wanted || p.prefix_len;
+    if (r.both) {
         r.tile.tiles = (int)(stacked / R) + p.n_seqs;
-        split(&r.tile, own, 512, 512);
+        split(&r.tile, (stacked + R - 1) / R, own, resident);
     }
     if (p.prefix_len) {
         r.prefix_by_tile = stacked > kRowKernelRows;
         r.prefix.tiles = (int)((stacked + (r.prefix_by_tile ? R : kRowTile) - 1) / (r.prefix_by_tile ? R : kRowTile));
-        split(&r.prefix, p.prefix_len, r.prefix_by_tile ? 512 : 2048, 256);
+        split(&r.prefix, r.prefix.tiles, p.prefix_len, r.prefix_by_tile ? resident : 512);
+    } else {
+        r.prefix.splits = 0;
     }
-    // partial results: of the row kernel, for as many rows as it can take of
-    // the sequences if that is less than all; of the others, for every row
-    r.per_seq = row_kernel_tokens(group);
-    if ((int64_t)p.n_seqs * r.per_seq >= p.n_rows) r.per_seq = 0;
-    r.rows_parts = r.rows.splits > 1 || p.prefix_len ? r.rows.splits : 0;
-    r.tile_parts = r.tile.splits > 1 || (p.prefix_len && r.tile.tiles) ? r.tile.splits : 0;
-    r.row_units = (size_t)(r.per_seq ? p.n_seqs * r.per_seq : p.n_rows) * p.n_heads * r.rows_parts;
+    // partial results: of the row kernel, 16 rows for every unit and kv head;
+    // of the others, for every row
+    r.tile_parts = r.tile.splits > 1 || p.prefix_len ? r.tile.splits : 0;
+    if (r.join_rows) r.row_units = (size_t)r.max_units * p.n_kv * kRowTile;
     r.all_units = (size_t)p.n_rows * p.n_heads * (r.tile_parts + r.prefix.splits);
+    r.per_seq = std::max(1, kRowKernelRows / group);
+    if (r.all_units || (int64_t)p.n_seqs * r.per_seq >= p.n_rows) r.per_seq = 0;
     r.bytes = (r.row_units + r.all_units) * (p.hd + 2) * sizeof(float);
+    if (r.wanted) r.bytes = ((r.bytes + 15) & ~(size_t)15) + (size_t)p.n_seqs * sizeof(int4);
     return r;
 }
 
@@ -916,10 +1054,7 @@ hipError_t launch_attn_hd(const PagedAttn& a, const dim3& grid, bool by_tile, bo
 }
 
 template <typename C>
-hipError_t launch_attn(PagedAttn a, const Launch& l, bool by_tile, bool prefix, hipStream_t s) {
-    a.splits = l.splits;
-    a.chunk = l.chunk;
-    const dim3 grid((unsigned)l.tiles * a.p.n_kv, l.splits);
+hipError_t launch_attn(const PagedAttn& a, const dim3& grid, bool by_tile, bool prefix, hipStream_t s) {
     return a.p.hd == 32 ? launch_attn_hd<C, 32>(a, grid, by_tile, prefix, s) : a.p.hd == 64 ? launch_attn_hd<C, 64>(a, grid, by_tile, prefix, s)
                                                                            : launch_attn_hd<C, 128>(a, grid, by_tile, prefix, s);
 }
@@ -930,32 +1065,30 @@ hipError_t launch_all(PagedAttn a, const AttnPlan& plan, float* space, hipStream
     float* const all_po = space + plan.row_units * a.p.hd;
     float2* const ml = reinterpret_cast<float2*>(space + units * a.p.hd);
     float2* const all_ml = ml + plan.row_units;
-    const int all_parts = plan.tile_parts + plan.prefix.splits;
-    a.both = plan.tile.tiles > 0;
-    a.per = plan.per;
+    a.both = plan.both;
+    a.per = plan.per; a.wanted = plan.wanted; a.max_units = plan.max_units;
+    a.units = reinterpret_cast<int4*>(reinterpret_cast<char*>(space) + (plan.bytes - (size_t)a.p.n_seqs * sizeof(int4)));
     a.po = space; a.pml = ml;
-    a.parts = plan.rows_parts; a.per_seq = plan.per_seq;
-    a.direct = !plan.rows_parts;
-    hipError_t e = launch_attn<C>(a, plan.rows, false, false, s);
+    a.direct = !a.p.prefix_len;
+    a.chunk = kLeastChunk;
+    hipError_t e = launch_attn<C>(a, dim3((unsigned)plan.max_units * a.p.n_kv), false, false, s);
     a.po = all_po; a.pml = all_ml;
-    a.parts = all_parts; a.per_seq = 0;
-    if (e == hipSuccess && plan.tile.tiles) {
+    a.parts = plan.tile_parts + plan.prefix.splits;
+    if (e == hipSuccess && plan.both) {
         a.direct = !plan.tile_parts;
-        e = launch_attn<C>(a, plan.tile, true, false, s);
+        a.splits = plan.tile.splits; a.chunk = plan.tile.chunk;
+        e = launch_attn<C>(a, dim3((unsigned)plan.tile.tiles * a.p.n_kv, plan.tile.splits), true, false, s);
     }
-    if (e == hipSuccess && plan.prefix.tiles) {
+    if (e == hipSuccess && a.p.prefix_len) {
         a.direct = 0;
         a.part0 = plan.tile_parts;
-        e = launch_attn<C>(a, plan.prefix, plan.prefix_by_tile, true, s);
+        a.splits = plan.prefix.splits; a.chunk = plan.prefix.chunk;
+        e = launch_attn<C>(a, dim3((unsigned)plan.prefix.tiles * a.p.n_kv, plan.prefix.splits), plan.prefix_by_tile, true, s);
     }
     if (e != hipSuccess || !units) return e;
-    a.per_seq = plan.per_seq;
-    const Parts rows{space, ml, plan.rows_parts, 0, plan.rows_parts}, tile{all_po, all_ml, all_parts, 0, plan.tile_parts};
-    const Parts prefix{all_po, all_ml, all_parts, plan.tile_parts, plan.prefix.splits};
-    const dim3 grid((unsigned)(all_parts || !plan.per_seq ? a.p.n_rows : a.p.n_seqs * plan.per_seq) * a.p.n_heads);
-    if (a.p.hd == 32) hipLaunchKernelGGL(k_paged_attn_join<32>, grid, dim3(256), 0, s, a, rows, tile, prefix);
-    else if (a.p.hd == 64) hipLaunchKernelGGL(k_paged_attn_join<64>, grid, dim3(256), 0, s, a, rows, tile, prefix);
-    else hipLaunchKernelGGL(k_paged_attn_join<128>, grid, dim3(256), 0, s, a, rows, tile, prefix);
+    const dim3 grid((unsigned)(plan.per_seq ? a.p.n_seqs * plan.per_seq : a.p.n_rows) * a.p.n_heads);
+    auto join = a.p.hd == 32 ? k_paged_attn_join<32> : a.p.hd == 64 ? k_paged_attn_join<64> : k_paged_attn_join<128>;
+    hipLaunchKernelGGL(join, grid, dim3(256), 0, s, a, plan.per_seq, (const float*)space, (const float2*)ml, plan.tile_parts, plan.prefix.splits);
     return hipGetLastError();
 }
 
