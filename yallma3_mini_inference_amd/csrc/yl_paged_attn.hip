@@ -48,6 +48,7 @@ constexpr float kSlack = 8.0f;      // a score may pass the running maximum by t
 // What depends on the cache's type.
 template <typename C> struct Type;
 template <> struct Type<_Float16> {
+    static constexpr uint32_t kOnes = 0x3c003c00u;
     static constexpr int kParts = 2, kTiles = 2;   // parts of an f32 value; 16-position tiles of one step
     // weights are held times 2^6: at most 2^14 with the slack, and a weight's
     // second part keeps its bits down to 2^-30
@@ -73,6 +74,7 @@ template <> struct Type<_Float16> {
     }
 };
 template <> struct Type<__bf16> {
+    static constexpr uint32_t kOnes = 0x3f803f80u;
     static constexpr int kParts = 3, kTiles = 2;
     static constexpr float kBias = 0.0f;
     static __device__ __forceinline__ vf4 mul(u4 a, u4 b, vf4 c) {
@@ -305,8 +307,11 @@ __device__ __forceinline__ bool unit_of(const PagedAttn& a, int u, Unit* r) {
 }
 
 // 16 stacked rows in a wavefront: lane (c, g) holds of row c the query parts,
-// the sums of dimensions (4g + i) NJ + j and those of its positions.
-template <typename C, int HD>
+// the sums acc[j][i] of dimensions dim(i, j) and those of its positions.
+// LDS: V^T's operands come transposed from LDS (f16 and bf16), a lane's
+// dimensions are 16 apart, and a matrix product with ones adds up the weights;
+// otherwise from whole rows in registers, NJ neighbouring dimensions per lane.
+template <typename C, int HD, bool LDS>
 struct Tile {
     using T = Type<C>;
     static constexpr bool F32 = sizeof(C) == 4;
@@ -315,13 +320,15 @@ struct Tile {
     static constexpr int NK = F32 ? HD / 16 : HD / 32;       // 16-byte pieces of a key per lane
     static constexpr int KD = F32 ? 16 : 32, KE = F32 ? 4 : 8;   // dimensions per piece of all lane groups, of one
     static constexpr int VW = NJ * (int)sizeof(C) / 4;       // words of a V row per lane
+    static constexpr bool TR = LDS && !F32;
     typedef Words<VW> Value;
+    static __device__ __forceinline__ int dim(int i, int j, int g) { return TR ? 16 * j + 4 * g + i : (4 * g + i) * NJ + j; }
 
     int row, head, lim;              // lim: positions below it are attended to
     bool live;
     float m, l, unscale;
     u4 qf[NP][NK];
-    vf4 acc[NJ];
+    vf4 acc[NJ], ones;               // ones: sums of the weights (TR)
 
     // Places the tile at stacked rows from `stacked` on.
     __device__ __forceinline__ void place(const PagedAttn& a, const RowSet& set, int stacked, int kvh, int c) {
@@ -333,7 +340,10 @@ struct Tile {
         l = 0.0f;
 #pragma unroll
         for (int j = 0; j < NJ; j++) acc[j] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
+        ones = vf4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    // The sum of row c's weights, in every lane of the row.
+    __device__ __forceinline__ float sum() const { return TR ? ones[0] : group_sum16(l); }
     // What the rows attend to, and the longest and the shortest of them
     // (spare rows follow the longest, so that they need no masks).
     __device__ __forceinline__ void reach(const PagedAttn& a, const RowSet& set, int* most, int* least) {
@@ -414,28 +424,30 @@ struct Tile {
                 if (page[t] < 0 || pos >= min(lim, hi)) s[t][i] = -INFINITY;
             }
     }
-    // scores -> weights, under a maximum that is raised where it has to be
-    __device__ __forceinline__ void weigh(float s[NT][4]) {
+    // scores -> weights of N tiles of positions, under a maximum that is raised where it has to be
+    template <int N>
+    __device__ __forceinline__ void weigh(float (*s)[4]) {
         float mx = s[0][0];
 #pragma unroll
-        for (int t = 0; t < NT; t++)
+        for (int t = 0; t < N; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[t][i]);
         if (__ballot(mx * unscale > m + kSlack)) {    // (m = -inf: any score raises it)
             const float m_new = fmaxf(m, group_max16(mx) * unscale);
             const float alpha = m_new == m ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
-            l *= alpha;
+            if constexpr (TR) ones *= alpha;
+            else l *= alpha;
 #pragma unroll
             for (int j = 0; j < NJ; j++) acc[j] *= alpha;
             m = m_new;
         }
         const float back = T::kBias - (m == -INFINITY ? 0.0f : m);
 #pragma unroll
-        for (int t = 0; t < NT; t++)
+        for (int t = 0; t < N; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], unscale, back));
-                l += s[t][i];
+                if constexpr (!TR) l += s[t][i];
             }
     }
     // V^T's operands: of f16 and bf16, dimension j's halves of the 8 positions
@@ -456,21 +468,26 @@ struct Tile {
                 for (int j = 0; j < NJ; j++)
                     acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[0][i].w[j]), s[0][i], acc[j], 0, 0, 0);
         } else {
-            u4 pf[NP];
-#pragma unroll
-            for (int d = 0; d < 4; d++) {
-                uint32_t part[NP];
-                T::cut(s[d >> 1][2 * (d & 1)], s[d >> 1][2 * (d & 1) + 1], part);
-#pragma unroll
-                for (int p = 0; p < NP; p++) pf[p][d] = part[p];
-            }
             u4 vf[NJ];
 #pragma unroll
             for (int j = 0; j < NJ; j++) vf[j] = operand(vr, j);
+            add(s, vf);
+        }
+    }
+    __device__ __forceinline__ void add(const float s[NT][4], const u4 vf[NJ]) {
+        u4 pf[NP];
 #pragma unroll
-            for (int p = NP - 1; p >= 0; p--)
+        for (int d = 0; d < 4; d++) {
+            uint32_t part[NP];
+            T::cut(s[d >> 1][2 * (d & 1)], s[d >> 1][2 * (d & 1) + 1], part);
 #pragma unroll
-                for (int j = 0; j < NJ; j++) acc[j] = T::mul(vf[j], pf[p], acc[j]);
+            for (int p = 0; p < NP; p++) pf[p][d] = part[p];
+        }
+#pragma unroll
+        for (int p = NP - 1; p >= 0; p--) {
+            if constexpr (TR) ones = T::mul(u4{T::kOnes, T::kOnes, T::kOnes, T::kOnes}, pf[p], ones);
+#pragma unroll
+            for (int j = 0; j < NJ; j++) acc[j] = T::mul(vf[j], pf[p], acc[j]);
         }
     }
     // Adds the values that are no numbers (clear_values has taken them out)
@@ -493,12 +510,12 @@ struct Tile {
             for (int tt = 1; tt < NT; tt++)
                 if (t == tt) pg = page[tt];
             if (pg < 0 || p0 + pos >= min(lim, hi)) continue;
-            const C* v = static_cast<const C*>(a.p.values) + paged_offset(a.p, pg, kvh, (p0 + pos) & slots) + (size_t)4 * g * NJ;
+            const C* v = static_cast<const C*>(a.p.values) + paged_offset(a.p, pg, kvh, (p0 + pos) & slots);
 #pragma unroll
             for (int ii = 0; ii < 4; ii++)
 #pragma unroll
                 for (int j = 0; j < NJ; j++) {
-                    const float x = (float)v[ii * NJ + j];
+                    const float x = (float)v[dim(ii, j, g)];
                     if (!(fabsf(x) < INFINITY)) acc[j][ii] = fmaf(w, x, acc[j][ii]);
                 }
         }
@@ -508,8 +525,8 @@ struct Tile {
 // Clears values that are not there, and among positions that not every row
 // attends to those that are no numbers; true if there was one of the latter.
 template <typename C, int HD>
-__device__ __forceinline__ bool clear_values(typename Tile<C, HD>::Value vr[Tile<C, HD>::NT][4], int p0, int hi, bool differ, const int page[], int g) {
-    using R = Tile<C, HD>;
+__device__ __forceinline__ bool clear_values(typename Tile<C, HD, false>::Value vr[Tile<C, HD, false>::NT][4], int p0, int hi, bool differ, const int page[], int g) {
+    using R = Tile<C, HD, false>;
     uint32_t odd = 0;
 #pragma unroll
     for (int t = 0; t < R::NT; t++)
@@ -527,6 +544,28 @@ __device__ __forceinline__ bool clear_values(typename Tile<C, HD>::Value vr[Tile
                 vr[t][i].w[w] = x;
             }
         }
+    return __ballot(odd != 0) != 0;
+}
+
+// The same of transposed operands: word d of each holds positions 16 (d / 2) + 4g + 2 (d % 2) and the next.
+template <typename C, int HD>
+__device__ __forceinline__ bool clear_operands(u4 vf[HD / 16], int p0, int hi, bool differ, const int page[2], int g) {
+    uint32_t odd = 0;
+#pragma unroll
+    for (int d = 0; d < 4; d++) {
+        const int pos = p0 + 16 * (d >> 1) + 4 * g + 2 * (d & 1), n = page[d >> 1] >= 0 ? hi - pos : 0;
+        const uint32_t held = n >= 2 ? ~0u : n == 1 ? 0xffffu : 0u;
+#pragma unroll
+        for (int j = 0; j < HD / 16; j++) {
+            uint32_t x = vf[j][d] & held;
+            if (differ) {
+                const uint32_t bad = Type<C>::not_finite(x);
+                odd |= bad;
+                x &= ~bad;
+            }
+            vf[j][d] = x;
+        }
+    }
     return __ballot(odd != 0) != 0;
 }
 
@@ -559,7 +598,7 @@ __device__ __forceinline__ size_t part_of(const PagedAttn& a, int row, int head,
 // the cache meets about as many operations as the matrix cores need.
 template <typename C, int HD>
 __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int prefix) {
-    using R = Tile<C, HD>;
+    using R = Tile<C, HD, false>;
     constexpr int NT = R::NT, NK = R::NK, NJ = R::NJ, STEP = R::STEP, LD = HD + 4, W = 4;
     __shared__ __align__(16) float so[4][kRowTile][LD];
     __shared__ float sm[4][kRowTile], sl[4][kRowTile];
@@ -658,7 +697,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
             r.mask(s, p0, hi, page, g);
             odd = clear_values<C, HD>(vr, p0, hi, p0 + STEP > least, page, g);
         }
-        r.weigh(s);
+        r.template weigh<NT>(s);
         r.add(s, vr);
         if (odd) r.add_odd(a, s, p0, hi, page, kvh, c, g);
 #pragma unroll
@@ -673,12 +712,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
     }
 
     // the wavefronts' results together
-    const float l = group_sum16(r.l);
+    const float l = r.sum();
     if (g == 0) { sm[wave][c] = r.m; sl[wave][c] = l; }
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < NJ; j++) so[wave][c][(4 * g + i) * NJ + j] = r.acc[j][i];
+        for (int j = 0; j < NJ; j++) so[wave][c][R::dim(i, j, g)] = r.acc[j][i];
     __syncthreads();
     const int tr = tid >> 4, e0 = (tid & 15) * NJ;      // row of the tile, NJ neighbouring dimensions
     float M = -INFINITY;
@@ -716,18 +755,27 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
 // DMA brings in while the tile before is computed.  In LDS a row's 16-byte
 // pieces are permuted by the row (piece ^ row), so that the 16 rows that a key
 // operand reads at one piece lie in different banks.
-constexpr int kTileThreads = 512;
+constexpr int kTileWaves = 8;
+// Of 4 rows by 16 columns of halfwords, of which the 16 lanes of a row of the
+// wavefront point to four halfwords each, lane c gets column c.
+__device__ __forceinline__ u2 load_transposed(const char* p) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p));
+}
 // 16 bytes per lane from `src` to LDS at `dst` + 16 lane
 __device__ __forceinline__ void load_to_lds(const char* src, char* dst) { __builtin_amdgcn_global_load_lds(src, dst, 16, 0, 0); }
 template <typename C, int HD, int MT>
-__global__ __launch_bounds__(kTileThreads, HD == 128 ? 2 : 4) void k_paged_attn_tile(PagedAttn a, int prefix) {
-    using R = Tile<C, HD>;
+__global__ __launch_bounds__(64 * kTileWaves, HD == 128 ? 2 : 4) void k_paged_attn_tile(PagedAttn a, int prefix) {
+    using R = Tile<C, HD, true>;
     constexpr int NT = R::NT, NK = R::NK, NJ = R::NJ, STEP = R::STEP;
     constexpr int RB = HD * (int)sizeof(C), PIECES = RB / 16;          // bytes and pieces of a row
     constexpr int POS = sizeof(C) == 4 ? 32 : 64;                      // positions of a tile
     constexpr int PER = PIECES >= 16 ? 1 : 16 / PIECES;                // rows of 256 bytes
     constexpr int SWZ = PIECES >= 16 ? 15 : PIECES - 1;
-    constexpr int ROWS = 8 * 16 * MT;
+    // values: f16 and bf16, transposed reads take 32 bytes of 16 rows, of which
+    // eight rows then lie in different banks; f32, 16 lanes read a whole row
+    constexpr int VSWZ = R::TR ? PIECES / 2 - 1 : PIECES >= 16 ? 0 : SWZ, VUNIT = R::TR ? 2 : 1;
+    constexpr int ROWS = kTileWaves * 16 * MT;
     __shared__ __align__(16) char lds[2][2][POS * RB];                 // [buffer][keys, values]
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -757,7 +805,7 @@ __global__ __launch_bounds__(kTileThreads, HD == 128 ? 2 : 4) void k_paged_attn_
     __syncthreads();
     int all = reach[0];
 #pragma unroll
-    for (int w = 1; w < 8; w++) all = max(all, reach[w]);
+    for (int w = 1; w < kTileWaves; w++) all = max(all, reach[w]);
     __syncthreads();
     int lo, hi;
     split_range(a, split, all, &lo, &hi);
@@ -777,35 +825,45 @@ __global__ __launch_bounds__(kTileThreads, HD == 128 ? 2 : 4) void k_paged_attn_
     constexpr int S = POS / 16;
     int page_reg = pages_from(lo + 16 * lane), next_reg = page_reg;
     // Brings a tile's keys and values into a buffer: RB bytes per position, 1024 per instruction.
+    const int prow = lane / PIECES, piece = lane % PIECES;
+    constexpr int PI = 1024 / RB, N = POS / PI;                // positions per instruction, instructions
     const auto fetch = [&](int t, int reg, int buffer) {
-        constexpr int PI = 1024 / RB, N = POS / PI;            // positions per instruction, instructions
-        const int prow = lane / PIECES, piece = lane % PIECES;
 #pragma unroll
-        for (int n = 0; n < (2 * N + 7) / 8; n++) {
-            const int i = wave + 8 * n;
+        for (int n = 0; n < (2 * N + kTileWaves - 1) / kTileWaves; n++) {
+            const int i = wave + kTileWaves * n;
             if (i < 2 * N) {
-                const int k = i < N ? i : i - N, row = k * PI + prow;
-                const int page = __builtin_amdgcn_readlane(reg, (t % (64 / S)) * S + k * PI / 16);
-                const char* src = static_cast<const char*>(i < N ? a.p.keys : a.p.values) +
-                                  paged_offset(a.p, max(page, 0), kvh, (lo + POS * t + row) & slots) * sizeof(C) + 16 * (piece ^ ((row / PER) & SWZ));
-                load_to_lds(src, &lds[buffer][i < N ? 0 : 1][k * 1024]);
+                const bool key = i < N;
+                const int row = (key ? i : i - N) * PI;        // of the tile, the instruction's first
+                const int page = __builtin_amdgcn_readlane(reg, (t % (64 / S)) * S + row / 16);
+                const char* src = static_cast<const char*>(key ? a.p.keys : a.p.values) +
+                                  paged_offset(a.p, max(page, 0), kvh, (lo + POS * t + row) & slots) * sizeof(C);
+                const int r16 = (row + prow) & 15;
+                const uint32_t at = prow * RB + 16 * (piece ^ (key ? (r16 / PER) & SWZ : VUNIT * ((r16 / PER) & VSWZ)));
+                load_to_lds(src + at, &lds[buffer][key ? 0 : 1][row * RB]);
             }
         }
     };
-    // where a lane's pieces of a key, and of a value at each of its four
-    // positions, stand in a stretch of 16 positions (the permutation repeats)
-    static_assert((16 / PER) % (SWZ + 1) == 0, "16 positions hold whole permutations");
+    // where a lane's pieces of a key, and of its values, stand in a stretch of
+    // 16 positions (the permutations repeat)
+    static_assert((16 / PER) % (SWZ + 1) == 0 && (16 / PER) % (VSWZ + 1) == 0, "16 positions hold whole permutations");
     constexpr int VB = 4 * R::VW, VH = VB > 16 ? VB / 16 : 1;
-    int k_at[NK], v_at[4][VH];
+    int k_at[NK], v_at[R::TR ? NJ : 4 * VH];
 #pragma unroll
     for (int i = 0; i < NK; i++) k_at[i] = c * RB + 16 * ((4 * i + g) ^ ((c / PER) & SWZ));
+    if constexpr (R::TR) {
+        // of the 4 rows by 16 dimensions that 16 lanes transpose, lane c brings row c / 4, dimensions 4 (c % 4) on
+        const int row = 4 * g + c / 4, f = (row / PER) & VSWZ;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+        for (int j = 0; j < NJ; j++) v_at[j] = row * RB + 32 * (j ^ f) + 8 * (c & 3);
+    } else {
 #pragma unroll
-        for (int h = 0; h < VH; h++) {
-            const int row = 4 * g + i, at = c * VB + 16 * h;
-            v_at[i][h] = row * RB + 16 * ((at / 16) ^ ((row / PER) & SWZ)) + at % 16;
-        }
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int h = 0; h < VH; h++) {
+                const int row = 4 * g + i, at = c * VB + 16 * h;
+                v_at[i * VH + h] = row * RB + 16 * ((at / 16) ^ ((row / PER) & VSWZ)) + at % 16;
+            }
+    }
     fetch(0, page_reg, 0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     lds_barrier();
@@ -817,47 +875,78 @@ __global__ __launch_bounds__(kTileThreads, HD == 128 ? 2 : 4) void k_paged_attn_
         }
         const char* kt = lds[buffer][0];
         const char* vt = lds[buffer][1];
+        // a whole tile of positions per row tile at once: independent chains of
+        // products, one look at the maximum
+        constexpr int NS = POS / STEP;
+        const int p0 = lo + POS * t;
+        if (p0 < min(wave_most, hi)) {
+            int page[NS][NT];
+            bool edge = p0 + POS > min(wave_least, hi);
 #pragma unroll
-        for (int st = 0; st < POS / STEP; st++) {
-            const int p0 = lo + POS * t + STEP * st;
-            if (p0 >= min(wave_most, hi)) break;
-            int page[NT];
-            u4 kc[NT][NK];
-            typename R::Value vr[NT][4];
+            for (int st = 0; st < NS; st++)
 #pragma unroll
-            for (int u = 0; u < NT; u++) {
-                page[u] = __builtin_amdgcn_readlane(page_reg, (t % (64 / S)) * S + st * NT + u);
+                for (int u = 0; u < NT; u++) {
+                    page[st][u] = __builtin_amdgcn_readlane(page_reg, (t % (64 / S)) * S + st * NT + u);
+                    edge = edge || page[st][u] < 0;
+                }
+            float s[MT][NS][NT][4];
 #pragma unroll
-                for (int i = 0; i < NK; i++) kc[u][i] = *reinterpret_cast<const u4*>(kt + (STEP * st + 16 * u) * RB + k_at[i]);
+            for (int st = 0; st < NS; st++) {
+                u4 kc[NT][NK];
+#pragma unroll
+                for (int u = 0; u < NT; u++)
+#pragma unroll
+                    for (int i = 0; i < NK; i++) kc[u][i] = *reinterpret_cast<const u4*>(kt + (STEP * st + 16 * u) * RB + k_at[i]);
+#pragma unroll
+                for (int k = 0; k < MT; k++) {
+                    r[k].scores(kc, s[k][st]);
+                    if (edge) r[k].mask(s[k][st], p0 + STEP * st, hi, page[st], g);
+                }
             }
 #pragma unroll
-            for (int u = 0; u < NT; u++)
+            for (int k = 0; k < MT; k++) r[k].template weigh<NS * NT>(&s[k][0][0]);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const char* v = vt + (STEP * st + 16 * u) * RB;
-                    if constexpr (VB <= 16) {
-                        vr[u][i] = load_words<R::VW>(v + v_at[i][0]);
-                    } else {
+            for (int st = 0; st < NS; st++) {
+                const int ps = p0 + STEP * st;
+                bool odd = false;
+                if constexpr (R::TR) {
+                    u4 vf[NJ];
 #pragma unroll
-                        for (int h = 0; h < VH; h++) {
-                            const Words<4> w = load_words<4>(v + v_at[i][h]);
+                    for (int j = 0; j < NJ; j++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++) vr[u][i].w[4 * h + e] = w.w[e];
+                        for (int u = 0; u < NT; u++) {
+                            const u2 x = load_transposed(vt + (STEP * st + 16 * u) * RB + v_at[j]);
+                            vf[j][2 * u] = x[0];
+                            vf[j][2 * u + 1] = x[1];
                         }
-                    }
+                    if (edge) odd = clear_operands<C, HD>(vf, ps, hi, ps + STEP > wave_least, page[st], g);
+#pragma unroll
+                    for (int k = 0; k < MT; k++) r[k].add(s[k][st], vf);
+                } else {
+                    typename R::Value vr[NT][4];
+#pragma unroll
+                    for (int u = 0; u < NT; u++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const char* v = vt + (STEP * st + 16 * u) * RB;
+                            if constexpr (VB <= 16) {
+                                vr[u][i] = load_words<R::VW>(v + v_at[i]);
+                            } else {
+#pragma unroll
+                                for (int h = 0; h < VH; h++) {
+                                    const Words<4> w = load_words<4>(v + v_at[i * VH + h]);
+#pragma unroll
+                                    for (int e = 0; e < 4; e++) vr[u][i].w[4 * h + e] = w.w[e];
+                                }
+                            }
+                        }
+                    if (edge) odd = clear_values<C, HD>(vr, ps, hi, ps + STEP > wave_least, page[st], g);
+#pragma unroll
+                    for (int k = 0; k < MT; k++) r[k].add(s[k][st], vr);
                 }
-            bool edge = p0 + STEP > min(wave_least, hi), odd = false;
+                if (odd)
 #pragma unroll
-            for (int u = 0; u < NT; u++) edge = edge || page[u] < 0;
-            if (edge) odd = clear_values<C, HD>(vr, p0, hi, p0 + STEP > wave_least, page, g);
-#pragma unroll
-            for (int k = 0; k < MT; k++) {
-                float s[NT][4];
-                r[k].scores(kc, s);
-                if (edge) r[k].mask(s, p0, hi, page, g);
-                r[k].weigh(s);
-                r[k].add(s, vr);
-                if (odd) r[k].add_odd(a, s, p0, hi, page, kvh, c, g);
+                    for (int k = 0; k < MT; k++) r[k].add_odd(a, s[k][st], ps, hi, page[st], kvh, c, g);
             }
         }
         page_reg = next_reg;
@@ -867,7 +956,7 @@ __global__ __launch_bounds__(kTileThreads, HD == 128 ? 2 : 4) void k_paged_attn_
 
 #pragma unroll
     for (int k = 0; k < MT; k++) {
-        const float L = group_sum16(r[k].l);
+        const float L = r[k].sum();
         if (!r[k].live) continue;
         float f = 1.0f;
         float* dst;
@@ -879,17 +968,17 @@ __global__ __launch_bounds__(kTileThreads, HD == 128 ? 2 : 4) void k_paged_attn_
             dst = a.po + at * HD;
             if (g == 0) a.pml[at] = make_float2(r[k].m == -INFINITY && L != 0.0f ? 0.0f : r[k].m, L);
         }
+        if constexpr (R::TR) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float* d = dst + (4 * g + i) * NJ;
-            if constexpr (NJ >= 4) {
-#pragma unroll
-                for (int j = 0; j < NJ; j += 4)
-                    *reinterpret_cast<f4u*>(d + j) = f4u{r[k].acc[j][i] * f, r[k].acc[j + 1][i] * f, r[k].acc[j + 2][i] * f, r[k].acc[j + 3][i] * f};
-            } else {
-#pragma unroll
-                for (int j = 0; j < NJ; j++) d[j] = r[k].acc[j][i] * f;
+            for (int j = 0; j < NJ; j++) {
+                const vf4 x = r[k].acc[j] * f;
+                *reinterpret_cast<f4u*>(dst + R::dim(0, j, g)) = f4u{x[0], x[1], x[2], x[3]};
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < NJ; j++) dst[R::dim(i, j, g)] = r[k].acc[j][i] * f;
         }
     }
 }
@@ -999,7 +1088,7 @@ struct AttnPlan {
 
 // Row tiles of 16 per wavefront in the tile kernel: as the registers allow.
 template <typename C> constexpr int tile_mt(int hd) { return 1; }
-int tile_rows(int dtype, int hd) { return 128 * (dtype == YL_T_F32 ? tile_mt<float>(hd) : dtype == YL_T_F16 ? tile_mt<_Float16>(hd) : tile_mt<__bf16>(hd)); }
+int tile_rows(int dtype, int hd) { return 16 * kTileWaves * (dtype == YL_T_F32 ? tile_mt<float>(hd) : dtype == YL_T_F16 ? tile_mt<_Float16>(hd) : tile_mt<__bf16>(hd)); }
 
 constexpr int kUnsplit = 640;        // own positions up to which a tile's are not split
 constexpr int kLeastChunk = 128;
@@ -1048,7 +1137,7 @@ AttnPlan plan_attention(const PagedArgs& p, int dtype, uint32_t max_len) {
 
 template <typename C, int HD>
 hipError_t launch_attn_hd(const PagedAttn& a, const dim3& grid, bool by_tile, bool prefix, hipStream_t s) {
-    if (by_tile) hipLaunchKernelGGL((k_paged_attn_tile<C, HD, tile_mt<C>(HD)>), grid, dim3(kTileThreads), 0, s, a, prefix);
+    if (by_tile) hipLaunchKernelGGL((k_paged_attn_tile<C, HD, tile_mt<C>(HD)>), grid, dim3(64 * kTileWaves), 0, s, a, prefix);
     else hipLaunchKernelGGL((k_paged_attn_rows<C, HD>), grid, dim3(256), 0, s, a, prefix);
     return hipGetLastError();
 }
