@@ -68,6 +68,56 @@ def test_shared_prefix(gpu, dtype, prefix, heads, kvh, hd):
     _check(sc, _attend(sc))
 
 
+# (enough rows and kv heads for the tile kernel: 160 workgroups of 128 stacked rows)
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kvh,hd", [(160, 160, 32), (160, 160, 64), (160, 160, 128), (160, 80, 64)])
+@pytest.mark.parametrize("prefix", [0, 37])
+def test_many_prompt_rows(gpu, dtype, heads, kvh, hd, prefix):
+    """Prompts beside single rows, sequences without rows and rows inside the prefix."""
+    rows = [1, 40, 0, 33, 2, 70] if kvh == 160 else [1, 70, 0, 17, 2, 60]
+    lens = [prefix + n for n in (90, 40, 7, 130, 20, 75)]
+    lens[1] -= prefix // 2
+    sc = Scene(rows, lens, heads, kvh, hd, 16, dtype, prefix=prefix, seed=hd)
+    _check(sc, _attend(sc))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_prompt_rows_over_gaps_and_no_numbers(gpu, dtype, hd):
+    """The tile kernel's masks: missing pages, lengths past the table, later
+    positions that hold no numbers, rows behind the sequences, odd strides."""
+    sc = Scene([50, 70, 3], [50, 300, 64], 160, 160, hd, 16, dtype, seed=hd, extra_entries=1, behind=2)
+    sc.table[1, 3] = -1
+    sc.table[1, 7] = sc.n_pages
+    sc.lens[2] = 16 * sc.table.shape[1] + 500
+    page = sc.table[0, 2]
+    sc.v32[page, :, 5, 3] = np.inf          # position 37 of the first sequence
+    sc.k32[sc.table[0, 2], :, 9] = np.nan   # position 41
+    call = Call(gpu, sc, q_ld=160 * hd + 5, out_ld=160 * hd + 3, offset=1)
+    call()
+    out, between = call.result()
+    n = int(sc.starts[-1])
+    assert (out[n:] == 7.0).all() and (between == 7.0).all()
+    rows = out[:50].reshape(50, 160, hd)
+    assert np.isfinite(rows[:37]).all() and not np.isfinite(rows[37:, :, 3]).any()
+    assert np.isfinite(rows[37:41][..., :3]).all() and not np.isfinite(rows[41:]).any()
+    sc.v32[page, :, 5, 3] = 0.0
+    ref, bound = sc.attention()
+    fine = np.isfinite(out[:n]) & np.isfinite(ref[:n])
+    assert (np.abs(out[:n] - ref[:n])[fine] <= bound[:n][fine]).all()
+    assert fine[:37].all() and fine[50:].all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_long_prefix_under_a_batch(gpu, dtype, hd):
+    """A prefix long enough, under rows enough, for the tile kernel (2^23 stacked rows times positions)."""
+    prefix, seqs = 1010, 36
+    sc = Scene([1] * (seqs - 1) + [9], [prefix + 1 + 7 * i for i in range(seqs)], 192, 32, hd, 32, dtype, prefix=prefix, seed=hd)
+    assert 44 * 6 * 32 * prefix >= 8 << 20
+    _check(sc, _attend(sc))
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_prefix_equals_own_pages(gpu, dtype):
     """The same positions as a prefix and as pages of each sequence's table

@@ -155,11 +155,14 @@ struct PagedAttn {
     int chunk;                       // positions of a split at least
     int splits;
     int direct;                      // this launch sees all that its rows attend to: it writes `out`
-    // the row kernel's own work: tiles of 16 rows a sequence can have; units
-    // wanted (0: a unit per tile, positions never split) and units there is
-    // room for; what each sequence's units are, for the joining kernel
+    // the row kernel's own work: units wanted, beyond one per tile, and units
+    // there is room for; where each sequence's units begin and how many its
+    // tiles have, for the joining kernel.  wanted 0: one row per sequence, a unit
+    // for each of its `per` tiles, positions not split
     int per, wanted, max_units;
+    float finer;                     // units wanted per tile where there are many tiles
     int4* units;
+    int joined;                      // the joining kernel follows
     int both;                        // sequences are divided between the row kernel and the tile kernel
     // partial results, unnormalised, and their maximum (base 2) and sum, maximum
     // -inf: nothing there.  Of the row kernel's own work [unit][n_kv][16 rows],
@@ -229,7 +232,7 @@ __device__ __forceinline__ int limit_of_row(const PagedAttn& a, const RowSet& se
 constexpr int kRowTile = 16;
 
 // Stacked rows of a sequence (tokens times heads per kv head) up to which the
-// row kernel takes it.
+// row kernel takes it where there is work for the tile kernel.
 constexpr int kRowKernelRows = 32;
 __device__ __forceinline__ bool row_kernel_takes(int rows, int group) { return (int64_t)rows * group <= kRowKernelRows; }
 
@@ -249,6 +252,14 @@ __device__ __forceinline__ int scan_add(int x) {       // inclusive, over the 64
     return x;
 }
 
+__device__ __forceinline__ float wave_sum(float x) {   // every lane active
+    x += dpp_mov<0xB1>(x);
+    x += dpp_mov<0x4E>(x);
+    x += dpp_mov<0x141>(x);
+    x += dpp_mov<0x140>(x);
+    return (lane_value(x, 0) + lane_value(x, 16)) + (lane_value(x, 32) + lane_value(x, 48));
+}
+
 // Unit `u` of the batch.  All tiles' positions together, divided by the units
 // wanted, are a unit's share: a long sequence becomes many units, a short one
 // one, whatever the lengths are when the work runs.  Every wavefront works
@@ -264,26 +275,22 @@ __device__ __forceinline__ bool unit_of(const PagedAttn& a, int u, Unit* r) {
         paged_rows(p, s, &first, &end);
         const int n = end - first;
         if (n == 0 || (a.both && !row_kernel_takes(n, a.group))) return;
-        *tiles = min((n * a.group + kRowTile - 1) / kRowTile, a.per);
+        *tiles = (n * a.group + kRowTile - 1) / kRowTile;
         *len = max(paged_limit(p, (int64_t)p.kv_len[s] - 1) - p.prefix_len, 0);
     };
     int tiles, len;
     of_seq(lane, &tiles, &len);
-    float sum = 0.0f;
+    float sum = 0.0f, all = 0.0f;
     for (int s0 = 0;;) {
-        float x = (float)tiles * (float)len;
-        x += dpp_mov<0xB1>(x);
-        x += dpp_mov<0x4E>(x);
-        x += dpp_mov<0x141>(x);
-        x += dpp_mov<0x140>(x);
-        sum += (lane_value(x, 0) + lane_value(x, 16)) + (lane_value(x, 32) + lane_value(x, 48));
+        sum += wave_sum((float)tiles * (float)len);
+        all += wave_sum((float)tiles);
         s0 += 64;
         if (s0 >= p.n_seqs) break;
         of_seq(s0 + lane, &tiles, &len);
     }
     // (rounded up beyond the sum's own rounding, so that the units never are more than there is room for)
-    const float share = sum * 1.001f / (float)a.wanted;
-    const int chunk = share < 1e9f ? (max((int)share + 1, a.chunk) + 63) & ~63 : 1 << 30;
+    const float share = sum * 1.001f / fmaxf((float)a.wanted, a.finer * all);
+    const int chunk = share < 1e9f && a.chunk < 1 << 30 ? (max((int)share + 1, a.chunk) + 63) & ~63 : 1 << 30;
     int before = 0;
     for (int s0 = 0; s0 < p.n_seqs; s0 += 64) {
         if (p.n_seqs > 64) of_seq(s0 + lane, &tiles, &len);
@@ -308,10 +315,10 @@ __device__ __forceinline__ bool unit_of(const PagedAttn& a, int u, Unit* r) {
 
 // 16 stacked rows in a wavefront: lane (c, g) holds of row c the query parts,
 // the sums acc[j][i] of dimensions dim(i, j) and those of its positions.
-// LDS: V^T's operands come transposed from LDS (f16 and bf16), a lane's
+// TR: V^T's operands come transposed from LDS (f16 and bf16), a lane's
 // dimensions are 16 apart, and a matrix product with ones adds up the weights;
 // otherwise from whole rows in registers, NJ neighbouring dimensions per lane.
-template <typename C, int HD, bool LDS>
+template <typename C, int HD, bool TR>
 struct Tile {
     using T = Type<C>;
     static constexpr bool F32 = sizeof(C) == 4;
@@ -320,7 +327,7 @@ struct Tile {
     static constexpr int NK = F32 ? HD / 16 : HD / 32;       // 16-byte pieces of a key per lane
     static constexpr int KD = F32 ? 16 : 32, KE = F32 ? 4 : 8;   // dimensions per piece of all lane groups, of one
     static constexpr int VW = NJ * (int)sizeof(C) / 4;       // words of a V row per lane
-    static constexpr bool TR = LDS && !F32;
+    static_assert(!(TR && F32), "halfwords are transposed");
     typedef Words<VW> Value;
     static __device__ __forceinline__ int dim(int i, int j, int g) { return TR ? 16 * j + 4 * g + i : (4 * g + i) * NJ + j; }
 
@@ -613,7 +620,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
     } else {
         if (a.wanted) {
             if (!unit_of(a, slot, &u)) return;
-            if (slot == u.first && kvh == 0 && tid == 0) a.units[u.seq] = make_int4(u.first, u.splits, 0, 0);
+            if (a.joined && slot == u.first && kvh == 0 && tid == 0) a.units[u.seq] = make_int4(u.first, u.splits, 0, 0);
         } else {
             u.seq = slot / a.per;
             u.first = u.seq * a.per;
@@ -750,12 +757,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
     }
 }
 
-// Many rows over the same pages (prompts, a prefix under a batch): eight
-// wavefronts of MT row tiles each share tiles of K and V in LDS, which LDS
+// Many rows over the same pages (prompts, a prefix under a batch) of an f16 or
+// bf16 cache: eight wavefronts of a row tile each share tiles of K and V in LDS, which LDS
 // DMA brings in while the tile before is computed.  In LDS a row's 16-byte
 // pieces are permuted by the row (piece ^ row), so that the 16 rows that a key
 // operand reads at one piece lie in different banks.
-constexpr int kTileWaves = 8;
+constexpr int kTileWaves = 8, kTileRows = kTileWaves * kRowTile;
 // Of 4 rows by 16 columns of halfwords, of which the 16 lanes of a row of the
 // wavefront point to four halfwords each, lane c gets column c.
 __device__ __forceinline__ u2 load_transposed(const char* p) {
@@ -764,18 +771,16 @@ __device__ __forceinline__ u2 load_transposed(const char* p) {
 }
 // 16 bytes per lane from `src` to LDS at `dst` + 16 lane
 __device__ __forceinline__ void load_to_lds(const char* src, char* dst) { __builtin_amdgcn_global_load_lds(src, dst, 16, 0, 0); }
-template <typename C, int HD, int MT>
+template <typename C, int HD>
 __global__ __launch_bounds__(64 * kTileWaves, HD == 128 ? 2 : 4) void k_paged_attn_tile(PagedAttn a, int prefix) {
     using R = Tile<C, HD, true>;
     constexpr int NT = R::NT, NK = R::NK, NJ = R::NJ, STEP = R::STEP;
     constexpr int RB = HD * (int)sizeof(C), PIECES = RB / 16;          // bytes and pieces of a row
-    constexpr int POS = sizeof(C) == 4 ? 32 : 64;                      // positions of a tile
+    constexpr int POS = 64;                                            // positions of a tile
     constexpr int PER = PIECES >= 16 ? 1 : 16 / PIECES;                // rows of 256 bytes
     constexpr int SWZ = PIECES >= 16 ? 15 : PIECES - 1;
-    // values: f16 and bf16, transposed reads take 32 bytes of 16 rows, of which
-    // eight rows then lie in different banks; f32, 16 lanes read a whole row
-    constexpr int VSWZ = R::TR ? PIECES / 2 - 1 : PIECES >= 16 ? 0 : SWZ, VUNIT = R::TR ? 2 : 1;
-    constexpr int ROWS = kTileWaves * 16 * MT;
+    constexpr int VSWZ = PIECES / 2 - 1;                               // values: 32 bytes of a row, so that eight rows differ
+    constexpr int ROWS = kTileRows;
     __shared__ __align__(16) char lds[2][2][POS * RB];                 // [buffer][keys, values]
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -790,15 +795,10 @@ __global__ __launch_bounds__(64 * kTileWaves, HD == 128 ? 2 : 4) void k_paged_at
     } else if (!tile_of_slot(a, slot, __builtin_ctz(ROWS), &set, &tile) || row_kernel_takes(set.rows, a.group)) {
         return;
     }
-    R r[MT];
-    int most[MT], least[MT], wave_most = 0, wave_least = 0x7fffffff;
-#pragma unroll
-    for (int k = 0; k < MT; k++) {
-        r[k].place(a, set, tile * ROWS + (wave * MT + k) * 16, kvh, c);
-        r[k].reach(a, set, &most[k], &least[k]);
-        wave_most = max(wave_most, most[k]);
-        wave_least = min(wave_least, least[k]);
-    }
+    R r;
+    int wave_most, least;
+    r.place(a, set, tile * ROWS + wave * kRowTile, kvh, c);
+    r.reach(a, set, &wave_most, &least);
     // the longest row of the workgroup
     int* reach = reinterpret_cast<int*>(lds);
     if (lane == 0) reach[wave] = wave_most;
@@ -810,13 +810,10 @@ __global__ __launch_bounds__(64 * kTileWaves, HD == 128 ? 2 : 4) void k_paged_at
     int lo, hi;
     split_range(a, split, all, &lo, &hi);
     if (lo >= hi && !a.direct) {
-#pragma unroll
-        for (int k = 0; k < MT; k++)
-            if (r[k].live && g == 0) a.pml[part_of(a, r[k].row, r[k].head, split)] = make_float2(-INFINITY, 0.0f);
+        if (r.live && g == 0) a.pml[part_of(a, r.row, r.head, split)] = make_float2(-INFINITY, 0.0f);
         return;
     }
-#pragma unroll
-    for (int k = 0; k < MT; k++) r[k].load_q(a, g);
+    r.load_q(a, g);
 
     const int slots = (1 << a.p.page_shift) - 1;
     const int tiles = (hi - lo + POS - 1) / POS;
@@ -838,7 +835,7 @@ __global__ __launch_bounds__(64 * kTileWaves, HD == 128 ? 2 : 4) void k_paged_at
                 const char* src = static_cast<const char*>(key ? a.p.keys : a.p.values) +
                                   paged_offset(a.p, max(page, 0), kvh, (lo + POS * t + row) & slots) * sizeof(C);
                 const int r16 = (row + prow) & 15;
-                const uint32_t at = prow * RB + 16 * (piece ^ (key ? (r16 / PER) & SWZ : VUNIT * ((r16 / PER) & VSWZ)));
+                const uint32_t at = prow * RB + 16 * (piece ^ (key ? (r16 / PER) & SWZ : 2 * ((r16 / PER) & VSWZ)));
                 load_to_lds(src + at, &lds[buffer][key ? 0 : 1][row * RB]);
             }
         }
@@ -846,24 +843,13 @@ __global__ __launch_bounds__(64 * kTileWaves, HD == 128 ? 2 : 4) void k_paged_at
     // where a lane's pieces of a key, and of its values, stand in a stretch of
     // 16 positions (the permutations repeat)
     static_assert((16 / PER) % (SWZ + 1) == 0 && (16 / PER) % (VSWZ + 1) == 0, "16 positions hold whole permutations");
-    constexpr int VB = 4 * R::VW, VH = VB > 16 ? VB / 16 : 1;
-    int k_at[NK], v_at[R::TR ? NJ : 4 * VH];
+    int k_at[NK], v_at[NJ];
 #pragma unroll
     for (int i = 0; i < NK; i++) k_at[i] = c * RB + 16 * ((4 * i + g) ^ ((c / PER) & SWZ));
-    if constexpr (R::TR) {
-        // of the 4 rows by 16 dimensions that 16 lanes transpose, lane c brings row c / 4, dimensions 4 (c % 4) on
-        const int row = 4 * g + c / 4, f = (row / PER) & VSWZ;
+    // (of the 4 rows by 16 dimensions that 16 lanes transpose, lane c brings row c / 4, dimensions 4 (c % 4) on)
+    const int v_row = 4 * g + c / 4, v_swz = (v_row / PER) & VSWZ;
 #pragma unroll
-        for (int j = 0; j < NJ; j++) v_at[j] = row * RB + 32 * (j ^ f) + 8 * (c & 3);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int h = 0; h < VH; h++) {
-                const int row = 4 * g + i, at = c * VB + 16 * h;
-                v_at[i * VH + h] = row * RB + 16 * ((at / 16) ^ ((row / PER) & VSWZ)) + at % 16;
-            }
-    }
+    for (int j = 0; j < NJ; j++) v_at[j] = v_row * RB + 32 * (j ^ v_swz) + 8 * (c & 3);
     fetch(0, page_reg, 0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     lds_barrier();
@@ -881,7 +867,7 @@ __global__ __launch_bounds__(64 * kTileWaves, HD == 128 ? 2 : 4) void k_paged_at
         const int p0 = lo + POS * t;
         if (p0 < min(wave_most, hi)) {
             int page[NS][NT];
-            bool edge = p0 + POS > min(wave_least, hi);
+            bool edge = p0 + POS > min(least, hi);
 #pragma unroll
             for (int st = 0; st < NS; st++)
 #pragma unroll
@@ -889,7 +875,7 @@ __global__ __launch_bounds__(64 * kTileWaves, HD == 128 ? 2 : 4) void k_paged_at
                     page[st][u] = __builtin_amdgcn_readlane(page_reg, (t % (64 / S)) * S + st * NT + u);
                     edge = edge || page[st][u] < 0;
                 }
-            float s[MT][NS][NT][4];
+            float s[NS * NT][4];
 #pragma unroll
             for (int st = 0; st < NS; st++) {
                 u4 kc[NT][NK];
@@ -897,56 +883,25 @@ __global__ __launch_bounds__(64 * kTileWaves, HD == 128 ? 2 : 4) void k_paged_at
                 for (int u = 0; u < NT; u++)
 #pragma unroll
                     for (int i = 0; i < NK; i++) kc[u][i] = *reinterpret_cast<const u4*>(kt + (STEP * st + 16 * u) * RB + k_at[i]);
-#pragma unroll
-                for (int k = 0; k < MT; k++) {
-                    r[k].scores(kc, s[k][st]);
-                    if (edge) r[k].mask(s[k][st], p0 + STEP * st, hi, page[st], g);
-                }
+                r.scores(kc, s + NT * st);
+                if (edge) r.mask(s + NT * st, p0 + STEP * st, hi, page[st], g);
             }
-#pragma unroll
-            for (int k = 0; k < MT; k++) r[k].template weigh<NS * NT>(&s[k][0][0]);
+            r.template weigh<NS * NT>(s);
 #pragma unroll
             for (int st = 0; st < NS; st++) {
                 const int ps = p0 + STEP * st;
-                bool odd = false;
-                if constexpr (R::TR) {
-                    u4 vf[NJ];
+                u4 vf[NJ];
 #pragma unroll
-                    for (int j = 0; j < NJ; j++)
+                for (int j = 0; j < NJ; j++)
 #pragma unroll
-                        for (int u = 0; u < NT; u++) {
-                            const u2 x = load_transposed(vt + (STEP * st + 16 * u) * RB + v_at[j]);
-                            vf[j][2 * u] = x[0];
-                            vf[j][2 * u + 1] = x[1];
-                        }
-                    if (edge) odd = clear_operands<C, HD>(vf, ps, hi, ps + STEP > wave_least, page[st], g);
-#pragma unroll
-                    for (int k = 0; k < MT; k++) r[k].add(s[k][st], vf);
-                } else {
-                    typename R::Value vr[NT][4];
-#pragma unroll
-                    for (int u = 0; u < NT; u++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const char* v = vt + (STEP * st + 16 * u) * RB;
-                            if constexpr (VB <= 16) {
-                                vr[u][i] = load_words<R::VW>(v + v_at[i]);
-                            } else {
-#pragma unroll
-                                for (int h = 0; h < VH; h++) {
-                                    const Words<4> w = load_words<4>(v + v_at[i * VH + h]);
-#pragma unroll
-                                    for (int e = 0; e < 4; e++) vr[u][i].w[4 * h + e] = w.w[e];
-                                }
-                            }
-                        }
-                    if (edge) odd = clear_values<C, HD>(vr, ps, hi, ps + STEP > wave_least, page[st], g);
-#pragma unroll
-                    for (int k = 0; k < MT; k++) r[k].add(s[k][st], vr);
-                }
-                if (odd)
-#pragma unroll
-                    for (int k = 0; k < MT; k++) r[k].add_odd(a, s[k][st], ps, hi, page[st], kvh, c, g);
+                    for (int u = 0; u < NT; u++) {
+                        const u2 x = load_transposed(vt + (STEP * st + 16 * u) * RB + v_at[j]);
+                        vf[j][2 * u] = x[0];
+                        vf[j][2 * u + 1] = x[1];
+                    }
+                const bool odd = edge && clear_operands<C, HD>(vf, ps, hi, ps + STEP > least, page[st], g);
+                r.add(s + NT * st, vf);
+                if (odd) r.add_odd(a, s + NT * st, ps, hi, page[st], kvh, c, g);
             }
         }
         page_reg = next_reg;
@@ -954,32 +909,22 @@ __global__ __launch_bounds__(64 * kTileWaves, HD == 128 ? 2 : 4) void k_paged_at
         lds_barrier();
     }
 
+    const float L = r.sum();
+    if (!r.live) return;
+    float f = 1.0f;
+    float* dst;
+    if (a.direct) {
+        f = L != 0.0f ? 1.0f / L : 0.0f;
+        dst = a.out + (size_t)r.row * a.out_ld + (size_t)r.head * HD;
+    } else {
+        const size_t at = part_of(a, r.row, r.head, split);
+        dst = a.po + at * HD;
+        if (g == 0) a.pml[at] = make_float2(r.m == -INFINITY && L != 0.0f ? 0.0f : r.m, L);
+    }
 #pragma unroll
-    for (int k = 0; k < MT; k++) {
-        const float L = r[k].sum();
-        if (!r[k].live) continue;
-        float f = 1.0f;
-        float* dst;
-        if (a.direct) {
-            f = L != 0.0f ? 1.0f / L : 0.0f;
-            dst = a.out + (size_t)r[k].row * a.out_ld + (size_t)r[k].head * HD;
-        } else {
-            const size_t at = part_of(a, r[k].row, r[k].head, split);
-            dst = a.po + at * HD;
-            if (g == 0) a.pml[at] = make_float2(r[k].m == -INFINITY && L != 0.0f ? 0.0f : r[k].m, L);
-        }
-        if constexpr (R::TR) {
-#pragma unroll
-            for (int j = 0; j < NJ; j++) {
-                const vf4 x = r[k].acc[j] * f;
-                *reinterpret_cast<f4u*>(dst + R::dim(0, j, g)) = f4u{x[0], x[1], x[2], x[3]};
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < NJ; j++) dst[R::dim(i, j, g)] = r[k].acc[j][i] * f;
-        }
+    for (int j = 0; j < NJ; j++) {
+        const vf4 x = r.acc[j] * f;
+        *reinterpret_cast<f4u*>(dst + R::dim(0, j, g)) = f4u{x[0], x[1], x[2], x[3]};
     }
 }
 
@@ -989,17 +934,19 @@ struct Parts {
     size_t first; int step, n;
 };
 
-// Joins the partial results of one row and head: weights 2^(m - max), a
-// quarter of the parts per wavefront, HD / 64 (or one) dimensions per lane.
+// Joins the partial results of `heads` heads of a row, one after the other:
+// weights 2^(m - max), a quarter of the parts per wavefront, HD / 64 (or one)
+// dimensions per lane.
 // `per_seq`: rows of every sequence that the row kernel took (that many of
 // each are looked at); 0: all rows.  Their own parts stand at `rows`, those
 // of the tile kernel (tile_parts, 0: it wrote `out`) and over the prefix at a.po.
 template <int HD>
-__global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttn a, int per_seq, const float* rows_po, const float2* rows_pml,
+__global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttn a, int heads, int per_seq, const float* rows_po, const float2* rows_pml,
                                                          int tile_parts, int prefix_parts) {
     constexpr int E = HD < 64 ? 1 : HD / 64;
     __shared__ float so[4][HD], sl[4], sm[4];
-    const int at = blockIdx.x / a.p.n_heads, head = blockIdx.x % a.p.n_heads;
+    const int groups = (a.p.n_heads + heads - 1) / heads;
+    const int at = blockIdx.x / groups, head0 = (blockIdx.x % groups) * heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int s = per_seq ? at / per_seq : paged_seq_of_row(a.p, at);
     if (s < 0) return;
@@ -1007,64 +954,70 @@ __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttn a, int per_se
     paged_rows(a.p, s, &first, &end);
     const int row = per_seq ? first + at % per_seq : at;
     if (row < first || row >= end) return;
-    Parts own{a.po, a.pml, ((size_t)row * a.p.n_heads + head) * a.parts, 1, tile_parts};
-    if (!a.both || row_kernel_takes(end - first, a.group)) {
-        const int k = (row - first) * a.group + head % a.group, tile = k / kRowTile;
-        int4 u = a.wanted ? a.units[s] : make_int4(s * a.per, 1, 0, 0);
-        if (u.y == 1 && !prefix_parts) return;             // written by its kernel
-        const int64_t unit = (int64_t)u.x + (int64_t)tile * u.y;
-        if (u.x < 0 || u.y < 1 || unit + u.y > a.max_units) return;    // (starts that do not ascend)
-        own = Parts{rows_po, rows_pml, ((size_t)unit * a.p.n_kv + head / a.group) * kRowTile + k % kRowTile, a.p.n_kv * kRowTile, u.y};
-    } else if (tile_parts + prefix_parts == 0) {
-        return;
+    const bool by_rows = !a.both || row_kernel_takes(end - first, a.group);
+    int4 u = make_int4(0, tile_parts, 0, 0);
+    if (by_rows) {
+        if (!a.joined) return;                             // not split: written by its kernel
+        u = a.wanted ? a.units[s] : make_int4(s * a.per, 1, 0, 0);
     }
-    const Parts pre{a.po, a.pml, ((size_t)row * a.p.n_heads + head) * a.parts + tile_parts, 1, prefix_parts};
-    const int parts = own.n + pre.n;
-    const auto index = [&](int i) { return i < own.n ? own.first + (size_t)i * own.step : pre.first + (size_t)(i - own.n); };
-    const auto ml = [&](int i) { return (i < own.n ? own.pml : pre.pml)[index(i)]; };
-    float M = -INFINITY;
-    for (int i = tid; i < parts; i += 256) M = fmaxf(M, ml(i).x);
-    M = wave_max(M);
-    if (lane == 0) sm[wave] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    // 64 parts' weights at a time, one per lane; eight parts' values in flight
-    // (a part that is not there has weight 0, its values are not looked at)
-    float L = 0.0f, o[E] = {};
-    const int per = (parts + 3) / 4, i0 = wave * per, i1 = min(parts, i0 + per);
-    for (int b = i0; b < i1; b += 64) {
-        const float2 v = b + lane < i1 ? ml(b + lane) : make_float2(-INFINITY, 0.0f);
-        const float w = v.x == -INFINITY ? 0.0f : v.x == M ? 1.0f : __builtin_amdgcn_exp2f(v.x - M);
-        L += w == 0.0f ? 0.0f : w * v.y;
-        const int n = min(64, i1 - b);
-        for (int j = 0; j < n; j += 8) {
-            float x[8][E];
+    if (prefix_parts == 0 && (by_rows ? u.y == 1 : u.y == 0)) return;
+    for (int head = head0; head < min(head0 + heads, a.p.n_heads); head++) {
+        Parts own{a.po, a.pml, ((size_t)row * a.p.n_heads + head) * a.parts, 1, tile_parts};
+        if (by_rows) {
+            const int k = (row - first) * a.group + head % a.group, tile = k / kRowTile;
+            const int64_t unit = (int64_t)u.x + (int64_t)tile * u.y;
+            if (u.x < 0 || u.y < 1 || unit + u.y > a.max_units) return;    // (starts that do not ascend)
+            own = Parts{rows_po, rows_pml, ((size_t)unit * a.p.n_kv + head / a.group) * kRowTile + k % kRowTile, a.p.n_kv * kRowTile, u.y};
+        }
+        const Parts pre{a.po, a.pml, ((size_t)row * a.p.n_heads + head) * a.parts + tile_parts, 1, prefix_parts};
+        const int parts = own.n + pre.n;
+        const auto index = [&](int i) { return i < own.n ? own.first + (size_t)i * own.step : pre.first + (size_t)(i - own.n); };
+        const auto ml = [&](int i) { return (i < own.n ? own.pml : pre.pml)[index(i)]; };
+        float M = -INFINITY;
+        for (int i = tid; i < parts; i += 256) M = fmaxf(M, ml(i).x);
+        M = wave_max(M);
+        if (lane == 0) sm[wave] = M;
+        __syncthreads();
+        M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+        // 64 parts' weights at a time, one per lane; eight parts' values in flight
+        // (a part that is not there has weight 0, its values are not looked at)
+        float L = 0.0f, o[E] = {};
+        const int per = (parts + 3) / 4, i0 = wave * per, i1 = min(parts, i0 + per);
+        for (int b = i0; b < i1; b += 64) {
+            const float2 v = b + lane < i1 ? ml(b + lane) : make_float2(-INFINITY, 0.0f);
+            const float w = v.x == -INFINITY ? 0.0f : v.x == M ? 1.0f : __builtin_amdgcn_exp2f(v.x - M);
+            L += w == 0.0f ? 0.0f : w * v.y;
+            const int n = min(64, i1 - b);
+            for (int j = 0; j < n; j += 8) {
+                float x[8][E];
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const int i = b + min(j + k, n - 1);
-                const float* po = (i < own.n ? own.po : pre.po) + index(i) * HD;
+                for (int k = 0; k < 8; k++) {
+                    const int i = b + min(j + k, n - 1);
+                    const float* po = (i < own.n ? own.po : pre.po) + index(i) * HD;
 #pragma unroll
-                for (int e = 0; e < E; e++) x[k][e] = po[E * min(lane, HD / E - 1) + e];
-            }
+                    for (int e = 0; e < E; e++) x[k][e] = po[E * min(lane, HD / E - 1) + e];
+                }
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const float f = j + k < n ? lane_value(w, j + k) : 0.0f;
+                for (int k = 0; k < 8; k++) {
+                    const float f = j + k < n ? lane_value(w, j + k) : 0.0f;
 #pragma unroll
-                for (int e = 0; e < E; e++)
-                    if (f != 0.0f) o[e] = fmaf(x[k][e], f, o[e]);
+                    for (int e = 0; e < E; e++)
+                        if (f != 0.0f) o[e] = fmaf(x[k][e], f, o[e]);
+                }
             }
         }
-    }
-    for (int off = 32; off > 0; off >>= 1) L += __shfl_xor(L, off, 64);
-    if (lane == 0) sl[wave] = L;
+        L = wave_sum(L);
+        if (lane == 0) sl[wave] = L;
 #pragma unroll
-    for (int e = 0; e < E; e++)
-        if (HD >= 64 || lane < HD) so[wave][E * lane + e] = o[e];
-    __syncthreads();
-    if (tid < HD) {
-        L = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-        const float v = (so[0][tid] + so[1][tid]) + (so[2][tid] + so[3][tid]);
-        a.out[(size_t)row * a.out_ld + (size_t)head * HD + tid] = L != 0.0f ? v / L : 0.0f;
+        for (int e = 0; e < E; e++)
+            if (HD >= 64 || lane < HD) so[wave][E * lane + e] = o[e];
+        __syncthreads();
+        if (tid < HD) {
+            L = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+            const float v = (so[0][tid] + so[1][tid]) + (so[2][tid] + so[3][tid]);
+            a.out[(size_t)row * a.out_ld + (size_t)head * HD + tid] = L != 0.0f ? v / L : 0.0f;
+        }
+        __syncthreads();
     }
 }
 
@@ -1078,7 +1031,8 @@ struct Launch {
 };
 struct AttnPlan {
     int per = 1, wanted = 0, max_units = 0;          // row kernel, own pages (PagedAttn)
-    bool join_rows = false, both = false;
+    float finer = 0.0f;
+    bool split = false, join_rows = false, both = false;
     int per_seq = 0;                                 // joining only what the row kernel took: rows of a sequence
     Launch tile, prefix;                             // tile kernel, own pages; the prefix
     bool prefix_by_tile = false;
@@ -1086,59 +1040,83 @@ struct AttnPlan {
     size_t row_units = 0, all_units = 0, bytes = 0;
 };
 
-// Row tiles of 16 per wavefront in the tile kernel: as the registers allow.
-template <typename C> constexpr int tile_mt(int hd) { return 1; }
-int tile_rows(int dtype, int hd) { return 16 * kTileWaves * (dtype == YL_T_F32 ? tile_mt<float>(hd) : dtype == YL_T_F16 ? tile_mt<_Float16>(hd) : tile_mt<__bf16>(hd)); }
-
-constexpr int kUnsplit = 640;        // own positions up to which a tile's are not split
+// Own positions up to which a tile's are not split (one kernel less): of few
+// tiles, of many.  One decoded row, 32 heads on 8, f16, hd 64, unsplit | split, in
+// us: 300 positions 7.0 | 8.9, 600 8.3 | 8.9, 1000 10.3 | 9.2, 2000 15.5 | 9.0.
+constexpr int kUnsplit = 640, kUnsplitMany = 2048;
 constexpr int kLeastChunk = 128;
+// The tile kernel from as many workgroups of rows on (f16 and bf16 caches; f32's
+// matrix instructions take so long that K and V need not be shared).  One prompt
+// over itself, 32 heads on 8, in us, row kernel | tile kernel:
+//   tokens            400            500            640            800           1280
+//   workgroups        104            128            160            200            320
+//   f16 hd 64   13.1 | 19.4    15.3 | 20.9    28.1 | 26.9    35.2 | 30.0    63.3 | 44.6
+//   bf16 hd 128 26.0 | 32.5    27.5 | 35.7    46.7 | 47.3    58.7 | 54.1     104 | 79.0
+// f32, 1280 tokens: 9 heads on 3, hd 64, 42.8 | 110; 32 on 8, hd 128, 187 | 214.
+constexpr int kTileKernelGroups = 160;
+// The tile kernel for a prefix from as many stacked rows of all kv heads times
+// prefix positions on.  Decoded rows, 32 heads on 8, whole call in us, row
+// kernel | tile kernel:
+//   sequences x prefix    32 x 2000      32 x 6000      96 x 2000      96 x 6000
+//   product (2^20)              2.0            5.9            5.9           17.6
+//   f16 hd 64           19.9 | 22.5    26.8 | 31.5    34.4 | 37.1    56.6 | 41.4
+//   bf16 hd 128         27.7 | 33.4    36.5 | 35.2    52.0 | 48.9    88.7 | 66.6
+constexpr int64_t kPrefixByTile = 8 << 20;
 
 AttnPlan plan_attention(const PagedArgs& p, int dtype, uint32_t max_len) {
     AttnPlan r;
-    const int group = p.n_heads / p.n_kv, R = tile_rows(dtype, p.hd);
+    const int group = p.n_heads / p.n_kv, R = kTileRows;
     const int64_t cap = paged_capacity(p), stacked = (int64_t)p.n_rows * group;
     const int64_t longest = max_len && max_len < cap ? max_len : cap;
     const int own = (int)std::max<int64_t>(longest - p.prefix_len, 0);
     // splits the positions of `tiles` tiles so that `wanted` workgroups have work
-    const auto split = [&](Launch* l, int64_t tiles, int positions, int wanted) {
+    const auto split = [&](Launch* l, int64_t tiles, int positions, int wanted, int least) {
         const int64_t want = std::max<int64_t>(wanted / std::max<int64_t>(tiles * p.n_kv, 1), 1);
-        l->splits = (int)std::clamp<int64_t>(want, 1, std::max(1, (positions + kLeastChunk - 1) / kLeastChunk));
+        l->splits = (int)std::clamp<int64_t>(want, 1, std::max(1, (positions + least - 1) / least));
         l->chunk = ((positions + l->splits - 1) / l->splits + 63) & ~63;
         l->splits = std::max(1, (positions + l->chunk - 1) / std::max(l->chunk, 1));
     };
     const int resident = p.hd == 128 ? 256 : 512;    // workgroups of the tile kernel that run at once
-    r.both = p.row_start && stacked > kRowKernelRows;
-    r.per = p.row_start ? kRowKernelRows / kRowTile : (group + kRowTile - 1) / kRowTile;
-    r.wanted = own > kUnsplit ? std::max(std::max(1, 512 / p.n_kv), 2 * p.n_seqs * r.per) : 0;
-    r.max_units = p.n_seqs * r.per + r.wanted;
-    r.join_rows = r.wanted || p.prefix_len;
-    if (r.both) {
-        r.tile.tiles = (int)(stacked / R) + p.n_seqs;
-        split(&r.tile, (stacked + R - 1) / R, own, resident);
-    }
+    r.both = p.row_start && dtype != YL_T_F32 && (stacked + R - 1) / R * p.n_kv >= kTileKernelGroups;
+    r.per = (group + kRowTile - 1) / kRowTile;
+    // tiles of the row kernel at most
+    const int64_t tiles = !p.row_start ? (int64_t)p.n_seqs * r.per
+                          : r.both     ? std::min<int64_t>((int64_t)p.n_seqs * (kRowKernelRows / kRowTile), stacked / kRowTile + p.n_seqs)
+                                       : stacked / kRowTile + p.n_seqs;
+    r.split = own > (p.row_start && !r.both && tiles * p.n_kv >= 512 ? kUnsplitMany : kUnsplit);
+    r.wanted = r.split ? std::max(1, 512 / p.n_kv) : p.row_start ? 1 : 0;
+    r.finer = p.row_start ? 0.95f : 2.0f;
+    r.max_units = (int)(tiles + std::max<int64_t>(r.wanted, r.split ? 2 * tiles : 0));
+    r.join_rows = r.split || p.prefix_len;
+    if (r.both) r.tile.tiles = (int)(stacked / R) + p.n_seqs;
     if (p.prefix_len) {
-        r.prefix_by_tile = stacked > kRowKernelRows;
+        r.prefix_by_tile = dtype != YL_T_F32 && stacked * p.n_kv * p.prefix_len >= kPrefixByTile;
         r.prefix.tiles = (int)((stacked + (r.prefix_by_tile ? R : kRowTile) - 1) / (r.prefix_by_tile ? R : kRowTile));
-        split(&r.prefix, r.prefix.tiles, p.prefix_len, r.prefix_by_tile ? resident : 512);
+        split(&r.prefix, r.prefix.tiles, p.prefix_len, r.prefix_by_tile ? resident : 512, kLeastChunk);
     } else {
         r.prefix.splits = 0;
     }
     // partial results: of the row kernel, 16 rows for every unit and kv head;
     // of the others, for every row
-    r.tile_parts = r.tile.splits > 1 || p.prefix_len ? r.tile.splits : 0;
+    r.tile_parts = r.both && p.prefix_len ? 1 : 0;
     if (r.join_rows) r.row_units = (size_t)r.max_units * p.n_kv * kRowTile;
     r.all_units = (size_t)p.n_rows * p.n_heads * (r.tile_parts + r.prefix.splits);
-    r.per_seq = std::max(1, kRowKernelRows / group);
+    r.per_seq = r.both ? std::max(1, kRowKernelRows / group) : 0;
     if (r.all_units || (int64_t)p.n_seqs * r.per_seq >= p.n_rows) r.per_seq = 0;
     r.bytes = (r.row_units + r.all_units) * (p.hd + 2) * sizeof(float);
-    if (r.wanted) r.bytes = ((r.bytes + 15) & ~(size_t)15) + (size_t)p.n_seqs * sizeof(int4);
+    if (r.wanted && r.join_rows) r.bytes = ((r.bytes + 15) & ~(size_t)15) + (size_t)p.n_seqs * sizeof(int4);
     return r;
 }
 
 template <typename C, int HD>
 hipError_t launch_attn_hd(const PagedAttn& a, const dim3& grid, bool by_tile, bool prefix, hipStream_t s) {
-    if (by_tile) hipLaunchKernelGGL((k_paged_attn_tile<C, HD, tile_mt<C>(HD)>), grid, dim3(64 * kTileWaves), 0, s, a, prefix);
-    else hipLaunchKernelGGL((k_paged_attn_rows<C, HD>), grid, dim3(256), 0, s, a, prefix);
+    if constexpr (sizeof(C) == 2) {
+        if (by_tile) {
+            hipLaunchKernelGGL((k_paged_attn_tile<C, HD>), grid, dim3(64 * kTileWaves), 0, s, a, prefix);
+            return hipGetLastError();
+        }
+    }
+    hipLaunchKernelGGL((k_paged_attn_rows<C, HD>), grid, dim3(256), 0, s, a, prefix);
     return hipGetLastError();
 }
 
@@ -1155,11 +1133,12 @@ hipError_t launch_all(PagedAttn a, const AttnPlan& plan, float* space, hipStream
     float2* const ml = reinterpret_cast<float2*>(space + units * a.p.hd);
     float2* const all_ml = ml + plan.row_units;
     a.both = plan.both;
-    a.per = plan.per; a.wanted = plan.wanted; a.max_units = plan.max_units;
+    a.per = plan.per; a.wanted = plan.wanted; a.finer = plan.finer; a.max_units = plan.max_units;
     a.units = reinterpret_cast<int4*>(reinterpret_cast<char*>(space) + (plan.bytes - (size_t)a.p.n_seqs * sizeof(int4)));
     a.po = space; a.pml = ml;
     a.direct = !a.p.prefix_len;
-    a.chunk = kLeastChunk;
+    a.joined = plan.join_rows;
+    a.chunk = plan.split ? kLeastChunk : 1 << 30;
     hipError_t e = launch_attn<C>(a, dim3((unsigned)plan.max_units * a.p.n_kv), false, false, s);
     a.po = all_po; a.pml = all_ml;
     a.parts = plan.tile_parts + plan.prefix.splits;
@@ -1174,10 +1153,12 @@ hipError_t launch_all(PagedAttn a, const AttnPlan& plan, float* space, hipStream
         a.splits = plan.prefix.splits; a.chunk = plan.prefix.chunk;
         e = launch_attn<C>(a, dim3((unsigned)plan.prefix.tiles * a.p.n_kv, plan.prefix.splits), plan.prefix_by_tile, true, s);
     }
-    if (e != hipSuccess || !units) return e;
-    const dim3 grid((unsigned)(plan.per_seq ? a.p.n_seqs * plan.per_seq : a.p.n_rows) * a.p.n_heads);
+    if (e != hipSuccess || !units) return e;    // (nothing was split)
+    const int rows = plan.per_seq ? a.p.n_seqs * plan.per_seq : a.p.n_rows;
+    const int heads = (int)std::clamp<int64_t>((int64_t)rows * a.p.n_heads / 4096, 1, a.p.n_heads);
+    const dim3 grid((unsigned)rows * ((a.p.n_heads + heads - 1) / heads));
     auto join = a.p.hd == 32 ? k_paged_attn_join<32> : a.p.hd == 64 ? k_paged_attn_join<64> : k_paged_attn_join<128>;
-    hipLaunchKernelGGL(join, grid, dim3(256), 0, s, a, plan.per_seq, (const float*)space, (const float2*)ml, plan.tile_parts, plan.prefix.splits);
+    hipLaunchKernelGGL(join, grid, dim3(256), 0, s, a, heads, plan.per_seq, (const float*)space, (const float2*)ml, plan.tile_parts, plan.prefix.splits);
     return hipGetLastError();
 }
 
