@@ -23,46 +23,105 @@ struct AppendArgs {
     int64_t rope_rows;
 };
 
-// One workgroup per row; a thread per pair of a query or key head, then one
-// per pair of value elements.
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // activations: any float address
+typedef float f2u __attribute__((ext_vector_type(2), aligned(4)));
+
+// Four neighbouring elements rounded to the cache's type, once, to nearest.
 template <typename C>
+__device__ __forceinline__ void store4(C* o, const f4u& x) {
+    typedef C c4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<c4*>(o) = __builtin_convertvector((vf4{x[0], x[1], x[2], x[3]}), c4);
+}
+
+// The sequence of a row by a whole wavefront, 64 starts per step (as paged_seq_of_row).
+__device__ __forceinline__ int seq_of_row(const PagedArgs& a, int row) {
+    if (!a.row_start) return row < a.n_seqs ? row : -1;
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = a.n_seqs;                 // the last start not above the row is one of lo .. lo + n - 1
+    while (n > 1) {
+        const int step = (n + 63) >> 6;
+        const bool ok = lane * step < n && a.row_start[lo + lane * step] <= (uint32_t)row;
+        const int c = max(1, (int)__builtin_popcountll(__ballot(ok))) - 1;
+        lo += c * step;
+        n = min(step, n - c * step);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    return a.row_start[lo] <= (uint32_t)row && (uint32_t)row < a.row_start[lo + 1] ? lo : -1;
+}
+
+// One workgroup per row; a thread takes 4 neighbouring elements (of a half
+// rotation, 4 pairs) at a time.  Bound by memory: 16-byte loads, several in
+// flight per thread; the keys and values of one head are neighbours in a page.
+template <typename C, int PAIRS>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
     const int row = blockIdx.x, hd = a.p.hd, half = hd / 2, tid = threadIdx.x;
-    const int s = paged_seq_of_row(a.p, row);
+    const int s = seq_of_row(a.p, row);
     if (s < 0) return;
     int first, end;
     paged_rows(a.p, s, &first, &end);
     if (row < first || row >= end) return;
     const int64_t pos = paged_row_pos(a.p.kv_len[s], end, row);
-    if (pos < 0 || (a.pairs != YL_ROPE_NONE && pos >= a.rope_rows)) return;
+    if (pos < 0 || (PAIRS != YL_ROPE_NONE && pos >= a.rope_rows)) return;
     int page = -1, slot = 0;
     const bool keep = pos >= a.p.prefix_len && paged_place(a.p, s, pos, &page, &slot);
-    const int nq = a.q ? a.p.n_heads * half : 0, nk = a.p.n_kv * half;
-    for (int i = tid; i < nq + nk; i += 256) {
-        const bool is_q = i < nq;
-        const int j = is_q ? i : i - nq, head = j / half, e = j % half;
-        const int lo = a.pairs == YL_ROPE_HALF ? e : 2 * e, hi = a.pairs == YL_ROPE_HALF ? e + half : 2 * e + 1;
-        const float* x = (is_q ? a.q + (size_t)row * a.q_ld : a.k + (size_t)row * a.k_ld) + (size_t)head * hd;
-        float x0 = x[lo], x1 = x[hi];
-        if (a.pairs != YL_ROPE_NONE) {
-            const float c = a.cos_t[(size_t)pos * half + e], sn = a.sin_t[(size_t)pos * half + e];
-            const float r0 = fmul(x0, c) - fmul(x1, sn), r1 = fadd(fmul(x0, sn), fmul(x1, c));
-            x0 = r0;
-            x1 = r1;
+    const float* ct = a.cos_t + (size_t)pos * half;
+    const float* st = a.sin_t + (size_t)pos * half;
+    // element offset of (head, element) in a page
+    const auto at = [&](int head, int e) { return paged_offset(a.p, page, head, slot) + e; };
+    const int shift = 31 - __builtin_clz(hd);             // (hd is a power of two)
+    const float* qr = a.q + (size_t)row * a.q_ld;
+    const float* kr = a.k + (size_t)row * a.k_ld;
+    const float* vr = a.v + (size_t)row * a.v_ld;
+    float* qo = a.q_out + (size_t)row * a.q_out_ld;
+    const int nq = a.q ? a.p.n_heads * hd : 0, nk = keep ? a.p.n_kv * hd : 0;
+    if constexpr (PAIRS == YL_ROPE_HALF) {
+        const int uq = nq / 8, uk = nk / 8;               // units of 4 pairs
+#pragma unroll 2
+        for (int i = tid; i < uq + uk; i += 256) {
+            const bool is_q = i < uq;
+            const int j = is_q ? i : i - uq, head = j >> (shift - 3), e = 4 * (j & (hd / 8 - 1));
+            const float* x = (is_q ? qr : kr) + (size_t)head * hd + e;
+            const f4u x0 = *reinterpret_cast<const f4u*>(x), x1 = *reinterpret_cast<const f4u*>(x + half);
+            const f4u c = *reinterpret_cast<const f4u*>(ct + e), sn = *reinterpret_cast<const f4u*>(st + e);
+            f4u r0, r1;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                r0[k] = fmul(x0[k], c[k]) - fmul(x1[k], sn[k]);
+                r1[k] = fadd(fmul(x0[k], sn[k]), fmul(x1[k], c[k]));
+            }
+            if (is_q) {
+                *reinterpret_cast<f4u*>(qo + (size_t)head * hd + e) = r0;
+                *reinterpret_cast<f4u*>(qo + (size_t)head * hd + e + half) = r1;
+            } else {
+                C* o = static_cast<C*>(a.p.keys) + at(head, e);
+                store4(o, r0);
+                store4(o + half, r1);
+            }
         }
-        if (is_q) {
-            float* o = a.q_out + (size_t)row * a.q_out_ld + (size_t)head * hd;
-            o[lo] = x0;
-            o[hi] = x1;
-        } else if (keep) {
-            C* o = static_cast<C*>(a.p.keys) + paged_offset(a.p, page, head, slot);
-            o[lo] = (C)x0;
-            o[hi] = (C)x1;
+    } else {
+        const int uq = nq / 4, uk = nk / 4;
+#pragma unroll 4
+        for (int i = tid; i < uq + uk; i += 256) {
+            const bool is_q = i < uq;
+            const int j = is_q ? i : i - uq, head = j >> (shift - 2), e = 4 * (j & (hd / 4 - 1));
+            f4u x = *reinterpret_cast<const f4u*>((is_q ? qr : kr) + 4 * (size_t)j);
+            if constexpr (PAIRS == YL_ROPE_ADJACENT) {
+                const f2u c = *reinterpret_cast<const f2u*>(ct + e / 2), sn = *reinterpret_cast<const f2u*>(st + e / 2);
+                f4u r;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    r[2 * k] = fmul(x[2 * k], c[k]) - fmul(x[2 * k + 1], sn[k]);
+                    r[2 * k + 1] = fadd(fmul(x[2 * k], sn[k]), fmul(x[2 * k + 1], c[k]));
+                }
+                x = r;
+            }
+            if (is_q) *reinterpret_cast<f4u*>(qo + 4 * (size_t)j) = x;
+            else store4(static_cast<C*>(a.p.keys) + at(head, e), x);
         }
     }
-    if (keep)
-        for (int i = tid; i < a.p.n_kv * hd; i += 256)
-            static_cast<C*>(a.p.values)[paged_offset(a.p, page, i / hd, slot) + i % hd] = (C)a.v[(size_t)row * a.v_ld + i];
+#pragma unroll 2
+    for (int j = tid; j < nk / 4; j += 256)
+        store4(static_cast<C*>(a.p.values) + at(j >> (shift - 2), 4 * (j & (hd / 4 - 1))), *reinterpret_cast<const f4u*>(vr + 4 * (size_t)j));
 }
 
 // ------------------------------------------------------------- host entries
@@ -103,6 +162,13 @@ yl_status paged_args(const yl_paged_cache* c, const yl_paged_batch* b, uint32_t 
 
 namespace {
 
+template <typename C>
+void launch_append(const AppendArgs& a, hipStream_t s) {
+    auto k = a.pairs == YL_ROPE_HALF ? k_paged_append<C, YL_ROPE_HALF> : a.pairs == YL_ROPE_ADJACENT ? k_paged_append<C, YL_ROPE_ADJACENT>
+                                                                                                  : k_paged_append<C, YL_ROPE_NONE>;
+    hipLaunchKernelGGL(k, dim3(a.p.n_rows), dim3(256), 0, s, a);
+}
+
 yl_status launched(const char* what) {
     const hipError_t e = hipGetLastError();
     if (e == hipSuccess) return YL_OK;
@@ -135,8 +201,10 @@ yl_status yl_paged_append(const yl_paged_cache* cache, const yl_paged_batch* bat
     a.q_out = q_out; a.q = q; a.k = k; a.v = v;
     a.q_out_ld = q_out_ld; a.q_ld = q_ld; a.k_ld = k_ld; a.v_ld = v_ld;
     a.pairs = pairs; a.cos_t = cos_t; a.sin_t = sin_t; a.rope_rows = rope_rows;
-    auto kern = cache->dtype == YL_T_F32 ? k_paged_append<float> : cache->dtype == YL_T_F16 ? k_paged_append<_Float16> : k_paged_append<__bf16>;
-    hipLaunchKernelGGL(kern, dim3(batch->n_rows), dim3(256), 0, (hipStream_t)stream, a);
+    const hipStream_t strm = (hipStream_t)stream;
+    if (cache->dtype == YL_T_F32) launch_append<float>(a, strm);
+    else if (cache->dtype == YL_T_F16) launch_append<_Float16>(a, strm);
+    else launch_append<__bf16>(a, strm);
     return launched("paged_append launch");
 }
 
