@@ -679,7 +679,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
     };
     int page[NT], next_page[NT] = {};
     const auto step_on = [&](int step, u4 (&kc)[NT][NK], u4 (&kn)[NT][NK]) {
-        // values of this step, keys of the next
+        // values of this step, keys of the next (the next step's values too
+        // measured the same or, with a wavefront per SIMD fewer, slower)
         typename R::Value vr[NT][4];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
@@ -934,9 +935,8 @@ struct Parts {
     size_t first; int step, n;
 };
 
-// Joins the partial results of `heads` heads of a row, one after the other:
-// weights 2^(m - max), a quarter of the parts per wavefront, HD / 64 (or one)
-// dimensions per lane.
+// Joins the partial results of a row, a wavefront per head (every fourth of
+// `heads` heads): weights 2^(m - max), HD / 64 (or one) dimensions per lane.
 // `per_seq`: rows of every sequence that the row kernel took (that many of
 // each are looked at); 0: all rows.  Their own parts stand at `rows`, those
 // of the tile kernel (tile_parts, 0: it wrote `out`) and over the prefix at a.po.
@@ -944,10 +944,9 @@ template <int HD>
 __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttn a, int heads, int per_seq, const float* rows_po, const float2* rows_pml,
                                                          int tile_parts, int prefix_parts) {
     constexpr int E = HD < 64 ? 1 : HD / 64;
-    __shared__ float so[4][HD], sl[4], sm[4];
     const int groups = (a.p.n_heads + heads - 1) / heads;
     const int at = blockIdx.x / groups, head0 = (blockIdx.x % groups) * heads;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int s = per_seq ? at / per_seq : paged_seq_of_row(a.p, at);
     if (s < 0) return;
     int first, end;
@@ -961,7 +960,7 @@ __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttn a, int heads,
         u = a.wanted ? a.units[s] : make_int4(s * a.per, 1, 0, 0);
     }
     if (prefix_parts == 0 && (by_rows ? u.y == 1 : u.y == 0)) return;
-    for (int head = head0; head < min(head0 + heads, a.p.n_heads); head++) {
+    for (int head = head0 + wave; head < min(head0 + heads, a.p.n_heads); head += 4) {
         Parts own{a.po, a.pml, ((size_t)row * a.p.n_heads + head) * a.parts, 1, tile_parts};
         if (by_rows) {
             const int k = (row - first) * a.group + head % a.group, tile = k / kRowTile;
@@ -972,33 +971,30 @@ __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttn a, int heads,
         const Parts pre{a.po, a.pml, ((size_t)row * a.p.n_heads + head) * a.parts + tile_parts, 1, prefix_parts};
         const int parts = own.n + pre.n;
         const auto index = [&](int i) { return i < own.n ? own.first + (size_t)i * own.step : pre.first + (size_t)(i - own.n); };
-        const auto ml = [&](int i) { return (i < own.n ? own.pml : pre.pml)[index(i)]; };
-        float M = -INFINITY;
-        for (int i = tid; i < parts; i += 256) M = fmaxf(M, ml(i).x);
+        const auto ml = [&](int i) { return i < parts ? (i < own.n ? own.pml : pre.pml)[index(i)] : make_float2(-INFINITY, 0.0f); };
+        float2 v = ml(lane);
+        float M = v.x;
+        for (int i = 64 + lane; i < parts; i += 64) M = fmaxf(M, ml(i).x);
         M = wave_max(M);
-        if (lane == 0) sm[wave] = M;
-        __syncthreads();
-        M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-        // 64 parts' weights at a time, one per lane; eight parts' values in flight
+        // 64 parts' weights at a time, one per lane; 16 parts' values in flight
         // (a part that is not there has weight 0, its values are not looked at)
         float L = 0.0f, o[E] = {};
-        const int per = (parts + 3) / 4, i0 = wave * per, i1 = min(parts, i0 + per);
-        for (int b = i0; b < i1; b += 64) {
-            const float2 v = b + lane < i1 ? ml(b + lane) : make_float2(-INFINITY, 0.0f);
+        for (int b = 0; b < parts; b += 64) {
+            if (b) v = ml(b + lane);
             const float w = v.x == -INFINITY ? 0.0f : v.x == M ? 1.0f : __builtin_amdgcn_exp2f(v.x - M);
             L += w == 0.0f ? 0.0f : w * v.y;
-            const int n = min(64, i1 - b);
-            for (int j = 0; j < n; j += 8) {
-                float x[8][E];
+            const int n = min(64, parts - b);
+            for (int j = 0; j < n; j += 16) {
+                float x[16][E];
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
+                for (int k = 0; k < 16; k++) {
                     const int i = b + min(j + k, n - 1);
                     const float* po = (i < own.n ? own.po : pre.po) + index(i) * HD;
 #pragma unroll
                     for (int e = 0; e < E; e++) x[k][e] = po[E * min(lane, HD / E - 1) + e];
                 }
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
+                for (int k = 0; k < 16; k++) {
                     const float f = j + k < n ? lane_value(w, j + k) : 0.0f;
 #pragma unroll
                     for (int e = 0; e < E; e++)
@@ -1007,17 +1003,10 @@ __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttn a, int heads,
             }
         }
         L = wave_sum(L);
-        if (lane == 0) sl[wave] = L;
+        float* dst = a.out + (size_t)row * a.out_ld + (size_t)head * HD;
 #pragma unroll
         for (int e = 0; e < E; e++)
-            if (HD >= 64 || lane < HD) so[wave][E * lane + e] = o[e];
-        __syncthreads();
-        if (tid < HD) {
-            L = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-            const float v = (so[0][tid] + so[1][tid]) + (so[2][tid] + so[3][tid]);
-            a.out[(size_t)row * a.out_ld + (size_t)head * HD + tid] = L != 0.0f ? v / L : 0.0f;
-        }
-        __syncthreads();
+            if (HD >= 64 || lane < HD) dst[E * lane + e] = L != 0.0f ? o[e] / L : 0.0f;
     }
 }
 
@@ -1155,7 +1144,7 @@ hipError_t launch_all(PagedAttn a, const AttnPlan& plan, float* space, hipStream
     }
     if (e != hipSuccess || !units) return e;    // (nothing was split)
     const int rows = plan.per_seq ? a.p.n_seqs * plan.per_seq : a.p.n_rows;
-    const int heads = (int)std::clamp<int64_t>((int64_t)rows * a.p.n_heads / 4096, 1, a.p.n_heads);
+    const int heads = (int)std::clamp<int64_t>((int64_t)rows * a.p.n_heads / 4096, 4, std::max(4, a.p.n_heads));
     const dim3 grid((unsigned)rows * ((a.p.n_heads + heads - 1) / heads));
     auto join = a.p.hd == 32 ? k_paged_attn_join<32> : a.p.hd == 64 ? k_paged_attn_join<64> : k_paged_attn_join<128>;
     hipLaunchKernelGGL(join, grid, dim3(256), 0, s, a, heads, plan.per_seq, (const float*)space, (const float2*)ml, plan.tile_parts, plan.prefix.splits);
