@@ -104,7 +104,7 @@ class Scene:
                     e = np.exp(sc - sc.max())
                     out[r, h] = e @ vv / e.sum()
                     ds = ((self.hd + 4) * U * (np.abs(kk) @ np.abs(qq)).max()
-                          + 8 * U * self.hd * np.abs(qq).max() * np.abs(kk).max()) * self.scale
+                          + 8 * U * self.hd * np.abs(qq).max() * np.abs(kk).max()) * abs(self.scale)
                     bound[r, h] = 2 * (ds + 12 * U + len(at) * U) * np.abs(vv).max()
         return out.reshape(self.total, -1), bound.reshape(self.total, -1)
 

@@ -64,6 +64,15 @@ def test_many_rows(gpu, rows):
     _check(x, rng.integers(0, 700, rows), 7, "f32")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab,top", [(100, 50000, 9), (300, 17000, 3), (300, 10000, 32), (2, 300000, 32), (2, 300000, 5)])
+def test_stretches_and_their_joining(gpu, dtype, rows, vocab, top):
+    """Both stretch lengths, rows of one stretch and of several, and lists too many for one selection."""
+    rng = np.random.default_rng(rows + vocab)
+    x = (rng.standard_normal((rows, vocab)) * 3).astype(np.float32)
+    _check(x, rng.integers(0, vocab, rows), top, dtype)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("vocab", [50, 40000])
 def test_equal_values_by_rising_id(gpu, dtype, vocab):

@@ -199,6 +199,27 @@ def test_small_and_large_scores(gpu, dtype, size):
     _check(sc, _attend(sc))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 3.0])
+def test_scales(gpu, dtype, scale):
+    """A negative scale turns the order of the scores around, 0 makes all weights equal."""
+    sc = Scene([1, 20, 60], [500, 90, 60], 4, 2, 64, 16, dtype, seed=15)
+    sc.scale = scale
+    _check(sc, _attend(sc))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("kvh,rows", [(2, 20), (160, 40)])
+def test_subnormal_keys_and_values(gpu, dtype, kvh, rows):
+    """f16 keys and values below its least normal number (and bf16 ones as small) count in full, in both kernels."""
+    sc = Scene([1, rows], [200, 70], kvh, kvh, 32, 16, dtype, seed=16)
+    sc.k32 *= np.float32(1e-5)
+    sc.v32 *= np.float32(1e-6)
+    sc.q *= np.float32(3e5)
+    ref = _check(sc, _attend(sc))
+    assert 0 < np.abs(ref).max() < 1e-5
+
+
 class Call:
     """A call on device arrays, as a program that keeps its own memory makes it."""
 

@@ -110,7 +110,8 @@ __device__ __forceinline__ void rank_keys(const u64* key, int n, int top, int ti
 // group maximum has `top` values at or above it and so bounds the stretch's top
 // values from below; the few values at or above the bound (some 25 of 4096 random
 // ones at top 20) are ranked by counting.  Where equal values make them more
-// than kCands, the entries are found one by one.
+// than kCands, the entries are found one by one.  Values of -inf and NaN are
+// looked for by id, where the others do not fill the list.
 template <typename T, int V>
 __global__ __launch_bounds__(kScoreThreads, 6) void k_score(const T* __restrict__ x, size_t vocab, size_t ld, const uint32_t* tokens,
                                                             float* logprob, float* entropy, int top, uint32_t* top_ids,
@@ -159,7 +160,7 @@ __global__ __launch_bounds__(kScoreThreads, 6) void k_score(const T* __restrict_
             if (__builtin_popcountll(__ballot(mine >= c)) >= top) b = c;
         }
         if (lane == 0) {
-            least_sh = key_value((u64)b << 32);
+            least_sh = b <= order_key(-INFINITY) ? -INFINITY : key_value((u64)b << 32);
             count = 0;
         }
     }
@@ -212,11 +213,11 @@ __global__ __launch_bounds__(kScoreThreads, 6) void k_score(const T* __restrict_
     }
     if (!top) return;
     const float least = least_sh;
-    if (mx >= least) {
+    if (mx >= least && mx > -INFINITY) {
 #pragma unroll
         for (int k = 0; k < N; k++) {
             const int i = W * (tid + (k / W) * kScoreThreads) + k % W;
-            if (v[k] >= least && i < n) {
+            if (v[k] >= least && v[k] > -INFINITY) {         // (what is past n is -inf)
                 const int c = atomicAdd(&count, 1);
                 if (c < kCands) key[c] = id_key(v[k], (uint32_t)(base + i));
             }
@@ -232,13 +233,27 @@ __global__ __launch_bounds__(kScoreThreads, 6) void k_score(const T* __restrict_
         }
     };
     const int found = count;
-    // (fewer than asked for: NaN, which the bound passes over, belongs to the list)
-    if (found <= kCands && found >= min(top, n)) {
+    if (found <= kCands) {
         if (tid < 8) key[found + tid] = 0;
         __syncthreads();
         rank_keys(key, found, top, tid, kScoreThreads, put);
+        // Fewer than asked for (a choice of few tokens): then the ids of -inf
+        // from the lowest on, then those of NaN, 64 values at a time.
+        int filled = found;
+        const int wanted = min(top, n);
+        if (wave == 0) {
+            for (int pass = 0; pass < 2 && filled < wanted; pass++)
+                for (int i0 = 0; i0 < n && filled < wanted; i0 += 64) {
+                    const float x0 = i0 + lane < n ? (float)xr[base + i0 + lane] : 0.0f;
+                    const bool take = pass ? x0 != x0 : x0 == -INFINITY;
+                    const u64 all = __ballot(take);
+                    const int r = filled + __builtin_popcountll(all & ((1ull << lane) - 1));
+                    if (take && r < wanted) put(r, id_key(x0, (uint32_t)(base + i0 + lane)));
+                    filled += __builtin_popcountll(all);
+                }
+        }
         if (!whole)
-            for (int r = found + tid; r < top; r += kScoreThreads) cand[at * top + r] = 0;
+            for (int r = wanted + tid; r < top; r += kScoreThreads) cand[at * top + r] = 0;
         return;
     }
     u64 last = ~0ull;
