@@ -207,7 +207,10 @@ __global__ __launch_bounds__(kScoreThreads, 6) void k_score(const T* __restrict_
         if (!whole) {
             part[at] = make_float4(st.m, st.rest, st.t, 0.0f);
         } else {
-            if (logprob) logprob[row] = tokens[row] < vocab ? score.logprob((float)xr[tokens[row]]) : score.rest != score.rest ? score.rest : -INFINITY;
+            if (logprob)
+                logprob[row] = tokens[row] < vocab          ? score.logprob((float)xr[tokens[row]])
+                               : score.rest != score.rest ? score.rest
+                                                          : -INFINITY;
             if (entropy) entropy[row] = score.entropy();
         }
     }

@@ -10,17 +10,24 @@
 // group g holds positions 4g .. 4g + 3, and the order of positions inside a
 // product is free as long as V's operand has the same one.  V^T's operand
 // wants one dimension of 8 positions per lane while rows are stored dimension
-// by dimension: a lane loads HD / 16 neighbouring dimensions of its 8 positions
-// and picks each dimension's halves with v_perm, no lane exchange.
+// by dimension: from registers (row kernel) a lane loads HD / 16 neighbouring
+// dimensions of its 8 positions and picks each dimension's halves with v_perm, no
+// lane exchange; from LDS (tile kernel) transposing reads bring it as it is wanted.
+//
+// Kernels of a call, in the stream's order: the row kernel (sequences of few
+// rows, every f32 call), the tile kernel (sequences of many rows), one of the
+// two over a shared prefix, and a join of partial results where there are any.
 //
 // Precision: the products run on f16 / bf16 matrix instructions with f32 sums
 // while q and the weights are f32, so these are cut into parts that add up to
 // them: two f16 (22 bits; q scaled per row by a power of two, the weights by
-// 2^kBias, so that the second part keeps its bits) or three bf16 (24 bits).  f32
-// caches take the f32 matrix instructions.
+// 2^kBias, so that the second part keeps its bits) or three bf16 (24 bits; two
+// would leave errors of 2^-18 of a weight).  f32 caches take the f32 matrix
+// instructions.
 //
 // Softmax: running maximum and sum per row in base 2 (one pass over the keys).
-// The maximum is only raised when a score passes it by more than 2^kSlack.
+// The maximum is only raised when a score passes it by more than kSlack powers
+// of two, so that most steps need no exchange between lanes and no rescaling.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -43,7 +50,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // activations: any float address
 
-constexpr float kSlack = 8.0f;      // a score may pass the running maximum by this power of two
+constexpr float kSlack = 8.0f;      // powers of two by which a score may pass the running maximum
 
 // What depends on the cache's type.
 template <typename C> struct Type;
@@ -532,7 +539,8 @@ struct Tile {
 // Clears values that are not there, and among positions that not every row
 // attends to those that are no numbers; true if there was one of the latter.
 template <typename C, int HD>
-__device__ __forceinline__ bool clear_values(typename Tile<C, HD, false>::Value vr[Tile<C, HD, false>::NT][4], int p0, int hi, bool differ, const int page[], int g) {
+__device__ __forceinline__ bool clear_values(typename Tile<C, HD, false>::Value vr[Tile<C, HD, false>::NT][4], int p0, int hi,
+                                             bool differ, const int page[], int g) {
     using R = Tile<C, HD, false>;
     uint32_t odd = 0;
 #pragma unroll
@@ -598,11 +606,14 @@ __device__ __forceinline__ size_t part_of(const PagedAttn& a, int row, int head,
     return ((size_t)row * a.p.n_heads + head) * a.parts + a.part0 + split;
 }
 
-// One tile of 16 stacked rows over one split of the positions, the positions
+// One tile of 16 stacked rows over one stretch of the positions, the positions
 // dealt to four wavefronts in steps of 16 NT.  K and V go from memory to
 // registers in the operands' order; the next step's keys are loaded while
-// this one is computed.  Bound by memory: with few rows per kv head a byte of
-// the cache meets about as many operations as the matrix cores need.
+// this one is computed.  Bound by memory where there are workgroups enough: two
+// rows at 128,000 positions, 32 heads on 8, f16, hd 64: 91 us, 5.8 TB/s; 64 rows
+// at 100 .. 8000, bf16, hd 128: 122 us, 5.3 TB/s (units of unlike lengths).  A
+// single row at 600 positions 8 us: launch, three round trips, then what one CU
+// loads (57 GB/s); eight wavefronts for four, or values a step ahead, the same.
 template <typename C, int HD>
 __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int prefix) {
     using R = Tile<C, HD, false>;
@@ -759,10 +770,16 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
 }
 
 // Many rows over the same pages (prompts, a prefix under a batch) of an f16 or
-// bf16 cache: eight wavefronts of a row tile each share tiles of K and V in LDS, which LDS
-// DMA brings in while the tile before is computed.  In LDS a row's 16-byte
-// pieces are permuted by the row (piece ^ row), so that the 16 rows that a key
-// operand reads at one piece lie in different banks.
+// bf16 cache: eight wavefronts of a row tile each share tiles of K and V in
+// LDS, which LDS DMA brings in while the tile before is computed.  In LDS a row's
+// pieces are permuted by the row (piece ^ row), so that the rows that an operand
+// reads at one piece lie in different banks (no conflicts counted).  Bound by
+// matrix and vector instructions, which hardly overlap: four prompts of 7781
+// tokens, 32 heads on 8, f16, hd 64: 256 us, 370 TFLOP/s of the 4 hd per pair
+// that a user sees, twice that in the two parts; counters: matrix cores 39% of
+// the time, vector instructions 49%, clock 2.05 GHz.  Measured and dropped: two
+// row tiles a wavefront (309 us), 4 wavefronts (281), 128 positions a tile
+// (262); at hd 128, 12 and 16 wavefronts spill (bf16 326 us -> 412 and 699).
 constexpr int kTileWaves = 8, kTileRows = kTileWaves * kRowTile;
 // Of 4 rows by 16 columns of halfwords, of which the 16 lanes of a row of the
 // wavefront point to four halfwords each, lane c gets column c.
@@ -937,6 +954,8 @@ struct Parts {
 
 // Joins the partial results of a row, a wavefront per head (every fourth of
 // `heads` heads): weights 2^(m - max), HD / 64 (or one) dimensions per lane.
+// Bound by its round trips (lengths, weights, values): 4 to 7 us; a workgroup
+// per head with two barriers took 12 us for 96 rows of 32 heads, now 6.
 // `per_seq`: rows of every sequence that the row kernel took (that many of
 // each are looked at); 0: all rows.  Their own parts stand at `rows`, those
 // of the tile kernel (tile_parts, 0: it wrote `out`) and over the prefix at a.po.
@@ -1033,7 +1052,7 @@ struct AttnPlan {
 // tiles, of many.  One decoded row, 32 heads on 8, f16, hd 64, unsplit | split, in
 // us: 300 positions 7.0 | 8.9, 600 8.3 | 8.9, 1000 10.3 | 9.2, 2000 15.5 | 9.0.
 constexpr int kUnsplit = 640, kUnsplitMany = 2048;
-constexpr int kLeastChunk = 128;
+constexpr int kLeastChunk = 128;     // positions of a part at least
 // The tile kernel from as many workgroups of rows on (f16 and bf16 caches; f32's
 // matrix instructions take so long that K and V need not be shared).  One prompt
 // over itself, 32 heads on 8, in us, row kernel | tile kernel:
@@ -1059,13 +1078,13 @@ AttnPlan plan_attention(const PagedArgs& p, int dtype, uint32_t max_len) {
     const int64_t longest = max_len && max_len < cap ? max_len : cap;
     const int own = (int)std::max<int64_t>(longest - p.prefix_len, 0);
     // splits the positions of `tiles` tiles so that `wanted` workgroups have work
-    const auto split = [&](Launch* l, int64_t tiles, int positions, int wanted, int least) {
+    const auto split = [&](Launch* l, int64_t tiles, int positions, int wanted) {
         const int64_t want = std::max<int64_t>(wanted / std::max<int64_t>(tiles * p.n_kv, 1), 1);
-        l->splits = (int)std::clamp<int64_t>(want, 1, std::max(1, (positions + least - 1) / least));
+        l->splits = (int)std::clamp<int64_t>(want, 1, std::max(1, (positions + kLeastChunk - 1) / kLeastChunk));
         l->chunk = ((positions + l->splits - 1) / l->splits + 63) & ~63;
         l->splits = std::max(1, (positions + l->chunk - 1) / std::max(l->chunk, 1));
     };
-    const int resident = p.hd == 128 ? 256 : 512;    // workgroups of the tile kernel that run at once
+    const int resident = p.hd == 128 ? 256 : 512;    // workgroups of the tile kernel that run at once (their registers)
     r.both = p.row_start && dtype != YL_T_F32 && (stacked + R - 1) / R * p.n_kv >= kTileKernelGroups;
     r.per = (group + kRowTile - 1) / kRowTile;
     // tiles of the row kernel at most
@@ -1074,6 +1093,9 @@ AttnPlan plan_attention(const PagedArgs& p, int dtype, uint32_t max_len) {
                                        : stacked / kRowTile + p.n_seqs;
     r.split = own > (p.row_start && !r.both && tiles * p.n_kv >= 512 ? kUnsplitMany : kUnsplit);
     r.wanted = r.split ? std::max(1, 512 / p.n_kv) : p.row_start ? 1 : 0;
+    // One row per sequence: lengths differ, tiles of more than half the mean are
+    // split (64 sequences of 100 .. 8000 139 -> 134 us); rows of prompts: tiles of
+    // one length, which stay whole where there are many.
     r.finer = p.row_start ? 0.95f : 2.0f;
     r.max_units = (int)(tiles + std::max<int64_t>(r.wanted, r.split ? 2 * tiles : 0));
     r.join_rows = r.split || p.prefix_len;
@@ -1081,7 +1103,7 @@ AttnPlan plan_attention(const PagedArgs& p, int dtype, uint32_t max_len) {
     if (p.prefix_len) {
         r.prefix_by_tile = dtype != YL_T_F32 && stacked * p.n_kv * p.prefix_len >= kPrefixByTile;
         r.prefix.tiles = (int)((stacked + (r.prefix_by_tile ? R : kRowTile) - 1) / (r.prefix_by_tile ? R : kRowTile));
-        split(&r.prefix, r.prefix.tiles, p.prefix_len, r.prefix_by_tile ? resident : 512, kLeastChunk);
+        split(&r.prefix, r.prefix.tiles, p.prefix_len, r.prefix_by_tile ? resident : 512);
     } else {
         r.prefix.splits = 0;
     }
@@ -1147,7 +1169,8 @@ hipError_t launch_all(PagedAttn a, const AttnPlan& plan, float* space, hipStream
     const int heads = (int)std::clamp<int64_t>((int64_t)rows * a.p.n_heads / 4096, 4, std::max(4, a.p.n_heads));
     const dim3 grid((unsigned)rows * ((a.p.n_heads + heads - 1) / heads));
     auto join = a.p.hd == 32 ? k_paged_attn_join<32> : a.p.hd == 64 ? k_paged_attn_join<64> : k_paged_attn_join<128>;
-    hipLaunchKernelGGL(join, grid, dim3(256), 0, s, a, heads, plan.per_seq, (const float*)space, (const float2*)ml, plan.tile_parts, plan.prefix.splits);
+    hipLaunchKernelGGL(join, grid, dim3(256), 0, s, a, heads, plan.per_seq, (const float*)space, (const float2*)ml,
+                       plan.tile_parts, plan.prefix.splits);
     return hipGetLastError();
 }
 
@@ -1188,8 +1211,9 @@ yl_status yl_paged_attention(float* out, size_t out_ld, const float* q, size_t q
     a.group = a.p.n_heads / a.p.n_kv;
     hipStream_t s = (hipStream_t)stream;
     float* space = static_cast<float*>(workspace);
-    const hipError_t e = cache->dtype == YL_T_F32 ? launch_all<float>(a, plan, space, s) : cache->dtype == YL_T_F16 ? launch_all<_Float16>(a, plan, space, s)
-                                                                                                                  : launch_all<__bf16>(a, plan, space, s);
+    const hipError_t e = cache->dtype == YL_T_F32   ? launch_all<float>(a, plan, space, s)
+                         : cache->dtype == YL_T_F16 ? launch_all<_Float16>(a, plan, space, s)
+                                                    : launch_all<__bf16>(a, plan, space, s);
     if (e == hipSuccess) return YL_OK;
     set_error(std::string("paged_attention launch: ") + hipGetErrorString(e));
     return YL_ERR_HIP;
