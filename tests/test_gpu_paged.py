@@ -363,6 +363,34 @@ def test_many_sequences(gpu):
     _check(sc, _attend(sc))
 
 
+@pytest.mark.parametrize("seqs", [200, 256, 257, 512, 513, 1500])
+@pytest.mark.parametrize("single,prefix", [(True, 0), (False, 0), (False, 37), (True, 37)])
+def test_long_sequences_among_many(gpu, seqs, single, prefix):
+    """Two long sequences among many short ones, on both sides of every number
+    of sequences from which on the work is divided in another way."""
+    rng = np.random.default_rng(seqs)
+    rows = [1] * seqs if single else [int(x) for x in rng.integers(0, 4, seqs)]
+    lens = [prefix + int(r + x) for r, x in zip(rows, rng.integers(0, 40, seqs))]
+    for at, n in ((seqs // 3, 2500), (seqs - 1, 1900)):
+        rows[at], lens[at] = max(rows[at], 1), prefix + n
+    sc = Scene(rows, lens, 2, 1, 32, 16, "f16", prefix=prefix, seed=seqs)
+    _check(sc, _attend(sc, single))
+
+
+@pytest.mark.parametrize("seqs", [300, 1040])
+@pytest.mark.parametrize("prefix", [0, 20])
+def test_prompts_among_many_sequences(gpu, seqs, prefix):
+    """The same, with prompts among them that the tile kernel takes (160 workgroups of 128 stacked rows)."""
+    rows = [1] * seqs
+    for at in range(5, 300, 15):
+        rows[at] = 33 + at // 3
+    lens = [prefix + r + i % 9 for i, r in enumerate(rows)]
+    lens[7] = prefix + 800
+    sc = Scene(rows, lens, 16, 16, 32, 16, "bf16", prefix=prefix, seed=seqs)
+    assert -(-sum(rows) // 128) * 16 >= 160
+    _check(sc, _attend(sc))
+
+
 # ------------------------------------------------------------------ append
 
 

@@ -33,6 +33,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "../../include/yallma3.h"
 #include "yl_device.h"
@@ -164,8 +165,8 @@ struct PagedAttn {
     int direct;                      // this launch sees all that its rows attend to: it writes `out`
     // the row kernel's own work: units wanted, beyond one per tile, and units
     // there is room for; where each sequence's units begin and how many its
-    // tiles have, for the joining kernel.  wanted 0: one row per sequence, a unit
-    // for each of its `per` tiles, positions not split
+    // tiles have, for the joining kernel.  wanted 0: positions not split, a unit
+    // for each slot of `per` per sequence of one row, or as of tile_of_slot
     int per, wanted, max_units;
     float finer;                     // units wanted per tile where there are many tiles
     int4* units;
@@ -200,13 +201,14 @@ __device__ __forceinline__ RowSet set_of_seq(const PagedArgs& p, int seq) {
 // group / rows of a tile) + s on, of which it uses one per tile: a sequence's
 // slots always suffice, and are found by a search over row_start alone (64
 // starts per step, one per lane).  False: a slot that nothing uses.
+__device__ __forceinline__ int first_slot(const PagedAttn& a, int s, int rows_log2) {
+    const uint32_t st = a.p.row_start[s];
+    return (int)(((int64_t)(st < (uint32_t)a.p.n_rows ? (int)st : a.p.n_rows) * a.group) >> rows_log2) + s;
+}
 __device__ __forceinline__ bool tile_of_slot(const PagedAttn& a, int slot, int rows_log2, RowSet* set, int* tile) {
     const PagedArgs& p = a.p;
     const int lane = threadIdx.x & 63;
-    const auto base = [&](int s) {
-        const uint32_t st = p.row_start[s];
-        return (int)(((int64_t)(st < (uint32_t)p.n_rows ? (int)st : p.n_rows) * a.group) >> rows_log2) + s;
-    };
+    const auto base = [&](int s) { return first_slot(a, s, rows_log2); };
     int lo = 0, n = p.n_seqs;
     while (n > 1) {
         const int step = (n + 63) >> 6;
@@ -236,7 +238,7 @@ __device__ __forceinline__ int limit_of_row(const PagedAttn& a, const RowSet& se
     return set.seq < 0 ? min(lim, a.p.prefix_len) : max(lim - a.p.prefix_len, 0);
 }
 
-constexpr int kRowTile = 16;
+constexpr int kRowTile = 16, kRowTileLog2 = 4;
 
 // Stacked rows of a sequence (tokens times heads per kv head) up to which the
 // row kernel takes it where there is work for the tile kernel.
@@ -267,51 +269,59 @@ __device__ __forceinline__ float wave_sum(float x) {   // every lane active
     return (lane_value(x, 0) + lane_value(x, 16)) + (lane_value(x, 32) + lane_value(x, 48));
 }
 
+// Sequences up to which their work is divided by their lengths: beyond it there
+// are workgroups enough, and the kernel finds its tile by a search.  32 heads on
+// 8, hd 64, f16, one row each, divided | not, in us: 512 of 100 .. 8000 positions
+// 373 | 407, of 100 .. 3000 208 | 194; 1024 of them 721 | 707, 405 | 338.
+constexpr int kDivided = 512;
+
 // Unit `u` of the batch.  All tiles' positions together, divided by the units
 // wanted, are a unit's share: a long sequence becomes many units, a short one
 // one, whatever the lengths are when the work runs.  Every wavefront works
-// this out from the lengths (64 sequences per step, one per lane), alike.
+// this out from the lengths, alike (all of them in flight at once: as two loops
+// of 64 a step 512 sequences of 100 .. 3000 took 251).
 __device__ __forceinline__ bool unit_of(const PagedAttn& a, int u, Unit* r) {
+    constexpr int K = kDivided / 64;
     const PagedArgs& p = a.p;
-    const int lane = threadIdx.x & 63;
-    // a sequence's tiles (none where the tile kernel takes it) and its longest row's positions
-    const auto of_seq = [&](int s, int* tiles, int* len) {
-        *tiles = *len = 0;
-        if (s >= p.n_seqs) return;
+    const int lane = threadIdx.x & 63, steps = (p.n_seqs + 63) >> 6;
+    // sequences' tiles (none where the tile kernel takes them) and their longest rows' positions
+    int tiles[K], len[K];
+    float sum = 0.0f, all = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const int s = 64 * k + lane;
+        tiles[k] = len[k] = 0;
+        if (k >= steps || s >= p.n_seqs) continue;
         int first, end;
         paged_rows(p, s, &first, &end);
-        const int n = end - first;
-        if (n == 0 || (a.both && !row_kernel_takes(n, a.group))) return;
-        *tiles = (n * a.group + kRowTile - 1) / kRowTile;
-        *len = max(paged_limit(p, (int64_t)p.kv_len[s] - 1) - p.prefix_len, 0);
-    };
-    int tiles, len;
-    of_seq(lane, &tiles, &len);
-    float sum = 0.0f, all = 0.0f;
-    for (int s0 = 0;;) {
-        sum += wave_sum((float)tiles * (float)len);
-        all += wave_sum((float)tiles);
-        s0 += 64;
-        if (s0 >= p.n_seqs) break;
-        of_seq(s0 + lane, &tiles, &len);
+        const int n = end - first, held = max(paged_limit(p, (int64_t)p.kv_len[s] - 1) - p.prefix_len, 0);
+        if (n == 0 || (a.both && !row_kernel_takes(n, a.group))) continue;
+        tiles[k] = (n * a.group + kRowTile - 1) / kRowTile;
+        len[k] = held;
+        sum += (float)tiles[k] * (float)held;
+        all += (float)tiles[k];
     }
+    sum = wave_sum(sum);
+    all = wave_sum(all);
     // (rounded up beyond the sum's own rounding, so that the units never are more than there is room for)
     const float share = sum * 1.001f / fmaxf((float)a.wanted, a.finer * all);
     const int chunk = share < 1e9f && a.chunk < 1 << 30 ? (max((int)share + 1, a.chunk) + 63) & ~63 : 1 << 30;
     int before = 0;
-    for (int s0 = 0; s0 < p.n_seqs; s0 += 64) {
-        if (p.n_seqs > 64) of_seq(s0 + lane, &tiles, &len);
-        const int splits = max(1, (int)(((unsigned)len + (unsigned)chunk - 1u) / (unsigned)chunk));
-        const int mine = tiles * splits, upto = before + scan_add(mine);
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        if (k >= steps) break;
+        const int splits = max(1, (int)(((unsigned)len[k] + (unsigned)chunk - 1u) / (unsigned)chunk));
+        const int mine = tiles[k] * splits, upto = before + scan_add(mine);
         const auto here = __ballot(u < upto);
         if (here) {
             const int l = __builtin_ctzll(here);
-            r->seq = s0 + l;
+            r->seq = 64 * k + l;
             r->splits = __builtin_amdgcn_readlane(splits, l);
             r->first = __builtin_amdgcn_readlane(upto - mine, l);
-            const int k = u - r->first;
-            r->tile = k / r->splits;
-            r->split = k - r->tile * r->splits;
+            const int i = u - r->first;
+            if (i < 0) return false;                       // (starts that do not ascend)
+            r->tile = i / r->splits;
+            r->split = i - r->tile * r->splits;
             r->chunk = chunk;
             return true;
         }
@@ -625,21 +635,24 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
     const int c = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x % a.p.n_kv, slot = blockIdx.x / a.p.n_kv;
     RowSet set;
-    Unit u{0, slot, (int)blockIdx.y, 1, 0, 0};
+    Unit u{0, slot, (int)blockIdx.y, 1, 0, 0};     // (own pages: the grid is flat)
     if (prefix) {
         set = prefix_set(a);
     } else {
         if (a.wanted) {
             if (!unit_of(a, slot, &u)) return;
             if (a.joined && slot == u.first && kvh == 0 && tid == 0) a.units[u.seq] = make_int4(u.first, u.splits, 0, 0);
+        } else if (a.p.row_start) {
+            if (!tile_of_slot(a, slot, kRowTileLog2, &set, &u.tile)) return;
+            u.seq = set.seq;
+            u.first = slot - u.tile;
         } else {
             u.seq = slot / a.per;
             u.first = u.seq * a.per;
             u.tile = slot - u.first;
-            u.split = 0;
         }
         set = set_of_seq(a.p, u.seq);
-        if (u.tile * kRowTile >= set.rows * a.group || (a.both && !row_kernel_takes(set.rows, a.group))) return;
+        if ((int64_t)(uint32_t)u.tile * kRowTile >= (int64_t)set.rows * a.group || (a.both && !row_kernel_takes(set.rows, a.group))) return;
     }
     const bool direct = a.direct && u.splits == 1;
     R r;
@@ -976,7 +989,7 @@ __global__ __launch_bounds__(256) void k_paged_attn_join(PagedAttn a, int heads,
     int4 u = make_int4(0, tile_parts, 0, 0);
     if (by_rows) {
         if (!a.joined) return;                             // not split: written by its kernel
-        u = a.wanted ? a.units[s] : make_int4(s * a.per, 1, 0, 0);
+        u = a.wanted ? a.units[s] : make_int4(a.p.row_start ? first_slot(a, s, kRowTileLog2) : s * a.per, 1, 0, 0);
     }
     if (prefix_parts == 0 && (by_rows ? u.y == 1 : u.y == 0)) return;
     for (int head = head0 + wave; head < min(head0 + heads, a.p.n_heads); head += 4) {
@@ -1052,6 +1065,7 @@ struct AttnPlan {
 // tiles, of many.  One decoded row, 32 heads on 8, f16, hd 64, unsplit | split, in
 // us: 300 positions 7.0 | 8.9, 600 8.3 | 8.9, 1000 10.3 | 9.2, 2000 15.5 | 9.0.
 constexpr int kUnsplit = 640, kUnsplitMany = 2048;
+constexpr int kEnough = 2048;        // tiles of all kv heads
 constexpr int kLeastChunk = 128;     // positions of a part at least
 // The tile kernel from as many workgroups of rows on (f16 and bf16 caches; f32's
 // matrix instructions take so long that K and V need not be shared).  One prompt
@@ -1087,17 +1101,23 @@ AttnPlan plan_attention(const PagedArgs& p, int dtype, uint32_t max_len) {
     const int resident = p.hd == 128 ? 256 : 512;    // workgroups of the tile kernel that run at once (their registers)
     r.both = p.row_start && dtype != YL_T_F32 && (stacked + R - 1) / R * p.n_kv >= kTileKernelGroups;
     r.per = (group + kRowTile - 1) / kRowTile;
-    // tiles of the row kernel at most
-    const int64_t tiles = !p.row_start ? (int64_t)p.n_seqs * r.per
-                          : r.both     ? std::min<int64_t>((int64_t)p.n_seqs * (kRowKernelRows / kRowTile), stacked / kRowTile + p.n_seqs)
-                                       : stacked / kRowTile + p.n_seqs;
-    r.split = own > (p.row_start && !r.both && tiles * p.n_kv >= 512 ? kUnsplitMany : kUnsplit);
-    r.wanted = r.split ? std::max(1, 512 / p.n_kv) : p.row_start ? 1 : 0;
+    // tiles of the row kernel at most: slots of tile_of_slot, or fewer where the
+    // tile kernel has the large sequences and the units are counted through
+    const int64_t slots = stacked / kRowTile + p.n_seqs;
+    const bool many = p.n_seqs > kDivided;
+    r.split = !many && own > (p.row_start && !r.both && slots * p.n_kv >= 512 ? kUnsplitMany : kUnsplit);
+    const bool search = !r.split && (!r.both || many || slots <= 4 * (int64_t)p.n_seqs);
+    const int64_t tiles = !p.row_start          ? (int64_t)p.n_seqs * r.per
+                          : r.both && !search ? std::min<int64_t>((int64_t)p.n_seqs * (kRowKernelRows / kRowTile), slots)
+                                              : slots;
+    r.wanted = r.split ? std::max(1, 512 / p.n_kv) : p.row_start && !search ? 1 : 0;
     // One row per sequence: lengths differ, tiles of more than half the mean are
-    // split (64 sequences of 100 .. 8000 139 -> 134 us); rows of prompts: tiles of
-    // one length, which stay whole where there are many.
-    r.finer = p.row_start ? 0.95f : 2.0f;
-    r.max_units = (int)(tiles + std::max<int64_t>(r.wanted, r.split ? 2 * tiles : 0));
+    // split (64 sequences of 100 .. 8000 139 -> 134 us; 128, hd 64, 98 against 102
+    // for those above the mean), those above the mean where there are workgroups
+    // enough (512 sequences 380 -> 373, of 100 .. 3000 232 -> 210).  Rows of
+    // prompts: tiles of one length, which stay whole where there are many.
+    r.finer = p.row_start ? 0.95f : tiles * p.n_kv >= kEnough ? 1.0f : 2.0f;
+    r.max_units = (int)(tiles + std::max<int64_t>(r.wanted, r.split ? (int64_t)std::ceil(r.finer * (float)tiles) + 1 : 0));
     r.join_rows = r.split || p.prefix_len;
     if (r.both) r.tile.tiles = (int)(stacked / R) + p.n_seqs;
     if (p.prefix_len) {
