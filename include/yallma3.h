@@ -301,7 +301,9 @@ yl_status yl_paged_append(const yl_paged_cache *cache, const yl_paged_batch *bat
  * h / (n_heads / n_kv_heads); out = sum_j e_j v_j / sum_j e_j with
  * e_j = exp(attn_scale q . k_j - max).  A row that has nothing to attend to
  * gets zeros.  Whatever lies at positions a row does not attend to takes no
- * part.  q, out: [n_rows] rows of n_heads * head_size floats (device), q_ld
+ * part.  An infinity or NaN in a row's own q, or in a key it attends to, leaves
+ * that row and head without defined values (in a value it attends to, that one
+ * component); no other row or head feels it.  q, out: [n_rows] rows of n_heads * head_size floats (device), q_ld
  * and out_ld floats apart; out may be q (with q_ld) but not overlap it
  * otherwise.  A prefix is read once for all sequences.  workspace (device,
  * 16-byte aligned): yl_paged_attention_workspace bytes, its contents of no

@@ -189,6 +189,26 @@ def test_non_finite_value_alone(gpu, dtype, bad):
     assert (np.abs(out - ref)[fine] <= bound[fine]).all()
 
 
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+@pytest.mark.parametrize("dtype,heads,kvh", [("f32", 8, 2), ("f16", 8, 2), ("bf16", 8, 2), ("f16", 160, 160), ("bf16", 160, 160)])
+@pytest.mark.parametrize("prefix", [0, 30])
+def test_non_finite_queries(gpu, dtype, heads, kvh, bad, prefix):
+    """Queries that are no numbers spoil their own row and head alone (in both kernels)."""
+    sc = Scene([1, 70, 60, 3], [prefix + n for n in (700, 90, 60, 5)], heads, kvh, 32, 16, dtype, prefix=prefix, seed=17)
+    spoilt = [(0, 1), (5, 0), (5, heads - 1), (100, 3), (133, 2)]
+    for row, head in spoilt:
+        sc.q[row, head * 32 + 3] = bad
+    out = _attend(sc).reshape(sc.total, heads, 32)
+    for row, head in spoilt:
+        sc.q[row, head * 32 + 3] = 0.0
+    ref, bound = (x.reshape(sc.total, heads, 32) for x in sc.attention())
+    fine = np.ones((sc.total, heads), bool)
+    for row, head in spoilt:
+        fine[row, head] = False
+    assert not np.isnan(bad) or np.isnan(out[~fine]).all()
+    assert (np.abs(out - ref)[fine] <= bound[fine]).all()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("size", [1e-4, 30.0])
 def test_small_and_large_scores(gpu, dtype, size):
