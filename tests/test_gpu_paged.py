@@ -591,3 +591,71 @@ def test_serving_steps(gpu):
         assert np.array_equal(ids, rids)
         for a, b in ((lp, rlp), (ent, rent), (tlp, rtlp)):
             assert np.abs(a - b).max() <= 1e-5
+
+
+@pytest.mark.parametrize("dtype,heads,kvh,prefix", [("f16", 8, 2, 0), ("bf16", 8, 2, 40), ("f32", 4, 4, 20), ("f16", 160, 160, 0)])
+def test_a_captured_step(gpu, dtype, heads, kvh, prefix):
+    """Append, attention and scoring captured once and replayed with other
+    rows per sequence and lengths, eager calls of the same between the replays."""
+    hd = 32
+    sc = Scene([0] * 4, [prefix + n for n in (900, 60, 300, 90)], heads, kvh, hd, 16, dtype, prefix=prefix, seed=31, behind=70)
+    width = (heads + 2 * kvh) * hd
+    cos, sin = _tables(hd, prefix + 900, seed=2)
+    dc, ds = buffer(cos), buffer(sin)
+    tokens = np.arange(sc.total) % 11
+
+    class Step:
+        def __init__(self):
+            self.call, self.x, self.tokens = Call(gpu, sc), filled((sc.total, width), 0.0), buffer(tokens.astype(np.uint32))
+            self.lp, self.ent = filled(sc.total, 0.0), filled(sc.total, 0.0)
+            self.ids, self.tlp = filled((sc.total, 5), 0, np.uint32), filled((sc.total, 5), 0.0)
+            self.need = gpu.lib().yl_token_logprobs_workspace(sc.total, heads * hd, 5)
+            self.space = bytes_of(self.need, 255)
+
+        def set(self, x):
+            self.x.upload(x)
+            self.call.put_q(x[:, :heads * hd])
+            self.call.kv_len.upload(np.array(sc.lens, np.uint32))
+            self.call.starts.upload(sc.starts)
+            self.call.out.upload(np.full(self.call.out.shape, 7.0, np.float32))
+
+        def __call__(self, stream=None):
+            c, at = self.call, self.x.ptr
+            gpu.check(gpu.lib().yl_paged_append(C.byref(c.cache), C.byref(c.batch), heads, c.q.ptr, heads * hd, at, width,
+                                                at + 4 * heads * hd, width, at + 4 * (heads + kvh) * hd, width,
+                                                gpu.ROPE_PAIRS["half"], dc.ptr, ds.ptr, prefix + 900, stream))
+            c(stream)
+            gpu.check(gpu.lib().yl_token_logprobs(c.out.ptr, 0, sc.total, heads * hd, heads * hd, self.tokens.ptr, self.lp.ptr,
+                                                  self.ent.ptr, 5, self.ids.ptr, self.tlp.ptr, self.space.ptr, self.need, stream))
+
+        def results(self):
+            gpu.check(gpu.lib().yl_synchronize())
+            return [b.numpy().copy() for b in (self.call.out, self.call.q, self.call.k, self.call.v, self.lp, self.ent, self.ids, self.tlp)]
+
+    captured, eager = Step(), Step()
+    graph = Graph(captured)
+    for rows, own in ([1, 20, 33, 6], [900, 60, 300, 90]), ([1, 1, 1, 1], [850, 30, 299, 1]), ([3, 0, 60, 7], [700, 10, 60, 90]), \
+                     ([70, 0, 0, 0], [70, 0, 5, 1]), ([0, 35, 0, 35], [1, 60, 1, 80]):
+        sc.rows, sc.lens = rows, [prefix + n for n in own]
+        sc.starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.uint32)
+        x = sc.rng.standard_normal((sc.total, width), np.float32)
+        for step in (captured, eager):
+            step.set(x)
+        graph.replay()
+        eager()
+        a, b = captured.results(), eager.results()
+        for p, q in zip(a, b):
+            assert np.array_equal(p.view(np.uint8), q.view(np.uint8))
+        out, q = a[0].reshape(sc.total, -1), a[1].reshape(sc.total, -1)
+        n = sum(rows)
+        sc.q = q
+        sc.k32, sc.v32 = widened(a[2]).astype(np.float32), widened(a[3]).astype(np.float32)
+        ref, bound = sc.attention()
+        assert (np.abs(out[:n] - ref[:n]) <= bound[:n]).all() and (out[n:] == 7.0).all()
+        pos = np.concatenate([np.arange(m - r, m) for r, m in zip(rows, sc.lens)])
+        assert np.abs(q[:n] - rotated(x[:n, :heads * hd], cos, sin, pos, "half", heads, hd).reshape(n, -1)).max() <= 6 * 2.0 ** -24 * np.abs(x).max()
+        assert np.array_equal(q[n:], x[n:, :heads * hd])
+        rlp, rent, rids, rtlp = logprobs(out.astype(np.float64), tokens, 5)
+        assert np.array_equal(a[6], rids)
+        for got, want in zip((a[4], a[5], a[7]), (rlp, rent, rtlp)):
+            assert np.abs(got - want).max() <= 1e-5
