@@ -25,9 +25,14 @@
 // would leave errors of 2^-18 of a weight).  f32 caches take the f32 matrix
 // instructions.
 //
-// Softmax: running maximum and sum per row in base 2 (one pass over the keys).
-// The maximum is only raised when a score passes it by more than kSlack powers
-// of two, so that most steps need no exchange between lanes and no rescaling.
+// Softmax: running reference and sum per row in base 2 (one pass over the keys);
+// the weight of a score is 2^(score - reference).  The reference is the largest
+// score less the type's bias when it is set, and is only raised when a weight
+// would pass 2^kMost, so that most steps need no exchange between lanes and no
+// rescaling.  Scores come out of the products times a power of two (the scale's
+// mantissa is multiplied into q), so that one fma subtracts the reference from
+// the score itself: a product rounded on its way would be off by many powers of
+// two where scores are large.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -51,16 +56,14 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // activations: any float address
 
-constexpr float kSlack = 8.0f;      // powers of two by which a score may pass the running maximum
-
 // What depends on the cache's type.
 template <typename C> struct Type;
 template <> struct Type<_Float16> {
     static constexpr uint32_t kOnes = 0x3c003c00u;
     static constexpr int kParts = 2, kTiles = 2;   // parts of an f32 value; 16-position tiles of one step
-    // weights are held times 2^6: at most 2^14 with the slack, and a weight's
-    // second part keeps its bits down to 2^-30
-    static constexpr float kBias = 6.0f;
+    // the largest weight is 2^6 when the reference is set, so that a weight's
+    // second part keeps its bits down to 2^-30 of it, and at most 2^14
+    static constexpr float kBias = 6.0f, kMost = 14.0f;
     static __device__ __forceinline__ vf4 mul(u4 a, u4 b, vf4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
     }
@@ -72,7 +75,7 @@ template <> struct Type<_Float16> {
         asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]\n\tv_fma_mixhi_f16 %0, %1, -1.0, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
             : "=&v"(part[1]) : "v"(part[0]), "v"(a), "v"(b));
     }
-    // the power of two that brings a row of q to [2^9, 2^10)
+    // the power of two that brings a row of q to [2^8, 2^9)
     static __device__ __forceinline__ int exponent(float amax) {
         return amax > 0.0f && amax < INFINITY ? min(9 - __builtin_amdgcn_frexp_expf(amax), 110) : 0;
     }
@@ -84,7 +87,7 @@ template <> struct Type<_Float16> {
 template <> struct Type<__bf16> {
     static constexpr uint32_t kOnes = 0x3f803f80u;
     static constexpr int kParts = 3, kTiles = 2;
-    static constexpr float kBias = 0.0f;
+    static constexpr float kBias = 0.0f, kMost = 8.0f;
     static __device__ __forceinline__ vf4 mul(u4 a, u4 b, vf4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
     }
@@ -106,7 +109,7 @@ template <> struct Type<__bf16> {
 };
 template <> struct Type<float> {
     static constexpr int kParts = 1, kTiles = 1;
-    static constexpr float kBias = 0.0f;
+    static constexpr float kBias = 0.0f, kMost = 8.0f;
     static __device__ __forceinline__ uint32_t not_finite(uint32_t x) { return (x & 0x7f800000u) == 0x7f800000u ? ~0u : 0u; }
     static __device__ __forceinline__ int exponent(float) { return 0; }
 };
@@ -157,7 +160,7 @@ struct PagedAttn {
     PagedArgs p;
     float* out; const float* q;
     size_t out_ld, q_ld;
-    float scale_log2;                // attn_scale * log2(e)
+    float scale; int scale_exp;      // attn_scale * log2(e) = scale * 2^scale_exp, 0.5 <= |scale| < 1
     int group;                       // query heads per kv head
     int parts, part0;                // partial results per row and head; the first of this launch's
     int chunk;                       // positions of a split at least
@@ -172,7 +175,7 @@ struct PagedAttn {
     int4* units;
     int joined;                      // the joining kernel follows
     int both;                        // sequences are divided between the row kernel and the tile kernel
-    // partial results, unnormalised, and their maximum (base 2) and sum, maximum
+    // partial results, unnormalised, and their reference (base 2) and sum, reference
     // -inf: nothing there.  Of the row kernel's own work [unit][n_kv][16 rows],
     // of the others [row][n_heads][parts]
     float* po;
@@ -350,7 +353,7 @@ struct Tile {
 
     int row, head, lim;              // lim: positions below it are attended to
     bool live;
-    float m, l, unscale;
+    float m, l, unscale;             // m: the weights' reference
     u4 qf[NP][NK];
     vf4 acc[NJ], ones;               // ones: sums of the weights (TR)
 
@@ -390,19 +393,17 @@ struct Tile {
 #pragma unroll
                 for (int i = 0; i < 4; i++) amax = fmaxf(amax, fabsf(v[k][e][i]));
             }
-        // scores times `unscale` > 0 are the exponents: q takes the sign (or the zero) of the scale
-        const float sign = a.scale_log2 < 0.0f ? -1.0f : a.scale_log2 == 0.0f ? 0.0f : 1.0f;
-        unscale = a.scale_log2 == 0.0f ? 1.0f : fabsf(a.scale_log2);
+        // scores times `unscale`, a power of two, are the exponents
 #pragma unroll
         for (int k = 0; k < NK; k++)
 #pragma unroll
-            for (int e = 0; e < KE / 4; e++) v[k][e] *= sign;
+            for (int e = 0; e < KE / 4; e++) v[k][e] *= a.scale;
+        int ex = 0;
         if constexpr (F32) {
 #pragma unroll
             for (int k = 0; k < NK; k++) qf[0][k] = __builtin_bit_cast(u4, v[k][0]);
         } else {
-            const int ex = T::exponent(group_max16(amax));
-            if (ex) unscale = __builtin_amdgcn_ldexpf(unscale, -ex);
+            ex = T::exponent(group_max16(amax * fabsf(a.scale)));
 #pragma unroll
             for (int k = 0; k < NK; k++)
 #pragma unroll
@@ -413,6 +414,7 @@ struct Tile {
                     for (int p = 0; p < NP; p++) qf[p][k][i] = part[p];
                 }
         }
+        unscale = __builtin_amdgcn_ldexpf(1.0f, min(max(a.scale_exp - ex, -126), 127));
     }
     // scores of the step's positions, before `unscale` (the tiles' chains of products side by side)
     __device__ __forceinline__ void scores(const u4 kc[NT][NK], float s[NT][4]) const {
@@ -448,7 +450,7 @@ struct Tile {
                 if (page[t] < 0 || pos >= min(lim, hi)) s[t][i] = -INFINITY;
             }
     }
-    // scores -> weights of N tiles of positions, under a maximum that is raised where it has to be
+    // scores -> weights of N tiles of positions, under a reference that is raised where it has to be
     template <int N>
     __device__ __forceinline__ void weigh(float (*s)[4]) {
         float mx = s[0][0];
@@ -456,21 +458,24 @@ struct Tile {
         for (int t = 0; t < N; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[t][i]);
-        if (__ballot(mx * unscale > m + kSlack)) {    // (m = -inf: any score raises it)
-            const float m_new = fmaxf(m, group_max16(mx) * unscale);
-            const float alpha = m_new == m ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+        if (__ballot(fmaf(mx, unscale, -m) > T::kMost)) {    // (m = -inf: any score raises it)
+            const float top = group_max16(mx) * unscale;
+            float to = fmaxf(m, top - T::kBias);
+            // (where floats are further apart than the bias)
+            if (T::kBias > 0.0f && top - to > T::kMost) to = top;
+            const float alpha = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
             if constexpr (TR) ones *= alpha;
             else l *= alpha;
 #pragma unroll
             for (int j = 0; j < NJ; j++) acc[j] *= alpha;
-            m = m_new;
+            m = to;
         }
-        const float back = T::kBias - (m == -INFINITY ? 0.0f : m);
+        const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
         for (int t = 0; t < N; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], unscale, back));
+                s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], unscale, -ref));
                 if constexpr (!TR) l += s[t][i];
             }
     }
@@ -777,7 +782,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
         float* dst = a.po + at * HD + e0;
 #pragma unroll
         for (int k = 0; k < NJ; k++) dst[k] = o[k];
-        // (NaN scores alone leave the maximum at -inf: 0 marks the part as there)
+        // (NaN scores alone leave the reference at -inf: 0 marks the part as there)
         if ((tid & 15) == 0) a.pml[at] = make_float2(M == -INFINITY && L != 0.0f ? 0.0f : M, L);
     }
 }
@@ -893,7 +898,7 @@ __global__ __launch_bounds__(64 * kTileWaves, HD == 128 ? 2 : 4) void k_paged_at
         const char* kt = lds[buffer][0];
         const char* vt = lds[buffer][1];
         // a whole tile of positions per row tile at once: independent chains of
-        // products, one look at the maximum
+        // products, one look at the reference
         constexpr int NS = POS / STEP;
         const int p0 = lo + POS * t;
         if (p0 < min(wave_most, hi)) {
@@ -1227,7 +1232,7 @@ yl_status yl_paged_attention(float* out, size_t out_ld, const float* q, size_t q
     if (plan.bytes && (!workspace || (uintptr_t)workspace % 16)) return refuse("paged_attention: the workspace has to be there, 16-byte aligned");
     if (workspace_bytes < plan.bytes) return refuse("paged_attention: the workspace is smaller than yl_paged_attention_workspace says", YL_ERR_RANGE);
     a.out = out; a.q = q; a.out_ld = out_ld; a.q_ld = q_ld;
-    a.scale_log2 = attn_scale * 1.4426950408889634f;
+    a.scale = frexpf(attn_scale * 1.4426950408889634f, &a.scale_exp);
     a.group = a.p.n_heads / a.p.n_kv;
     hipStream_t s = (hipStream_t)stream;
     float* space = static_cast<float*>(workspace);
