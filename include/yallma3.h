@@ -305,7 +305,10 @@ yl_status yl_paged_append(const yl_paged_cache *cache, const yl_paged_batch *bat
  * that row and head without defined values (in a value it attends to, that one
  * component); no other row or head feels it.  q, out: [n_rows] rows of n_heads * head_size floats (device), q_ld
  * and out_ld floats apart; out may be q (with q_ld) but not overlap it
- * otherwise.  A prefix is read once for all sequences.  workspace (device,
+ * otherwise.  Sums are f32, products those of f32 but over f16 caches: there q
+ * has 22 bits, and so has a weight e_j (of 16 to 64 positions taken together,
+ * one below 2^-13 of their largest has fewer, and is right to 2^-23 of that).
+ * A prefix is read once for all sequences.  workspace (device,
  * 16-byte aligned): yl_paged_attention_workspace bytes, its contents of no
  * matter before and after; calls that may run at the same time need one each.
  * Smaller: YL_ERR_RANGE. */

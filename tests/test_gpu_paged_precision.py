@@ -49,3 +49,41 @@ def test_scores_far_from_zero(gpu, dtype, layout, hd, prefix, power):
                 looked_at += 1
                 assert (np.abs(out[r, h] - vv[first]) <= 4 * U * np.abs(vv[first])).all(), (r, h)
     assert looked_at >= 5
+
+
+def _sink(dtype, rows, heads, kvh, hd, n, at, gap, prefix=0):
+    """Position `at` has e^(gap ln 2) times every other position's weight and values of 0."""
+    sc = Scene([rows], [n], heads, kvh, hd, 16, dtype, prefix=prefix, seed=int(gap))
+    sc.scale = 0.125
+    held = ~np.isnan(sc.k32[:, :, :, :1])
+    sc.k32 = np.where(held, np.float32(0.0), np.float32(np.nan)) + np.zeros_like(sc.k32)
+    sc.v32 = np.where(held, sc.rng.uniform(0.5, 1.5, sc.v32.shape).astype(np.float32), np.float32(np.nan))
+    page, slot = sc.places(0, n)[at]
+    sc.k32[page, :, slot, 0] = 8.0
+    sc.v32[page, :, slot] = 0.0
+    sc.q = np.zeros_like(sc.q)
+    sc.q[:, ::hd] = gap * np.log(2.0)        # times 8, times the scale
+    return sc
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("layout,hd,n,prefix", [(ROWS, 64, 3000, 0), (ROWS, 128, 3000, 1500), (TILE, 32, 1500, 0), (TILE, 64, 700, 0)])
+@pytest.mark.parametrize("gap", [13.9, 21.3, 24.4, 31.0, 36.0])
+def test_small_weights_beside_a_large_one(gpu, dtype, layout, hd, n, prefix, gap):
+    """One position takes nearly all of the weight and adds nothing (its values
+    are 0): the result is made of weights of 2^-gap.
+
+    Bound, relative to the result: the exponent gap is rounded as the scale,
+    the scale times log2(e), the product and the difference (4 U gap ln 2 <=
+    3 U gap), exp2 (2 U), the parts of a weight (2 U, 2^-23), and the sums of equal
+    terms, up to n / 64 of them in a row and 64 in a product; twice for the
+    quotient.  Beside it, the positions of the large one's own step (at most 64)
+    may be off by 2^-36 of it each."""
+    rows, heads, kvh = layout
+    for at in (0, n // 2 + 3):
+        sc = _sink(dtype, rows, heads, kvh, hd, n, at, gap, prefix)
+        ref, _ = sc.attention()
+        assert 0 < ref.max() < 2 * n * 2.0 ** -gap
+        err = np.abs(_attend(sc) - ref)
+        bound = 2 * (3 * gap + 4 + n / 64 + 64) * U * ref + 64 * 2.0 ** -36 * 1.5
+        assert (err <= bound).all(), f"sink at {at}: off by {np.max(err / ref):.3g} of the result, {np.max(err / bound):.3g} of the bound"

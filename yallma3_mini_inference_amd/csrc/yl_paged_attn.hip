@@ -29,7 +29,9 @@
 // the weight of a score is 2^(score - reference).  The reference is the largest
 // score less the type's bias when it is set, and is only raised when a weight
 // would pass 2^kMost, so that most steps need no exchange between lanes and no
-// rescaling.  Scores come out of the products times a power of two (the scale's
+// rescaling.  Over f16 caches it also falls, by up to some 40 powers of two, where all of a step's
+// weights would be below 2^kLeast: f16 parts end at 2^-24, and beside one position
+// that has nearly all of the weight the others would lose their bits.  Scores come out of the products times a power of two (the scale's
 // mantissa is multiplied into q), so that one fma subtracts the reference from
 // the score itself: a product rounded on its way would be off by many powers of
 // two where scores are large.
@@ -61,9 +63,15 @@ template <typename C> struct Type;
 template <> struct Type<_Float16> {
     static constexpr uint32_t kOnes = 0x3c003c00u;
     static constexpr int kParts = 2, kTiles = 2;   // parts of an f32 value; 16-position tiles of one step
-    // the largest weight is 2^6 when the reference is set, so that a weight's
-    // second part keeps its bits down to 2^-30 of it, and at most 2^14
-    static constexpr float kBias = 6.0f, kMost = 14.0f;
+    // The largest weight of a step is between 2^-2 and 2^15 (2^11 when the
+    // reference is raised, 2^7 when it falls): a weight has 22 bits, and what is
+    // below 2^-2 is right to 2^-25, at most 2^-23 of the step's largest.  A prompt
+    // of 5280 tokens, hd 64, without falls | with kLeast 1 | -2 | -4, in us: scores of
+    // deviation 1 258.7 | 257.9 | 257.8 | 258.0, 2 258.6 | 262.1 | 260.3 | 259.9, 3 257.0 |
+    // 275.8 | 268.5 | 263.3.
+    static constexpr bool kFalls = true;
+    static constexpr float kBias = 11.0f, kMost = 15.0f, kLeast = -2.0f, kFall = 7.0f;
+    static constexpr int kRoom = 52;               // sums of weights are left below 2^52 by a fall
     static __device__ __forceinline__ vf4 mul(u4 a, u4 b, vf4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
     }
@@ -87,6 +95,7 @@ template <> struct Type<_Float16> {
 template <> struct Type<__bf16> {
     static constexpr uint32_t kOnes = 0x3f803f80u;
     static constexpr int kParts = 3, kTiles = 2;
+    static constexpr bool kFalls = false;
     static constexpr float kBias = 0.0f, kMost = 8.0f;
     static __device__ __forceinline__ vf4 mul(u4 a, u4 b, vf4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
@@ -109,6 +118,7 @@ template <> struct Type<__bf16> {
 };
 template <> struct Type<float> {
     static constexpr int kParts = 1, kTiles = 1;
+    static constexpr bool kFalls = false;
     static constexpr float kBias = 0.0f, kMost = 8.0f;
     static __device__ __forceinline__ uint32_t not_finite(uint32_t x) { return (x & 0x7f800000u) == 0x7f800000u ? ~0u : 0u; }
     static __device__ __forceinline__ int exponent(float) { return 0; }
@@ -458,11 +468,21 @@ struct Tile {
         for (int t = 0; t < N; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[t][i]);
-        if (__ballot(fmaf(mx, unscale, -m) > T::kMost)) {    // (m = -inf: any score raises it)
+        const float e = fmaf(mx, unscale, -m);               // (m = -inf: any score raises it)
+        bool off = e > T::kMost;
+        if constexpr (T::kFalls) off = !(e >= T::kLeast && e <= T::kMost);
+        if (__ballot(off)) {
             const float top = group_max16(mx) * unscale;
             float to = fmaxf(m, top - T::kBias);
             // (where floats are further apart than the bias)
             if (T::kBias > 0.0f && top - to > T::kMost) to = top;
+            if constexpr (T::kFalls) {
+                const bool low = top - m < T::kLeast && top > -INFINITY && fabsf(m) < 0x1p20f;   // (beyond it scores are not this exact)
+                if (__ballot(low)) {
+                    const int room = max(T::kRoom - __builtin_amdgcn_frexp_expf(sum()), 0);
+                    if (low) to = fmaxf(top - T::kFall, m - (float)room);
+                }
+            }
             const float alpha = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
             if constexpr (TR) ones *= alpha;
             else l *= alpha;
