@@ -87,3 +87,36 @@ def test_small_weights_beside_a_large_one(gpu, dtype, layout, hd, n, prefix, gap
         err = np.abs(_attend(sc) - ref)
         bound = 2 * (3 * gap + 4 + n / 64 + 64) * U * ref + 64 * 2.0 ** -36 * 1.5
         assert (err <= bound).all(), f"sink at {at}: off by {np.max(err / ref):.3g} of the result, {np.max(err / bound):.3g} of the bound"
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("layout,hd", [((16, 2, 1), 32), ((16, 2, 1), 64), ((16, 2, 1), 128), (TILE, 64)])
+def test_small_elements_of_a_query(gpu, dtype, layout, hd):
+    """Equal elements of q some 2^-24 of its largest decide between two
+    positions, whose keys are 2^14 and -2^14 there (and 0 at the largest element,
+    which keeps every other position out).
+
+    An element may be off by 2^-38 of the largest, 1.5, and by U of itself, all
+    of a row to the same side; a score by that times hd 2^14 and by its sum's
+    roundings, (hd + 8) U of its size; the result by a quarter of the two
+    scores' errors times the values' difference, and 14 U of the values."""
+    rows, heads, kvh = layout
+    sc = Scene([rows], [rows + 2], heads, kvh, hd, 16, dtype, seed=hd)
+    sc.scale = 1.0
+    small = (np.linspace(0.6, 1.7, sc.total * heads) * 2.0 ** -24).astype(np.float32).reshape(sc.total, heads)
+    q = np.repeat(small[..., None], hd, 2)
+    q[..., 0] = 1.5
+    sc.q = q.reshape(sc.total, heads * hd)
+    sc.k32[..., 1:] = 0.0
+    sc.k32[..., 0] = -1024.0
+    (pa, sa), (pb, sb) = sc.places(0, 2)
+    for page, slot, key in ((pa, sa, 2.0 ** 14), (pb, sb, -2.0 ** 14)):
+        sc.k32[page, :, slot] = key
+        sc.k32[page, :, slot, 0] = 0.0
+    ref, _ = sc.attention()
+    v = np.nan_to_num(widened(sc.pools()[1]))
+    va, vb = (np.repeat(v[page, :, slot], heads // kvh, 0)[None] for page, slot in ((pa, sa), (pb, sb)))
+    score = hd * 2.0 ** 14 * (2.0 ** -38 * 1.5 + (hd + 9) * U * small.astype(np.float64))[..., None]
+    bound = 0.5 * score * np.abs(va - vb) + 14 * U * np.maximum(np.abs(va), np.abs(vb))
+    err = np.abs(_attend(sc) - ref).reshape(sc.total, heads, hd)
+    assert (err <= bound).all(), f"off by {err.max():.3g}, {(err / bound).max():.3g} of the bound"

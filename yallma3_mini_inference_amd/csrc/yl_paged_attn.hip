@@ -20,8 +20,8 @@
 //
 // Precision: the products run on f16 / bf16 matrix instructions with f32 sums
 // while q and the weights are f32, so these are cut into parts that add up to
-// them: two f16 (22 bits; q scaled per row by a power of two, the weights by
-// 2^kBias, so that the second part keeps its bits) or three bf16 (24 bits; two
+// them: two f16 (22 bits; q scaled per row by a power of two, the weights against a
+// reference, so that the second part keeps its bits) or three bf16 (24 bits; two
 // would leave errors of 2^-18 of a weight).  f32 caches take the f32 matrix
 // instructions.
 //
@@ -83,9 +83,10 @@ template <> struct Type<_Float16> {
         asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]\n\tv_fma_mixhi_f16 %0, %1, -1.0, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
             : "=&v"(part[1]) : "v"(part[0]), "v"(a), "v"(b));
     }
-    // the power of two that brings a row of q to [2^8, 2^9)
+    // the power of two that brings a row of q to [2^13, 2^14): its elements keep
+    // 22 bits down to 2^-15 of the largest, and are right to 2^-38 of it below
     static __device__ __forceinline__ int exponent(float amax) {
-        return amax > 0.0f && amax < INFINITY ? min(9 - __builtin_amdgcn_frexp_expf(amax), 110) : 0;
+        return amax > 0.0f && amax < INFINITY ? min(14 - __builtin_amdgcn_frexp_expf(amax), 110) : 0;
     }
     // all bits of the halves that are no numbers
     static __device__ __forceinline__ uint32_t not_finite(uint32_t two) {
