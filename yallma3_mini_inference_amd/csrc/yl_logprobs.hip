@@ -55,6 +55,16 @@ __device__ __forceinline__ u64 wave_max64(u64 k) {
     return k;
 }
 
+// e^d for d <= 0 (NaN of NaN, 0 from -200 on: *d is raised to it).  exp2 is right to an
+// ulp, but its argument, d log2(e), is rounded, which at d = -30 would be 20 ulp
+// of the result: e^d = 2^t e^(d - t log(2)), whose second factor is 1 + (d - t
+// log(2)) to 2^-40.
+__device__ __forceinline__ float exp_below(float* d) {
+    *d = __builtin_elementwise_maximum(*d, -200.0f);       // (keeps NaN)
+    const float t = *d * 1.4426950408889634f, p = __builtin_amdgcn_exp2f(t);
+    return fmaf(p, fmaf(t, -0.6931471805599453f, *d), p);
+}
+
 // A stretch of a row: its maximum, the sum of exp(x - m) over all but one
 // holder of the maximum (whose 1 would hide the small ones), and the sum of
 // (x - m) exp(x - m).  m = -inf with rest 0: nothing probable.
@@ -67,9 +77,10 @@ __device__ __forceinline__ Stretch stretch_of(float m, float z, float t, int hol
 // Adds stretch b at the common maximum m; holder: whose maximum's 1 is left out.
 __device__ __forceinline__ void add_stretch(const Stretch& b, float m, bool holder, float* rest, float* t) {
     if (b.m == -INFINITY) { *rest += b.rest; return; }         // (0, or NaN)
-    const float d = b.m - m, all = b.rest + 1.0f;
+    float d = b.m - m;
+    const float all = b.rest + 1.0f;
     if (holder) { *rest += b.rest; *t += b.t; return; }
-    const float f = __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
+    const float f = exp_below(&d);
     if (f == 0.0f && all == all) return;
     *rest = fmaf(all, f, *rest);
     *t = fmaf(f, fmaf(d, all, b.t), *t);
@@ -172,25 +183,26 @@ __global__ __launch_bounds__(kScoreThreads, 6) void k_score(const T* __restrict_
     const float ms = m == -INFINITY ? 0.0f : m;
     float z = 0.0f, t = 0.0f;
     int holders = 0;
-    // (-inf: weight 0 times the lower bound of the difference; NaN stays NaN)
+    // (-inf: weight 0 times the least difference; NaN stays NaN)
     if (__ballot(mx == m)) {
         int mine = 0;
 #pragma unroll
         for (int k = 0; k < N; k++) {
-            const float d = v[k] - ms;
+            float d = v[k] - ms;
             const bool holds = d >= 0.0f;
-            const float e = holds ? 0.0f : __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
+            const float x = exp_below(&d), e = holds ? 0.0f : x;
             mine += holds;
             z += e;
-            t = fmaf(fmaxf(d, -200.0f), e, t);
+            t = fmaf(d, e, t);
         }
         for (u64 left = __ballot(mine > 0); left; left &= left - 1) holders += __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
     } else {
 #pragma unroll
         for (int k = 0; k < N; k++) {
-            const float d = v[k] - ms, e = __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
+            float d = v[k] - ms;
+            const float e = exp_below(&d);
             z += e;
-            t = fmaf(fmaxf(d, -200.0f), e, t);
+            t = fmaf(d, e, t);
         }
     }
     z = wave_sum(z);
