@@ -1,0 +1,98 @@
+"""What f32 evaluations of attention and of log probabilities are off by, in
+numpy: yardsticks that are tight enough to miss a lost part of a number, or a
+lost logit."""
+import numpy as np
+
+from paged_np import Scene, U, widened
+
+# name -> scene of a cache type: decoded rows, long contexts, prompts
+# of the row kernel and of the tile kernel (160 workgroups of 128 stacked rows),
+# prefixes of both (the tile kernel's from 2^23 stacked rows times positions on)
+SCENES = {
+    "decode_64": lambda d: Scene([1] * 6, [33, 64, 127, 200, 257, 600], 32, 8, 64, 16, d, seed=1),
+    "decode_128": lambda d: Scene([1] * 6, [33, 64, 127, 200, 257, 600], 8, 1, 128, 16, d, seed=1),
+    "long_64": lambda d: Scene([1, 1, 1, 2], [3001, 40, 1777, 2050], 4, 1, 64, 64, d, seed=2),
+    "long_128": lambda d: Scene([1, 1, 1, 2], [3001, 40, 1777, 2050], 4, 1, 128, 64, d, seed=2),
+    "prompt_32": lambda d: Scene([70, 3], [90, 300], 8, 2, 32, 16, d, seed=3),
+    "short": lambda d: Scene([16], [16], 8, 2, 64, 16, d, seed=3),
+    "prefix_64": lambda d: Scene([1, 5, 1, 2, 40, 1, 3], [334, 342, 383, 333, 393, 330, 334], 8, 2, 64, 16, d, prefix=333, seed=4),
+    "tile_32": lambda d: Scene([40, 0, 33, 70], [40, 7, 130, 75], 160, 160, 32, 16, d, seed=5),
+    "tile_64": lambda d: Scene([40, 0, 33, 70], [40, 7, 530, 75], 160, 160, 64, 16, d, seed=5),
+    "tile_128": lambda d: Scene([40, 0, 33, 70], [77, 44, 167, 112], 160, 160, 128, 16, d, prefix=37, seed=5),
+    "tile_prefix_64": lambda d: Scene([1] * 35 + [9], [1011 + 7 * i for i in range(36)], 192, 32, 64, 32, d, prefix=1010, seed=6),
+    "tile_prefix_128": lambda d: Scene([1] * 35 + [9], [1011 + 7 * i for i in range(36)], 192, 32, 128, 32, d, prefix=1010, seed=6),
+}
+
+
+def _of(sc, row, head):
+    """q, keys and values (f64) of a row and head of the scene."""
+    s = int(np.searchsorted(sc.starts, row, side="right")) - 1
+    k, v = sc._widened
+    pg, sl = np.array(sc.places(s, sc.lens[s] - (int(sc.starts[s + 1]) - row) + 1)).T
+    g = head // (sc.heads // sc.kvh)
+    return sc.q[row, head * sc.hd:(head + 1) * sc.hd].astype(np.float64), k[pg, g, sl], v[pg, g, sl]
+
+
+def sample(sc, count, seed=0):
+    """Up to `count` (row, head) that attend to something, from all of the batch."""
+    sc._widened = tuple(widened(x) for x in sc.pools())
+    rng = np.random.default_rng(seed)
+    rows = [r for s, n in enumerate(sc.lens) for r in range(sc.starts[s], sc.starts[s + 1])
+            if sc.places(s, max(0, n - (int(sc.starts[s + 1]) - r) + 1))]
+    return [(int(rng.choice(rows)), int(rng.integers(sc.heads))) for _ in range(count)]
+
+
+def exact(sc, at):
+    out = []
+    for q, k, v in (_of(sc, *a) for a in at):
+        s = k @ q * float(sc.scale)
+        e = np.exp(s - s.max())
+        out.append(e @ v / e.sum())
+    return np.array(out)
+
+
+def serial_f32(sc, at):
+    """The plain loop in f32: every product and every sum rounded, one after another."""
+    out = []
+    f = np.float32
+    for q, k, v in (_of(sc, *a) for a in at):
+        q, k, v = q.astype(f), k.astype(f), v.astype(f)
+        s = np.cumsum(q * k, axis=1, dtype=f)[:, -1] * f(sc.scale)
+        e = np.exp(s - s.max())
+        out.append(np.cumsum(e[:, None] * v, axis=0, dtype=f)[-1] / np.cumsum(e, dtype=f)[-1])
+    return np.array(out, np.float64)
+
+
+def cut(x, dtype, parts):
+    """f64 values as the sum of `parts` values of f16 (rounded, the largest of
+    the array brought to 2^13) or bf16 (cut off)."""
+    left, got = x.copy(), np.zeros_like(x)
+    unit = 2.0 ** (13 - np.floor(np.log2(np.abs(x).max())))
+    for _ in range(parts):
+        if dtype == "f16":
+            p = (left * unit).astype(np.float16).astype(np.float64) / unit
+        else:
+            p = (left.astype(np.float32).view(np.uint32) & np.uint32(0xFFFF0000)).view(np.float32).astype(np.float64)
+        got, left = got + p, left - p
+    return got
+
+
+def in_parts(sc, at, dtype, q_parts, weight_parts):
+    """64-bit sums of queries and weights that are held in so many parts."""
+    out = []
+    for q, k, v in (_of(sc, *a) for a in at):
+        s = k @ cut(q * float(sc.scale), dtype, q_parts)
+        e = np.exp(s - s.max())
+        out.append(cut(e, dtype, weight_parts) @ v / cut(e, dtype, weight_parts).sum())
+    return np.array(out)
+
+
+def rms(x):
+    return float(np.sqrt(np.mean(np.square(x))))
+
+
+def allowed(sc, at, ref):
+    """RMS error that a kernel may have: twice the serial loop's, which rounds
+    more sums than any kernel here, and 2 U of the results for the parts (U / 2
+    rms each at most) and the quotient."""
+    return 2 * rms(serial_f32(sc, at) - ref) + 2 * U * rms(ref)

@@ -3,6 +3,7 @@
 import numpy as np
 import pytest
 
+import precision_np as P
 from paged_np import Scene, U, widened
 
 pytestmark = pytest.mark.gpu
@@ -120,3 +121,16 @@ def test_small_elements_of_a_query(gpu, dtype, layout, hd):
     bound = 0.5 * score * np.abs(va - vb) + 14 * U * np.maximum(np.abs(va), np.abs(vb))
     err = np.abs(_attend(sc) - ref).reshape(sc.total, heads, hd)
     assert (err <= bound).all(), f"off by {err.max():.3g}, {(err / bound).max():.3g} of the bound"
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("scene", list(P.SCENES))
+def test_no_less_exact_than_f32_loops(gpu, dtype, scene):
+    """The RMS error over rows and heads is that of an f32 evaluation: a lost
+    part of the queries or weights is 5 times that and more (test_paged_bounds.py)."""
+    sc = P.SCENES[scene](dtype)
+    at = P.sample(sc, 150)
+    ref = P.exact(sc, at)
+    out = _attend(sc).reshape(sc.total, sc.heads, sc.hd)
+    err = P.rms(np.array([out[a] for a in at]) - ref)
+    assert err <= P.allowed(sc, at, ref), f"{err / P.allowed(sc, at, ref):.3g} of what is allowed"
