@@ -96,3 +96,35 @@ def allowed(sc, at, ref):
     more sums than any kernel here, and 2 U of the results for the parts (U / 2
     rms each at most) and the quotient."""
     return 2 * rms(serial_f32(sc, at) - ref) + 2 * U * rms(ref)
+
+
+def logprob_bounds(x, lp):
+    """Bounds of log probabilities and entropies of f64 rows.
+
+    A weight is off by the rounding of d = x - m (U |d|), its exponential
+    (exp2 to an ulp, the product's rounding, 0.05 U |d|) and that of its
+    stretch where it is joined (again).  Sums: a thread adds up to 32 terms, a wavefront its threads in 6 steps, a workgroup its 8
+    wavefronts, the join up to one stretch per thread of 256 (these vocabularies) and
+    8 steps: 55 roundings.  With E1 = sum p |d| and E2 = sum p d^2, log Z is off
+    by U (61 + 2.1 E1), sum d e / Z by U (61 E1 + 2.1 E2) and |sum d e / Z| = E1
+    times Z's; the logarithm and the differences add 4 U times their sizes."""
+    m = x.max(1, keepdims=True)
+    d = np.where(np.isneginf(x), -1e4, x - m)
+    p = np.exp(d)
+    p /= p.sum(1, keepdims=True)
+    e1, e2 = (p * -d).sum(1), (p * d * d).sum(1)
+    z = U * (61 + 2.1 * e1)
+    return z[:, None] + 4 * U * np.abs(lp), z + U * (61 * e1 + 2.1 * e2) + e1 * z + 4 * U * (e1 + np.log(1 / p.max(1)))
+
+
+def edge_rows(rows, vocab):
+    """(logits, ids): a row for each of the last 7 ids and of those beside the
+    ends of threads', wavefronts' and stretches' shares, at least `rows` of them;
+    that id and one other hold all of the weight."""
+    edges = {e for n in (1, 4, 8, 64, 512, 2048, 4096, 8192, 16384, 32768, 65536, 122880, vocab) for e in range(n - 7, n + 8)}
+    ids = np.array(sorted(i for i in edges if 0 <= i < vocab))
+    who = np.resize(ids, max(rows, len(ids)))
+    x = np.full((len(who), vocab), -40.0, np.float32)
+    x[np.arange(len(x)), (who + vocab // 2 + 1) % vocab] = 0.0
+    x[np.arange(len(x)), who] = 0.5
+    return x, who

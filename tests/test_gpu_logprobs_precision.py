@@ -2,7 +2,8 @@
 import numpy as np
 import pytest
 
-from paged_np import U
+from paged_np import U, bf16_bits, logprobs, widened
+from precision_np import edge_rows, logprob_bounds
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +34,40 @@ def test_exponentials_of_far_logits(gpu, vocab, other):
     assert (err <= bound).all(), f"{(err / U).max():.1f} U"
     assert (eent <= bound + 4 * U).all(), f"{(eent / U).max():.1f} U"
     assert np.array_equal(tlp[:, 0], lp) and (ids[:, 0] == 3).all() and (ids[:, 1] == at).all()
+
+
+def _check(x, tokens, top, dtype):
+    from yallma3_mini_inference_amd import ops
+    y = x.astype(np.float32) if dtype == "f32" else x.astype(np.float16) if dtype == "f16" else bf16_bits(x)
+    w = widened(y)
+    lp, ent, ids, tlp = ops.token_logprobs(y, tokens, top)
+    rlp, rent, rids, rtlp = logprobs(w, tokens, top)
+    assert np.array_equal(ids, rids)
+    both, rboth = np.concatenate([lp[:, None], tlp], 1), np.concatenate([rlp[:, None], rtlp], 1)
+    bl, be = logprob_bounds(w, rboth)
+    assert (np.abs(both - rboth) <= bl).all(), f"{(np.abs(both - rboth) / bl).max():.3g} of the bound"
+    assert (np.abs(ent - rent) <= be).all(), f"{(np.abs(ent - rent) / be).max():.3g} of the bound"
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [1, 2, 65, 257, 4097, 8192, 8193, 16384, 16385, 49152, 128256])
+@pytest.mark.parametrize("size", [0.5, 3.0, 9.0])
+def test_random_rows(gpu, dtype, vocab, size):
+    rng = np.random.default_rng(vocab)
+    x = (rng.standard_normal((4, vocab)) * size).astype(np.float32)
+    _check(x, rng.integers(0, vocab, 4), min(5, vocab), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("vocab", [7, 1000, 8191, 8195, 16384, 16387, 24583, 49157, 128256])
+def test_no_logit_is_left_out_or_counted_twice(gpu, dtype, rows, vocab):
+    """A row for each of the last 7 ids, and for the ids on both sides of the
+    places where a thread's, a wavefront's or a stretch's share ends: that id
+    and one other hold all of the weight, so a log Z without it (or with it
+    twice) is off by 0.3 or more.  Few rows and many: both stretch lengths."""
+    x, who = edge_rows(rows, vocab)
+    if rows == 1:
+        for r in range(0, len(x), 9):
+            _check(x[r:r + 1], who[r:r + 1], min(2, vocab), dtype)
+    _check(x, who, min(2, vocab), dtype)
