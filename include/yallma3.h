@@ -312,7 +312,10 @@ yl_status yl_paged_append(const yl_paged_cache *cache, const yl_paged_batch *bat
  * A prefix is read once for all sequences.  workspace (device,
  * 16-byte aligned): yl_paged_attention_workspace bytes, its contents of no
  * matter before and after; calls that may run at the same time need one each.
- * Smaller: YL_ERR_RANGE. */
+ * Smaller: YL_ERR_RANGE.  What the size function says for a batch also serves every
+ * one of the same pool and heads with no more n_seqs, n_rows, max_pages, max_len
+ * (0 being the most) and prefix_len, row_start given or not: a program takes it
+ * once, for the largest batch that it admits. */
 size_t yl_paged_attention_workspace(const yl_paged_cache *cache, const yl_paged_batch *batch, uint32_t n_heads);
 yl_status yl_paged_attention(float *out, size_t out_ld, const float *q, size_t q_ld, const yl_paged_cache *cache,
                              const yl_paged_batch *batch, uint32_t n_heads, float attn_scale, void *workspace,
@@ -327,7 +330,8 @@ yl_status yl_paged_attention(float *out, size_t out_ld, const float *q, size_t q
  * Logits of -inf have probability 0.  A row of nothing else: logprob and
  * top_logprobs -inf, entropy 0, ids from 0 on.  A row that holds NaN or +inf:
  * NaN in all of them, ids with NaN last.  workspace as above, of
- * yl_token_logprobs_workspace bytes. */
+ * yl_token_logprobs_workspace bytes, which serve every call with no more rows,
+ * vocabulary and top. */
 size_t yl_token_logprobs_workspace(size_t rows, size_t vocab, uint32_t top);
 yl_status yl_token_logprobs(const void *logits, int32_t dtype, size_t rows, size_t vocab, size_t ld,
                             const uint32_t *tokens, float *logprob, float *entropy, uint32_t top, uint32_t *top_ids,

@@ -413,16 +413,25 @@ struct ScorePlan {
 //  16384  10.7   11.1   11.4   11.7   14.7   30.5
 // (4096: 10.0, 10.6, 11.5, 14.6, 20.8, 51.6).  A row that one stretch of 16384
 // holds needs no second kernel.
+constexpr size_t kScoreEnough = 256;
 ScorePlan plan_score(size_t rows, size_t vocab, uint32_t top) {
     ScorePlan p;
     const auto segs = [&](int v) { return (vocab + (size_t)kScoreThreads * 8 * v - 1) / ((size_t)kScoreThreads * 8 * v); };
-    p.v = rows * segs(4) >= 256 || (segs(4) == 1 && segs(2) > 1) ? 4 : 2;
+    p.v = rows * segs(4) >= kScoreEnough || (segs(4) == 1 && segs(2) > 1) ? 4 : 2;
     p.segs = (int)segs(p.v);
     if (p.segs > 1) {
         p.part_bytes = rows * p.segs * sizeof(float4);
         p.bytes = p.part_bytes + rows * p.segs * top * sizeof(u64);
     }
     return p;
+}
+
+// What every call of no more rows, a vocabulary and a list no longer takes: fewer
+// rows may be cut into the shorter stretches, fewer than 256 * 2 in all.
+size_t score_bytes_at_most(size_t rows, size_t vocab, uint32_t top) {
+    const auto segs = [&](int v) { return (vocab + (size_t)kScoreThreads * 8 * v - 1) / ((size_t)kScoreThreads * 8 * v); };
+    if (segs(4) == 1) return 0;
+    return std::max(rows * segs(4), std::min<size_t>(rows * segs(2), 2 * (kScoreEnough - 1))) * (sizeof(float4) + top * sizeof(u64));
 }
 
 struct ScoreArgs {
@@ -465,7 +474,7 @@ extern "C" {
 
 size_t yl_token_logprobs_workspace(size_t rows, size_t vocab, uint32_t top) {
     if (!rows || rows >= (1ull << 31) || !vocab || vocab >= (1ull << 31) || top > (uint32_t)kTopMost) return 0;
-    return plan_score(rows, vocab, top).bytes;
+    return std::max(plan_score(rows, vocab, top).bytes, score_bytes_at_most(rows, vocab, top));
 }
 
 yl_status yl_token_logprobs(const void* logits, int32_t dtype, size_t rows, size_t vocab, size_t ld,
@@ -483,8 +492,9 @@ yl_status yl_token_logprobs(const void* logits, int32_t dtype, size_t rows, size
     if (top && (!top_ids || !top_logprobs)) return refuse("token_logprobs: top needs top_ids and top_logprobs");
     if (!logprob && !entropy && !top) return refuse("token_logprobs: nothing is asked for");
     const ScorePlan plan = plan_score(rows, vocab, top);
-    if (plan.bytes && (!workspace || (uintptr_t)workspace % 16)) return refuse("token_logprobs: the workspace has to be there, 16-byte aligned");
-    if (workspace_bytes < plan.bytes) return refuse("token_logprobs: the workspace is smaller than yl_token_logprobs_workspace says", YL_ERR_RANGE);
+    const size_t need = std::max(plan.bytes, score_bytes_at_most(rows, vocab, top));
+    if (need && (!workspace || (uintptr_t)workspace % 16)) return refuse("token_logprobs: the workspace has to be there, 16-byte aligned");
+    if (workspace_bytes < need) return refuse("token_logprobs: the workspace is smaller than yl_token_logprobs_workspace says", YL_ERR_RANGE);
     const ScoreArgs a{logits, rows, vocab, ld, tokens, logprob, entropy, (int)top, top_ids, top_logprobs, workspace};
     hipStream_t s = (hipStream_t)stream;
     const hipError_t e = dtype == YL_T_F32 ? launch_score<float>(a, plan, s) : dtype == YL_T_F16 ? launch_score<_Float16>(a, plan, s)

@@ -1090,7 +1090,7 @@ struct AttnPlan {
 // Own positions up to which a tile's are not split (one kernel less): of few
 // tiles, of many.  One decoded row, 32 heads on 8, f16, hd 64, unsplit | split, in
 // us: 300 positions 7.0 | 8.9, 600 8.3 | 8.9, 1000 10.3 | 9.2, 2000 15.5 | 9.0.
-constexpr int kUnsplit = 640, kUnsplitMany = 2048;
+constexpr int kUnsplit = 640, kUnsplitMany = 2048, kManyTiles = 512;
 constexpr int kEnough = 2048;        // tiles of all kv heads
 constexpr int kLeastChunk = 128;     // positions of a part at least
 // The tile kernel from as many workgroups of rows on (f16 and bf16 caches; f32's
@@ -1111,6 +1111,15 @@ constexpr int kTileKernelGroups = 160;
 //   bf16 hd 128         27.7 | 33.4    36.5 | 35.2    52.0 | 48.9    88.7 | 66.6
 constexpr int64_t kPrefixByTile = 8 << 20;
 
+// (units: where each sequence's begin)
+size_t bytes_of(const PagedArgs& p, size_t row_units, size_t all_units) {
+    const size_t bytes = (row_units + all_units) * (p.hd + 2) * sizeof(float);
+    return bytes ? ((bytes + 15) & ~(size_t)15) + (size_t)p.n_seqs * sizeof(int4) : 0;
+}
+
+// Workgroups of the tile kernel that run at once (their registers).
+int tile_resident(const PagedArgs& p) { return p.hd == 128 ? 256 : 512; }
+
 AttnPlan plan_attention(const PagedArgs& p, int dtype, uint32_t max_len) {
     AttnPlan r;
     const int group = p.n_heads / p.n_kv, R = kTileRows;
@@ -1124,14 +1133,13 @@ AttnPlan plan_attention(const PagedArgs& p, int dtype, uint32_t max_len) {
         l->chunk = ((positions + l->splits - 1) / l->splits + 63) & ~63;
         l->splits = std::max(1, (positions + l->chunk - 1) / std::max(l->chunk, 1));
     };
-    const int resident = p.hd == 128 ? 256 : 512;    // workgroups of the tile kernel that run at once (their registers)
     r.both = p.row_start && dtype != YL_T_F32 && (stacked + R - 1) / R * p.n_kv >= kTileKernelGroups;
     r.per = (group + kRowTile - 1) / kRowTile;
     // tiles of the row kernel at most: slots of tile_of_slot, or fewer where the
     // tile kernel has the large sequences and the units are counted through
     const int64_t slots = stacked / kRowTile + p.n_seqs;
     const bool many = p.n_seqs > kDivided;
-    r.split = !many && own > (p.row_start && !r.both && slots * p.n_kv >= 512 ? kUnsplitMany : kUnsplit);
+    r.split = !many && own > (p.row_start && !r.both && slots * p.n_kv >= kManyTiles ? kUnsplitMany : kUnsplit);
     const bool search = !r.split && (!r.both || many || slots <= 4 * (int64_t)p.n_seqs);
     const int64_t tiles = !p.row_start          ? (int64_t)p.n_seqs * r.per
                           : r.both && !search ? std::min<int64_t>((int64_t)p.n_seqs * (kRowKernelRows / kRowTile), slots)
@@ -1149,7 +1157,7 @@ AttnPlan plan_attention(const PagedArgs& p, int dtype, uint32_t max_len) {
     if (p.prefix_len) {
         r.prefix_by_tile = dtype != YL_T_F32 && stacked * p.n_kv * p.prefix_len >= kPrefixByTile;
         r.prefix.tiles = (int)((stacked + (r.prefix_by_tile ? R : kRowTile) - 1) / (r.prefix_by_tile ? R : kRowTile));
-        split(&r.prefix, r.prefix.tiles, p.prefix_len, r.prefix_by_tile ? resident : 512);
+        split(&r.prefix, r.prefix.tiles, p.prefix_len, r.prefix_by_tile ? tile_resident(p) : 512);
     } else {
         r.prefix.splits = 0;
     }
@@ -1160,9 +1168,48 @@ AttnPlan plan_attention(const PagedArgs& p, int dtype, uint32_t max_len) {
     r.all_units = (size_t)p.n_rows * p.n_heads * (r.tile_parts + r.prefix.splits);
     r.per_seq = r.both ? std::max(1, kRowKernelRows / group) : 0;
     if (r.all_units || (int64_t)p.n_seqs * r.per_seq >= p.n_rows) r.per_seq = 0;
-    r.bytes = (r.row_units + r.all_units) * (p.hd + 2) * sizeof(float);
-    if (r.wanted && r.join_rows) r.bytes = ((r.bytes + 15) & ~(size_t)15) + (size_t)p.n_seqs * sizeof(int4);
+    r.bytes = bytes_of(p, r.row_units, r.all_units);
     return r;
+}
+
+// What every call of no more sequences, rows, entries, positions and prefix
+// takes: the largest of plan_attention's over them, or a little more.
+size_t bytes_at_most(const PagedArgs& p, int dtype, uint32_t max_len) {
+    const int group = p.n_heads / p.n_kv, R = kTileRows;
+    const int64_t stacked = (int64_t)p.n_rows * group, entries = (int64_t)p.max_pages << p.page_shift;
+    const int64_t own = max_len && max_len < entries ? max_len : entries;
+    const bool tiled = dtype != YL_T_F32;
+    const auto tiles_of = [&](int64_t rows, int64_t seqs) { return rows / kRowTile + seqs; };
+    const auto finer = [](float f, int64_t tiles) { return (int64_t)std::ceil(f * (float)tiles) + 1; };
+    int64_t units = 0;
+    if (own > kUnsplit) {
+        const int64_t seqs = std::min(p.n_seqs, kDivided), wanted = std::max(1, 512 / p.n_kv);
+        // row_start: batches without the tile kernel have few stacked rows (of f32, all), and few
+        // tiles while contexts are short; of the others, the row kernel has sequences of few rows
+        int64_t tiles = tiles_of(tiled ? std::min<int64_t>(stacked, (int64_t)R * ((kTileKernelGroups - 1) / p.n_kv)) : stacked, seqs);
+        if (own <= kUnsplitMany) tiles = std::min<int64_t>(tiles, (kManyTiles - 1) / p.n_kv);
+        if (tiled) tiles = std::max(tiles, std::min(seqs * (kRowKernelRows / kRowTile), tiles_of(stacked, seqs)));
+        units = tiles + std::max(wanted, finer(0.95f, tiles));
+        // one row per sequence: twice the tiles' number again up to kEnough of all kv heads
+        const int64_t single = std::min<int64_t>(seqs, p.n_rows) * ((group + kRowTile - 1) / kRowTile);
+        const int64_t few = std::min<int64_t>(single, (kEnough - 1) / p.n_kv);
+        units = std::max({units, single + std::max(wanted, finer(1.0f, single)), few + finer(2.0f, few)});
+    }
+    size_t all = 0;
+    if (p.prefix_len) {
+        units = std::max(units, tiles_of(stacked, p.n_seqs) + 1);
+        // a part of the tile kernel, and the prefix's: more than one per row only where
+        // the tiles of 16 or 128 rows are fewer than the workgroups wanted
+        const int64_t heads = (int64_t)p.n_rows * p.n_heads, parts = (p.prefix_len + kLeastChunk - 1) / kLeastChunk;
+        const int64_t wanted = tiled && heads * p.prefix_len >= kPrefixByTile ? (int64_t)tile_resident(p) * R : 512 * kRowTile;
+        all = heads * (tiled && (stacked + R - 1) / R * p.n_kv >= kTileKernelGroups) + std::max(heads, std::min(heads * parts, wanted));
+    }
+    return bytes_of(p, (size_t)units * p.n_kv * kRowTile, all);
+}
+
+// The workspace that a call asks for.
+size_t workspace_of(const PagedArgs& p, int dtype, uint32_t max_len, const AttnPlan& plan) {
+    return std::max(plan.bytes, bytes_at_most(p, dtype, max_len));
 }
 
 template <typename C, int HD>
@@ -1235,7 +1282,7 @@ extern "C" {
 size_t yl_paged_attention_workspace(const yl_paged_cache* cache, const yl_paged_batch* batch, uint32_t n_heads) {
     PagedArgs p{};
     if (paged_args(cache, batch, n_heads, &p) != YL_OK || !p.n_rows || !p.n_seqs) return 0;
-    return plan_attention(p, cache->dtype, batch->max_len).bytes;
+    return workspace_of(p, cache->dtype, batch->max_len, plan_attention(p, cache->dtype, batch->max_len));
 }
 
 yl_status yl_paged_attention(float* out, size_t out_ld, const float* q, size_t q_ld, const yl_paged_cache* cache,
@@ -1250,8 +1297,9 @@ yl_status yl_paged_attention(float* out, size_t out_ld, const float* q, size_t q
     if (q_ld < att || out_ld < att) return refuse("paged_attention: rows further apart than they are long");
     if (q == out && q_ld != out_ld) return refuse("paged_attention: in place, q_ld and out_ld are the same");
     const AttnPlan plan = plan_attention(a.p, cache->dtype, batch->max_len);
-    if (plan.bytes && (!workspace || (uintptr_t)workspace % 16)) return refuse("paged_attention: the workspace has to be there, 16-byte aligned");
-    if (workspace_bytes < plan.bytes) return refuse("paged_attention: the workspace is smaller than yl_paged_attention_workspace says", YL_ERR_RANGE);
+    const size_t need = workspace_of(a.p, cache->dtype, batch->max_len, plan);
+    if (need && (!workspace || (uintptr_t)workspace % 16)) return refuse("paged_attention: the workspace has to be there, 16-byte aligned");
+    if (workspace_bytes < need) return refuse("paged_attention: the workspace is smaller than yl_paged_attention_workspace says", YL_ERR_RANGE);
     a.out = out; a.q = q; a.out_ld = out_ld; a.q_ld = q_ld;
     a.scale = frexpf(attn_scale * 1.4426950408889634f, &a.scale_exp);
     a.group = a.p.n_heads / a.p.n_kv;
