@@ -255,7 +255,14 @@ __device__ __forceinline__ int limit_of_row(const PagedAttn& a, const RowSet& se
 constexpr int kRowTile = 16, kRowTileLog2 = 4;
 
 // Stacked rows of a sequence (tokens times heads per kv head) up to which the
-// row kernel takes it where there is work for the tile kernel.
+// row kernel takes it where there is work for the tile kernel.  64 turns of so many
+// stacked rows beside a prompt of 1500 tokens, 32 heads on 8, in us, row kernel |
+// tile kernel:
+//   stacked rows               24             32             40             64
+//   f16 hd 64,  300 long   73.6 | 61.5    75.0 | 62.5    83.9 | 69.8    81.7 | 70.7
+//              2000 long    122 | 107      126 | 107      145 | 113      156 | 114
+//   bf16 hd 128, 300 long   116 | 116      117 | 117      134 | 131      146 | 125
+//              2000 long                   207 | 226      242 | 266      274 | 243
 constexpr int kRowKernelRows = 32;
 __device__ __forceinline__ bool row_kernel_takes(int rows, int group) { return (int64_t)rows * group <= kRowKernelRows; }
 
@@ -1081,7 +1088,8 @@ struct AttnPlan {
     float finer = 0.0f;
     bool split = false, join_rows = false, both = false;
     int per_seq = 0;                                 // joining only what the row kernel took: rows of a sequence
-    Launch tile, prefix;                             // tile kernel, own pages; the prefix
+    int tile_groups = 0;                             // tile kernel, own pages (not split): row tiles
+    Launch prefix;
     bool prefix_by_tile = false;
     int tile_parts = 0;
     size_t row_units = 0, all_units = 0, bytes = 0;
@@ -1090,9 +1098,23 @@ struct AttnPlan {
 // Own positions up to which a tile's are not split (one kernel less): of few
 // tiles, of many.  One decoded row, 32 heads on 8, f16, hd 64, unsplit | split, in
 // us: 300 positions 7.0 | 8.9, 600 8.3 | 8.9, 1000 10.3 | 9.2, 2000 15.5 | 9.0.
+// Many (kManyTiles tiles of all kv heads), f32 prompts of hd 64: 1000 tokens 57.4 |
+// 64.8, 1500 106 | 114, 3000 365 | 373; 8 turns of 60 tokens at 3000 positions, f16
+// hd 64 87.2 | 76.8, bf16 hd 128 118 | 122.  Near kManyTiles: f32 prompts of 130 tokens
+// (208 tiles) at 1000 positions 25.1 | 32.2, of 300 (608) 32.4 | 36.6, f16 24.3 for
+// the latter split, 20.2 whole.
 constexpr int kUnsplit = 640, kUnsplitMany = 2048, kManyTiles = 512;
-constexpr int kEnough = 2048;        // tiles of all kv heads
-constexpr int kLeastChunk = 128;     // positions of a part at least
+// Tiles of all kv heads, one row per sequence, from which on a tile is split above
+// the mean length, not above half of it.  Sequences of 100 .. 3000, bf16 hd 128, in us,
+// mean | half: 140 (1120 tiles) 108 | 111, 240 173 | 183, 300 218 | 235, 500 373 |
+// 412; of 100 .. 8000, f16 hd 64: 140 113 | 110, 240 171 | 172, 300 216 | 219, 500
+// 363 | 378.
+constexpr int kEnough = 2048;
+// Positions of a part at least.  One decoded row, f16 hd 64, in us, 64 | 128 | 256: 700
+// positions 10.3 | 10.3 | 11.0, 1000 10.3 | 10.6 | 11.3, 2000 11.6 | 10.3 | 11.0, 4000
+// 14.8 | 11.7 | 11.2; bf16 hd 128: 1000 12.0 | 12.6 | 13.7, 4000 18.2 | 15.0 | 15.2; four
+// rows under a prefix of 1500 15.3 | 14.0 | 15.0.
+constexpr int kLeastChunk = 128;
 // The tile kernel from as many workgroups of rows on (f16 and bf16 caches; f32's
 // matrix instructions take so long that K and V need not be shared).  One prompt
 // over itself, 32 heads on 8, in us, row kernel | tile kernel:
@@ -1136,7 +1158,10 @@ AttnPlan plan_attention(const PagedArgs& p, int dtype, uint32_t max_len) {
     r.both = p.row_start && dtype != YL_T_F32 && (stacked + R - 1) / R * p.n_kv >= kTileKernelGroups;
     r.per = (group + kRowTile - 1) / kRowTile;
     // tiles of the row kernel at most: slots of tile_of_slot, or fewer where the
-    // tile kernel has the large sequences and the units are counted through
+    // tile kernel has the large sequences and the units are counted through (where
+    // slots, most of them unused, are many: 8 prompts of 600 tokens beside 64 decoded rows at
+    // 500, 20 slots a sequence, f16 hd 64, in us, search | count 91.8 | 79.1, 6 beside 30
+    // 62.8 | 55.7; 2 beside 500, 2 slots a sequence, 165 | 191)
     const int64_t slots = stacked / kRowTile + p.n_seqs;
     const bool many = p.n_seqs > kDivided;
     r.split = !many && own > (p.row_start && !r.both && slots * p.n_kv >= kManyTiles ? kUnsplitMany : kUnsplit);
@@ -1153,7 +1178,7 @@ AttnPlan plan_attention(const PagedArgs& p, int dtype, uint32_t max_len) {
     r.finer = p.row_start ? 0.95f : tiles * p.n_kv >= kEnough ? 1.0f : 2.0f;
     r.max_units = (int)(tiles + std::max<int64_t>(r.wanted, r.split ? (int64_t)std::ceil(r.finer * (float)tiles) + 1 : 0));
     r.join_rows = r.split || p.prefix_len;
-    if (r.both) r.tile.tiles = (int)(stacked / R) + p.n_seqs;
+    if (r.both) r.tile_groups = (int)(stacked / R) + p.n_seqs;
     if (p.prefix_len) {
         r.prefix_by_tile = dtype != YL_T_F32 && stacked * p.n_kv * p.prefix_len >= kPrefixByTile;
         r.prefix.tiles = (int)((stacked + (r.prefix_by_tile ? R : kRowTile) - 1) / (r.prefix_by_tile ? R : kRowTile));
@@ -1248,8 +1273,8 @@ hipError_t launch_all(PagedAttn a, const AttnPlan& plan, float* space, hipStream
     a.parts = plan.tile_parts + plan.prefix.splits;
     if (e == hipSuccess && plan.both) {
         a.direct = !plan.tile_parts;
-        a.splits = plan.tile.splits; a.chunk = plan.tile.chunk;
-        e = launch_attn<C>(a, dim3((unsigned)plan.tile.tiles * a.p.n_kv, plan.tile.splits), true, false, s);
+        a.splits = 1;
+        e = launch_attn<C>(a, dim3((unsigned)plan.tile_groups * a.p.n_kv), true, false, s);
     }
     if (e == hipSuccess && a.p.prefix_len) {
         a.direct = 0;
