@@ -6,8 +6,9 @@
 //   H = log Z - sum (x - m) exp(x - m) / Z     (both terms are >= 0)
 // log Z is taken as log1p of Z - 1, summed without the maximum's own 1, so that
 // a sharp row keeps the small rest.  Bound by reading the logits once: 700 rows
-// of 128256 f32 62 us, 5.8 TB/s (one pass for the maximum, one for the sums and
-// one per top entry: 1740 us); one row 10 us, two launches and three round trips.
+// of 128256 f32 64 us, 5.6 TB/s (one pass for the maximum, one for the sums and
+// one per top entry: 1740 us); of bf16 64 us too, bound by the vector instructions;
+// one row 11 us, two launches and three round trips.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -409,9 +410,9 @@ struct ScorePlan {
 // Stretches of 16384 values where at least one per CU is left of these, else
 // of 8192 (more workgroups): rows of 128256, top 5, in us
 //   rows     1      8     16     32     64    256
-//   8192  10.1   10.3   10.6   11.8   15.8   33.9
-//  16384  10.7   11.1   11.4   11.7   14.7   30.5
-// (4096: 10.0, 10.6, 11.5, 14.6, 20.8, 51.6).  A row that one stretch of 16384
+//   8192  10.8   11.2   11.8   13.9   17.4   34.7
+//  16384  11.6   12.1   12.6   13.9   17.2   31.8
+// (4096: 10.5, 11.4, 12.8, 16.4, 22.1, 52.8).  A row that one stretch of 16384
 // holds needs no second kernel.
 constexpr size_t kScoreEnough = 256;
 ScorePlan plan_score(size_t rows, size_t vocab, uint32_t top) {

@@ -1100,9 +1100,9 @@ struct AttnPlan {
 // us: 300 positions 7.0 | 8.9, 600 8.3 | 8.9, 1000 10.3 | 9.2, 2000 15.5 | 9.0.
 // Many (kManyTiles tiles of all kv heads), f32 prompts of hd 64: 1000 tokens 57.4 |
 // 64.8, 1500 106 | 114, 3000 365 | 373; 8 turns of 60 tokens at 3000 positions, f16
-// hd 64 87.2 | 76.8, bf16 hd 128 118 | 122.  Near kManyTiles: f32 prompts of 130 tokens
-// (208 tiles) at 1000 positions 25.1 | 32.2, of 300 (608) 32.4 | 36.6, f16 24.3 for
-// the latter split, 20.2 whole.
+// hd 64 87.2 | 76.8, bf16 hd 128 118 | 122.  Near kManyTiles: prompts of 130
+// tokens (264 tiles) at 1000 positions, f32, 25.1 | 32.2, of 300 (608) 32.4 | 36.6, f16
+// 20.2 | 24.3.
 constexpr int kUnsplit = 640, kUnsplitMany = 2048, kManyTiles = 512;
 // Tiles of all kv heads, one row per sequence, from which on a tile is split above
 // the mean length, not above half of it.  Sequences of 100 .. 3000, bf16 hd 128, in us,
