@@ -224,7 +224,8 @@ yl_status yl_swiglu_quantize(const float *gate, const float *up, size_t hidden, 
  * No counterparts in the reference, which holds one conversation: ops for
  * programs that serve many conversations from one pool of cache pages.
  * Activations are f32 as in the ops above; results differ from a serial f32
- * evaluation in rounding only (f32 sums in another order).  Everything is
+ * evaluation in rounding only (f32 sums in another order, and what f16 caches
+ * round as yl_paged_attention says).  Everything is
  * enqueued on `stream` and not waited for, nothing is allocated and the host
  * reads no device memory, so calls can be captured into a graph; lengths and
  * page tables are read when the work runs, so a replay sees their new values. */

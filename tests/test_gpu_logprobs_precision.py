@@ -71,3 +71,25 @@ def test_no_logit_is_left_out_or_counted_twice(gpu, dtype, rows, vocab):
         for r in range(0, len(x), 9):
             _check(x[r:r + 1], who[r:r + 1], min(2, vocab), dtype)
     _check(x, who, min(2, vocab), dtype)
+
+
+@pytest.mark.parametrize("vocab", [50, 16390])
+def test_more_rows_than_a_grid_has(gpu, vocab):
+    """Beyond 65535 rows a call is several launches: rows of one stretch and of two."""
+    from yallma3_mini_inference_amd import ops
+    rows, kinds = 65535 + 70, 7
+    rng = np.random.default_rng(vocab)
+    x = bf16_bits((rng.standard_normal((kinds, vocab)) * 3).astype(np.float32))
+    tokens = rng.integers(0, vocab, rows)
+    kind = np.arange(rows) % kinds
+    lp, ent, ids, tlp = ops.token_logprobs(x[kind], tokens, 3)
+    w = widened(x)
+    _, rent, rids, rtlp = logprobs(w, None, 3)
+    logp = w - w.max(1, keepdims=True)
+    logp -= np.log(np.exp(logp).sum(1, keepdims=True))
+    rlp = logp[kind, tokens]
+    bl, be = logprob_bounds(w, rtlp)
+    z = (bl - 4 * U * np.abs(rtlp))[:, 0]          # log Z's part of the bound
+    assert (np.abs(lp - rlp) <= z[kind] + 4 * U * np.abs(rlp)).all()
+    assert (np.abs(ent - rent[kind]) <= be[kind]).all()
+    assert np.array_equal(ids, rids[kind]) and (np.abs(tlp - rtlp[kind]) <= bl[kind]).all()

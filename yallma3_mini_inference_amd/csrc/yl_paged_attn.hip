@@ -387,7 +387,8 @@ struct Tile {
         for (int j = 0; j < NJ; j++) acc[j] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
         ones = vf4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // The sum of row c's weights, in every lane of the row.
+    // The sum of row c's weights, in every lane of the row (!TR: before they are
+    // cut, which is within their parts' own rounding).
     __device__ __forceinline__ float sum() const { return TR ? ones[0] : group_sum16(l); }
     // What the rows attend to, and the longest and the shortest of them
     // (spare rows follow the longest, so that they need no masks).
