@@ -304,15 +304,15 @@ yl_status yl_paged_append(const yl_paged_cache *cache, const yl_paged_batch *bat
  * gets zeros.  Whatever lies at positions a row does not attend to takes no
  * part.  An infinity or NaN in a row's own q, or in a key it attends to, leaves
  * that row and head without defined values (in a value it attends to, that one
- * component); no other row or head feels it.  q, out: [n_rows] rows of n_heads * head_size floats (device), q_ld
- * and out_ld floats apart; out may be q (with q_ld) but not overlap it
- * otherwise.  Sums are f32, products those of f32 but over f16 caches: there an
- * element of q has 22 bits (below 2^-15 of its head's largest: right to 2^-38 of
- * that) and so has the largest weight e_j of 32 or 64 positions taken together
- * (the others: right to 2^-23 of that at least).
- * A prefix is read once for all sequences.  workspace (device,
- * 16-byte aligned): yl_paged_attention_workspace bytes, its contents of no
- * matter before and after; calls that may run at the same time need one each.
+ * component); no other row or head feels it.  Sums are f32, products those of
+ * f32 but over f16 caches: there an element of q has 22 bits (below 2^-15 of its
+ * head's largest: right to 2^-38 of that) and so has the largest weight e_j of
+ * 32 or 64 positions taken together (the others: right to 2^-23 of that at least).
+ * q, out: [n_rows] rows of n_heads * head_size floats (device), q_ld and out_ld
+ * floats apart; out may be q (with q_ld) but not overlap it otherwise.  A prefix
+ * is read once for all sequences.  workspace (device, 16-byte aligned):
+ * yl_paged_attention_workspace bytes, its contents of no matter before and
+ * after; calls that may run at the same time need one each.
  * Smaller: YL_ERR_RANGE.  What the size function says for a batch also serves every
  * one of the same pool and heads with no more n_seqs, n_rows, max_pages, max_len
  * (0 being the most) and prefix_len, row_start given or not: a program takes it

@@ -134,3 +134,22 @@ def test_no_less_exact_than_f32_loops(gpu, dtype, scene):
     out = _attend(sc).reshape(sc.total, sc.heads, sc.hd)
     err = P.rms(np.array([out[a] for a in at]) - ref)
     assert err <= P.allowed(sc, at, ref), f"{err / P.allowed(sc, at, ref):.3g} of what is allowed"
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("layout", [ROWS, (40, 8, 2), TILE])
+@pytest.mark.parametrize("size", [2.0, 5.0, 12.0])
+def test_scores_far_apart(gpu, dtype, layout, size):
+    """Scores of a deviation of 2 to 12: what the weights are taken against rises
+    and falls from step to step; the RMS error stays that of an f32 evaluation."""
+    rows, heads, kvh = layout
+    sc = Scene([rows, 1], [640, 900], heads, kvh, 64, 16, dtype, seed=int(size))
+    sc.q *= np.float32(size)
+    for at in (5, 130, 131, 400):            # and single positions far above the others
+        page, slot = sc.places(0, 600)[at]
+        sc.k32[page, :, slot] *= 2.5
+    at = P.sample(sc, 150)
+    ref = P.exact(sc, at)
+    out = _attend(sc).reshape(sc.total, sc.heads, sc.hd)
+    err = P.rms(np.array([out[a] for a in at]) - ref)
+    assert err <= P.allowed(sc, at, ref), f"{err / P.allowed(sc, at, ref):.3g} of what is allowed"

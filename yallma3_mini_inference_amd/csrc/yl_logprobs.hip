@@ -56,10 +56,10 @@ __device__ __forceinline__ u64 wave_max64(u64 k) {
     return k;
 }
 
-// e^d for d <= 0 (NaN of NaN, 0 from -200 on: *d is raised to it).  exp2 is right to an
-// ulp, but its argument, d log2(e), is rounded, which at d = -30 would be 20 ulp
-// of the result: e^d = 2^t e^(d - t log(2)), whose second factor is 1 + (d - t
-// log(2)) to 2^-40.
+// e^d for d <= 0 (NaN of NaN, 0 from -200 on: *d is raised to it).  exp2 is right
+// to an ulp, but its argument, d log2(e), is rounded, which at d = -30 would be 11
+// ulp of the result: e^d = 2^t e^(d - t log(2)), whose second factor is
+// 1 + (d - t log(2)) to 2^-39.
 __device__ __forceinline__ float exp_below(float* d) {
     *d = __builtin_elementwise_maximum(*d, -200.0f);       // (keeps NaN)
     const float t = *d * 1.4426950408889634f, p = __builtin_amdgcn_exp2f(t);

@@ -29,9 +29,10 @@
 // the weight of a score is 2^(score - reference).  The reference is the largest
 // score less the type's bias when it is set, and is only raised when a weight
 // would pass 2^kMost, so that most steps need no exchange between lanes and no
-// rescaling.  Over f16 caches it also falls, by up to some 40 powers of two, where all of a step's
-// weights would be below 2^kLeast: f16 parts end at 2^-24, and beside one position
-// that has nearly all of the weight the others would lose their bits.  Scores come out of the products times a power of two (the scale's
+// rescaling.  Over f16 caches it also falls, by up to some 40 powers of two, where
+// all of a step's weights would be below 2^kLeast: f16 parts end at 2^-24, and
+// beside one position that has nearly all of the weight the others would lose
+// their bits.  Scores come out of the products times a power of two (the scale's
 // mantissa is multiplied into q), so that one fma subtracts the reference from
 // the score itself: a product rounded on its way would be off by many powers of
 // two where scores are large.
