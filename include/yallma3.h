@@ -230,12 +230,18 @@ yl_status yl_swiglu_quantize(const float *gate, const float *up, size_t hidden, 
  * reads no device memory, so calls can be captured into a graph; lengths and
  * page tables are read when the work runs, so a replay sees their new values. */
 
-typedef enum { YL_T_F32 = 0, YL_T_F16 = 1, YL_T_BF16 = 2 } yl_dtype;
+typedef enum { YL_T_F32 = 0, YL_T_F16 = 1, YL_T_BF16 = 2, YL_T_MXFP4 = 4 } yl_dtype;
 
 /* One layer's pool of pages (device): keys and values, each
  * [n_pages][n_kv_heads][page_size][head_size] of `dtype`, 16-byte aligned.
  * head_size 32, 64 or 128; page_size 16, 32, 64, 128 or 256 positions;
- * n_pages * page_size below 2^31. */
+ * n_pages * page_size below 2^31.
+ * YL_T_MXFP4 (pages only): a page's kv head is page_size rows of head_size / 2
+ * bytes of codes, then page_size rows of head_size / 32 scale bytes: 17/32 byte
+ * an element.  Element 2i is the low half of byte i, 2i + 1 the high half:
+ * sign, two bits of exponent, one of mantissa (0, 1/2, 1, 3/2, 2, 3, 4, 6).
+ * A scale byte E, of 32 neighbouring elements, stands for 2^(E - 127); 255
+ * makes them NaN.  Bytes 2 .. 252 keep every value exact in the products. */
 typedef struct {
     void *keys, *values;
     int32_t dtype;               /* yl_dtype */
@@ -291,11 +297,23 @@ yl_status yl_rope_table(const yl_rope_params *p, int32_t pairs, uint32_t rows, f
  * as it is.  A row at a negative position, or at one not below rope_rows
  * while there is a rotation, is passed over; one below prefix_len writes q_out
  * only (prefix pages are shared).  No two rows of a call may hold the same
- * slot of a page. */
+ * slot of a page.
+ * MXFP4 pages: of each 32 elements, E = exponent of the largest (biased, of f32;
+ * one more from a mantissa of 1.75 on) less 2, at least 2 and at most 252; each
+ * element becomes the nearest code, ties to even codes, beyond 6 units 6.  An
+ * infinity or NaN makes E 255. */
 yl_status yl_paged_append(const yl_paged_cache *cache, const yl_paged_batch *batch, uint32_t n_heads, float *q_out,
                           size_t q_out_ld, const float *q, size_t q_ld, const float *k, size_t k_ld, const float *v,
                           size_t v_ld, int32_t pairs, const float *cos_t, const float *sin_t, uint32_t rope_rows,
                           void *stream);
+
+/* The keys and values of the rows' positions back out of their pages, as f32:
+ * row r of k and v (device, [n_rows] rows of n_kv_heads * head_size floats,
+ * k_ld and v_ld floats apart; either may be NULL) is the position that the
+ * batch gives row r, on the prefix's pages too.  Rows of positions that
+ * nothing holds are left as they were. */
+yl_status yl_paged_gather(const yl_paged_cache *cache, const yl_paged_batch *batch, float *k, size_t k_ld, float *v,
+                          size_t v_ld, void *stream);
 
 /* Causal attention over the pages: a row of position p attends to positions
  * 0 .. p that its sequence or the prefix holds, query head h to kv head

@@ -32,12 +32,12 @@ EXPORTS = [
     "yl_infer_reset", "yl_tokenizer_load", "yl_tokenizer_free", "yl_model_tokenizer", "yl_tokenizer_vocab_size",
     "yl_tokenize", "yl_detokenize", "yl_chat_template", "yl_chat_prompt", "yl_pretokenize", "yl_sampler_new",
     "yl_sampler_sample", "yl_sampler_free", "yl_generate_text", "yl_weight_upload_f16", "yl_matmul_f32",
-    "yl_rope_table", "yl_paged_append", "yl_paged_attention_workspace", "yl_paged_attention",
+    "yl_rope_table", "yl_paged_append", "yl_paged_gather", "yl_paged_attention_workspace", "yl_paged_attention",
     "yl_token_logprobs_workspace", "yl_token_logprobs",
 ]
 
 # yl_dtype, and which elements of a head a rotation turns together (YL_ROPE_*)
-DTYPES = {"f32": 0, "f16": 1, "bf16": 2}
+DTYPES = {"f32": 0, "f16": 1, "bf16": 2, "mxfp4": 4}
 ROPE_PAIRS = {"none": -1, "adjacent": 0, "half": 1}
 
 
@@ -183,6 +183,7 @@ def lib():
         "yl_rope_table": (st, [C.POINTER(RopeParams), st, u32, vp, vp]),
         "yl_paged_append": (st, [C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), u32, vp, sz, vp, sz, vp, sz, vp, sz,
                                  st, vp, vp, u32, vp]),
+        "yl_paged_gather": (st, [C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), vp, sz, vp, sz, vp]),
         "yl_paged_attention_workspace": (sz, [C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), u32]),
         "yl_paged_attention": (st, [vp, sz, vp, sz, C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), u32, f32, vp,
                                     sz, vp]),

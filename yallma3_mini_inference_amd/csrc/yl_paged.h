@@ -19,7 +19,7 @@
 namespace yl {
 
 struct PagedArgs {
-    void* keys; void* values;        // [n_pages][n_kv][page][hd]
+    void* keys; void* values;        // [n_pages][n_kv][page][hd]; MXFP4: [n_pages][n_kv][paged_mx_block]
     int n_pages, page_shift, n_kv, hd;
     int n_seqs, n_rows, max_pages;
     const int32_t* table;            // [n_seqs][max_pages]
@@ -71,6 +71,17 @@ YL_HD int paged_page(int32_t entry, int n_pages) { return (uint32_t)entry < (uin
 // Element offset of (page, kv head, slot): 64 bits, a pool may hold more than 2^31 elements.
 YL_HD size_t paged_offset(const PagedArgs& a, int page, int kvh, int slot) {
     return (((((size_t)page * a.n_kv + kvh) << a.page_shift) + slot)) * (size_t)a.hd;
+}
+
+// MXFP4 pages: of each (page, kv head), page_size rows of hd / 2 bytes of codes,
+// then page_size rows of hd / 32 scale bytes.  Bytes of one, and the byte
+// offsets of a slot's codes and scales.
+YL_HD size_t paged_mx_block(const PagedArgs& a) { return (size_t)(a.hd / 32 * 17) << a.page_shift; }
+YL_HD size_t paged_mx_codes(const PagedArgs& a, int page, int kvh, int slot) {
+    return ((size_t)page * a.n_kv + kvh) * paged_mx_block(a) + (size_t)slot * (a.hd / 2);
+}
+YL_HD size_t paged_mx_scales(const PagedArgs& a, int page, int kvh, int slot) {
+    return ((size_t)page * a.n_kv + kvh) * paged_mx_block(a) + ((size_t)(a.hd / 2) << a.page_shift) + (size_t)slot * (a.hd / 32);
 }
 
 // The page and slot of position pos (0 <= pos < capacity) of sequence s; false where nothing is held.

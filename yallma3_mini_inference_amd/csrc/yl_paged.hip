@@ -5,9 +5,12 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "../../include/yallma3.h"
 #include "yl_device.h"
 #include "yl_internal.h"
+#include "yl_mx.h"
 #include "yl_paged.h"
 
 namespace yl {
@@ -31,6 +34,24 @@ template <typename C>
 __device__ __forceinline__ void store4(C* o, const f4u& x) {
     typedef C c4 __attribute__((ext_vector_type(4)));
     *reinterpret_cast<c4*>(o) = __builtin_convertvector((vf4{x[0], x[1], x[2], x[3]}), c4);
+}
+
+template <typename C> constexpr bool kMx = std::is_same<C, Mx4>::value;
+
+__device__ __forceinline__ uint32_t amax4(const f4u& x) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) m = max(m, __float_as_uint(x[k]) & 0x7fffffffu);
+    return m;
+}
+
+// Four neighbouring elements from `e` on of a slot's head in MXFP4, whose block's largest has the bits `amax`.
+__device__ __forceinline__ void store_mx(const PagedArgs& p, void* pool, int page, int head, int slot, int e, const f4u& x, uint32_t amax) {
+    const uint32_t scale = mx_scale(amax);
+    char* base = static_cast<char*>(pool);
+    const uint32_t codes = mx_codes(x[0], x[1], x[2], x[3], mx_unit(scale));
+    *reinterpret_cast<uint16_t*>(base + paged_mx_codes(p, page, head, slot) + e / 2) = (uint16_t)codes;
+    if (e % 32 == 0) base[paged_mx_scales(p, page, head, slot) + e / 32] = (char)scale;
 }
 
 // The sequence of a row by a whole wavefront, 64 starts per step (as paged_seq_of_row).
@@ -77,7 +98,7 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
     const int nq = a.q ? a.p.n_heads * hd : 0, nk = keep ? a.p.n_kv * hd : 0;
     if constexpr (PAIRS == YL_ROPE_HALF) {
         const int uq = nq / 8, uk = nk / 8;               // units of 4 pairs
-#pragma unroll 2
+#pragma unroll kMx<C> ? 1 : 2
         for (int i = tid; i < uq + uk; i += 256) {
             const bool is_q = i < uq;
             const int j = is_q ? i : i - uq, head = j >> (shift - 3), e = 4 * (j & (hd / 8 - 1));
@@ -93,6 +114,13 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
             if (is_q) {
                 *reinterpret_cast<f4u*>(qo + (size_t)head * hd + e) = r0;
                 *reinterpret_cast<f4u*>(qo + (size_t)head * hd + e + half) = r1;
+            } else if constexpr (kMx<C>) {
+                // (a head's lanes stand together: half / 4 of them, 8 to a block of one half, at hd 32 all 4 of both)
+                const uint32_t m0 = amax4(r0), m1 = amax4(r1);
+                const uint32_t b0 = hd == 32 ? mx_group_max<4>(max(m0, m1)) : mx_group_max<8>(m0);
+                const uint32_t b1 = hd == 32 ? b0 : mx_group_max<8>(m1);
+                store_mx(a.p, a.p.keys, page, head, slot, e, r0, b0);
+                store_mx(a.p, a.p.keys, page, head, slot, e + half, r1, b1);
             } else {
                 C* o = static_cast<C*>(a.p.keys) + at(head, e);
                 store4(o, r0);
@@ -101,7 +129,7 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
         }
     } else {
         const int uq = nq / 4, uk = nk / 4;
-#pragma unroll 4
+#pragma unroll kMx<C> ? 1 : 4
         for (int i = tid; i < uq + uk; i += 256) {
             const bool is_q = i < uq;
             const int j = is_q ? i : i - uq, head = j >> (shift - 2), e = 4 * (j & (hd / 4 - 1));
@@ -117,12 +145,65 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
                 x = r;
             }
             if (is_q) *reinterpret_cast<f4u*>(qo + 4 * (size_t)j) = x;
+            else if constexpr (kMx<C>) store_mx(a.p, a.p.keys, page, head, slot, e, x, mx_group_max<8>(amax4(x)));
             else store4(static_cast<C*>(a.p.keys) + at(head, e), x);
         }
     }
+#pragma unroll kMx<C> ? 1 : 2
+    for (int j = tid; j < nk / 4; j += 256) {
+        const f4u x = *reinterpret_cast<const f4u*>(vr + 4 * (size_t)j);
+        const int head = j >> (shift - 2), e = 4 * (j & (hd / 4 - 1));
+        if constexpr (kMx<C>) store_mx(a.p, a.p.values, page, head, slot, e, x, mx_group_max<8>(amax4(x)));
+        else store4(static_cast<C*>(a.p.values) + at(head, e), x);
+    }
+}
+
+// ----------------------------------------------------------------- gathering
+
+struct GatherArgs {
+    PagedArgs p;
+    float* k; float* v;
+    size_t k_ld, v_ld;
+};
+
+// Four neighbouring elements of a slot's head, widened.
+template <typename C>
+__device__ __forceinline__ f4u load4(const PagedArgs& p, const void* pool, int page, int head, int slot, int e) {
+    if constexpr (kMx<C>) {
+        const char* base = static_cast<const char*>(pool);
+        const uint32_t codes = *reinterpret_cast<const uint16_t*>(base + paged_mx_codes(p, page, head, slot) + e / 2);
+        const float unit = mx_unit((uint8_t)base[paged_mx_scales(p, page, head, slot) + e / 32]);
+        const uint32_t lo = mx_pair<0>(codes, unit), hi = mx_pair<1>(codes, unit);
+        return f4u{__uint_as_float(lo << 16), __uint_as_float(lo & 0xffff0000u), __uint_as_float(hi << 16), __uint_as_float(hi & 0xffff0000u)};
+    } else {
+        typedef C c4 __attribute__((ext_vector_type(4)));
+        const c4 x = *reinterpret_cast<const c4*>(static_cast<const C*>(pool) + paged_offset(p, page, head, slot) + e);
+        return f4u{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
+    }
+}
+
+// One workgroup per row, as k_paged_append; bound by memory.
+template <typename C>
+__global__ __launch_bounds__(256) void k_paged_gather(GatherArgs a) {
+    const int row = blockIdx.x, hd = a.p.hd, tid = threadIdx.x;
+    const int s = seq_of_row(a.p, row);
+    if (s < 0) return;
+    int first, end;
+    paged_rows(a.p, s, &first, &end);
+    if (row < first || row >= end) return;
+    const int64_t pos = paged_row_pos(a.p.kv_len[s], end, row);
+    int page = -1, slot = 0;
+    if (pos < 0 || !paged_place(a.p, s, pos, &page, &slot)) return;
+    const int shift = 31 - __builtin_clz(hd), n = a.p.n_kv * hd / 4;
 #pragma unroll 2
-    for (int j = tid; j < nk / 4; j += 256)
-        store4(static_cast<C*>(a.p.values) + at(j >> (shift - 2), 4 * (j & (hd / 4 - 1))), *reinterpret_cast<const f4u*>(vr + 4 * (size_t)j));
+    for (int i = tid; i < 2 * n; i += 256) {
+        const bool key = i < n;
+        const int j = key ? i : i - n;
+        float* out = key ? a.k : a.v;
+        if (!out) continue;
+        const f4u x = load4<C>(a.p, key ? a.p.keys : a.p.values, page, j >> (shift - 2), slot, 4 * (j & (hd / 4 - 1)));
+        *reinterpret_cast<f4u*>(out + (size_t)row * (key ? a.k_ld : a.v_ld) + 4 * (size_t)j) = x;
+    }
 }
 
 // ------------------------------------------------------------- host entries
@@ -138,8 +219,8 @@ yl_status refuse(const char* what, yl_status st = YL_ERR_ARG) {
 
 yl_status paged_args(const yl_paged_cache* c, const yl_paged_batch* b, uint32_t n_heads, PagedArgs* a) {
     if (!c || !b) return refuse("paged: no cache or no batch");
-    if (c->dtype != YL_T_F32 && c->dtype != YL_T_F16 && c->dtype != YL_T_BF16)
-        return refuse("paged: the cache's type is f32, f16 or bf16", YL_ERR_FORMAT);
+    if (c->dtype != YL_T_F32 && c->dtype != YL_T_F16 && c->dtype != YL_T_BF16 && c->dtype != YL_T_MXFP4)
+        return refuse("paged: the cache's type is f32, f16, bf16 or MXFP4", YL_ERR_FORMAT);
     if (c->head_size != 32 && c->head_size != 64 && c->head_size != 128) return refuse("paged: head size 32, 64 or 128");
     if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128 && c->page_size != 256)
         return refuse("paged: page size 16, 32, 64, 128 or 256");
@@ -205,8 +286,26 @@ yl_status yl_paged_append(const yl_paged_cache* cache, const yl_paged_batch* bat
     const hipStream_t strm = (hipStream_t)stream;
     if (cache->dtype == YL_T_F32) launch_append<float>(a, strm);
     else if (cache->dtype == YL_T_F16) launch_append<_Float16>(a, strm);
-    else launch_append<__bf16>(a, strm);
+    else if (cache->dtype == YL_T_BF16) launch_append<__bf16>(a, strm);
+    else launch_append<Mx4>(a, strm);
     return launched("paged_append launch");
+}
+
+yl_status yl_paged_gather(const yl_paged_cache* cache, const yl_paged_batch* batch, float* k, size_t k_ld, float* v, size_t v_ld,
+                          void* stream) {
+    GatherArgs a{};
+    const yl_status st = paged_args(cache, batch, cache ? cache->n_kv_heads : 0, &a.p);
+    if (st != YL_OK) return st;
+    if (!k && !v) return refuse("paged_gather: k or v, or both");
+    const size_t kv = (size_t)cache->n_kv_heads * cache->head_size;
+    if ((k && k_ld < kv) || (v && v_ld < kv)) return refuse("paged_gather: rows further apart than they are long");
+    if (!batch->n_rows || !batch->n_seqs) return YL_OK;
+    a.k = k; a.v = v; a.k_ld = k_ld; a.v_ld = v_ld;
+    const hipStream_t strm = (hipStream_t)stream;
+    auto kernel = cache->dtype == YL_T_F32 ? k_paged_gather<float> : cache->dtype == YL_T_F16 ? k_paged_gather<_Float16>
+                  : cache->dtype == YL_T_BF16 ? k_paged_gather<__bf16> : k_paged_gather<Mx4>;
+    hipLaunchKernelGGL(kernel, dim3(a.p.n_rows), dim3(256), 0, strm, a);
+    return launched("paged_gather launch");
 }
 
 }  // extern "C"

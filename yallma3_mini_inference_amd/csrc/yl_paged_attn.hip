@@ -42,10 +42,12 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "../../include/yallma3.h"
 #include "yl_device.h"
 #include "yl_internal.h"
+#include "yl_mx.h"
 #include "yl_paged.h"
 
 namespace yl {
@@ -118,6 +120,10 @@ template <> struct Type<__bf16> {
         return ((two & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((two & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
     }
 };
+// MXFP4 values are bf16 values: a block's codes become them on their way into the
+// products, two by an instruction.
+template <> struct Type<Mx4> : Type<__bf16> {};
+template <typename C> constexpr bool kMx = std::is_same<C, Mx4>::value;
 template <> struct Type<float> {
     static constexpr int kParts = 1, kTiles = 1;
     static constexpr bool kFalls = false;
@@ -366,6 +372,10 @@ struct Tile {
     static constexpr int NK = F32 ? HD / 16 : HD / 32;       // 16-byte pieces of a key per lane
     static constexpr int KD = F32 ? 16 : 32, KE = F32 ? 4 : 8;   // dimensions per piece of all lane groups, of one
     static constexpr int VW = NJ * (int)sizeof(C) / 4;       // words of a V row per lane
+    // where a lane group's dimensions of a key begin, and how far its pieces are
+    // apart: MXFP4 rows are so short that each takes neighbouring pieces
+    static constexpr bool MX = kMx<C>;
+    static constexpr int KG = MX && !TR ? HD / 4 : KE, KP = MX && !TR ? 8 : KD;
     static_assert(!(TR && F32), "halfwords are transposed");
     typedef Words<VW> Value;
     static __device__ __forceinline__ int dim(int i, int j, int g) { return TR ? 16 * j + 4 * g + i : (4 * g + i) * NJ + j; }
@@ -401,14 +411,14 @@ struct Tile {
     }
     // q of the lane's row, cut into parts, in the order of the keys' pieces
     __device__ __forceinline__ void load_q(const PagedAttn& a, int g) {
-        const float* qr = a.q + (size_t)row * a.q_ld + (size_t)head * HD + KE * g;
+        const float* qr = a.q + (size_t)row * a.q_ld + (size_t)head * HD + KG * g;
         f4u v[NK][KE / 4];
         float amax = 0.0f;
 #pragma unroll
         for (int k = 0; k < NK; k++)
 #pragma unroll
             for (int e = 0; e < KE / 4; e++) {
-                v[k][e] = *reinterpret_cast<const f4u*>(qr + k * KD + 4 * e);
+                v[k][e] = *reinterpret_cast<const f4u*>(qr + k * KP + 4 * e);
                 if (!live) v[k][e] = f4u{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int i = 0; i < 4; i++) amax = fmaxf(amax, fabsf(v[k][e][i]));
@@ -569,6 +579,14 @@ struct Tile {
             for (int tt = 1; tt < NT; tt++)
                 if (t == tt) pg = page[tt];
             if (pg < 0 || p0 + pos >= min(lim, hi)) continue;
+            if constexpr (MX) {                          // only whole blocks are no numbers
+                const uint8_t* e = static_cast<const uint8_t*>(a.p.values) + paged_mx_scales(a.p, pg, kvh, (p0 + pos) & slots);
+#pragma unroll
+                for (int ii = 0; ii < 4; ii++)
+#pragma unroll
+                    for (int j = 0; j < NJ; j++)
+                        if (e[dim(ii, j, g) / 32] == 255) acc[j][ii] = __uint_as_float(0x7fc00000u);
+            } else {
             const C* v = static_cast<const C*>(a.p.values) + paged_offset(a.p, pg, kvh, (p0 + pos) & slots);
 #pragma unroll
             for (int ii = 0; ii < 4; ii++)
@@ -577,6 +595,48 @@ struct Tile {
                     const float x = (float)v[dim(ii, j, g)];
                     if (!(fabsf(x) < INFINITY)) acc[j][ii] = fmaf(w, x, acc[j][ii]);
                 }
+            }
+        }
+    }
+};
+
+// A lane's part of 16 keys: its pieces, or of an MXFP4 row HD / 4 codes and their scale byte.
+template <int NK> struct KeyPieces { u4 f[NK]; };
+template <int HD> struct KeyCodes {
+    Words<HD / 32> codes;
+    uint32_t scale;
+    __device__ __forceinline__ void widen(u4 k[HD / 32]) const {
+        const float unit = mx_unit(scale);
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++)
+            k[i] = u4{mx_pair<0>(codes.w[i], unit), mx_pair<1>(codes.w[i], unit), mx_pair<2>(codes.w[i], unit), mx_pair<3>(codes.w[i], unit)};
+    }
+};
+template <typename C, int HD> struct KeyOf { typedef KeyPieces<HD * sizeof(C) / 64> type; };
+template <int HD> struct KeyOf<Mx4, HD> { typedef KeyCodes<HD> type; };
+
+// A lane's part of four neighbouring positions' values in MXFP4: HD / 16 codes of
+// each, and the scale bytes of all.
+template <int HD> struct MxValues {
+    typedef typename std::conditional<HD == 128, uint32_t, typename std::conditional<HD == 64, uint16_t, uint8_t>::type>::type Codes;
+    Codes codes[4];
+    Words<HD / 32> scales;
+    // `block`: of the page and kv head; `at`: where its scales begin
+    __device__ __forceinline__ void load(const char* block, int slot, int at, int c) {
+        const Codes* p = reinterpret_cast<const Codes*>(block + slot * (HD / 2)) + c;
+#pragma unroll
+        for (int i = 0; i < 4; i++) codes[i] = p[i * (HD / 2 / (int)sizeof(Codes))];
+        scales = load_words<HD / 32>(block + at + slot * (HD / 32));
+    }
+    __device__ __forceinline__ void widen(int i, uint32_t w[HD / 32], int c) const {
+        constexpr int B = HD / 32;                        // blocks, and scale bytes, of a position
+        const uint32_t shift = 8 * (i * B % 4) + 8 * (c / (32 / (HD / 16)));
+        const float unit = mx_unit((scales.w[i * B / 4] >> shift) & 255u);
+        w[0] = mx_pair<0>(codes[i], unit);
+        if constexpr (HD >= 64) w[1] = mx_pair<1>(codes[i], unit);
+        if constexpr (HD == 128) {
+            w[2] = mx_pair<2>(codes[i], unit);
+            w[3] = mx_pair<3>(codes[i], unit);
         }
     }
 };
@@ -725,24 +785,40 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
     const C* values = static_cast<const C*>(a.p.values);
     const int slots = (1 << a.p.page_shift) - 1;
     const int steps = (hi - lo + STEP - 1) / STEP;
-    u4 kf[2][NT][NK];
-    const auto load_keys = [&](int step, int page[NT], u4 f[NT][NK]) {
+    using Key = typename KeyOf<C, HD>::type;
+    Key kf[2][NT];
+    const auto load_keys = [&](int step, int page[NT], Key f[NT]) {
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             const int got = __builtin_amdgcn_readlane(page_reg, page_n * NT + t);
             page[t] = lo + STEP * step + 16 * t < hi ? got : -1;
+            if constexpr (R::MX) {
+                const size_t block = ((size_t)max(page[t], 0) * a.p.n_kv + kvh) * paged_mx_block(a.p);
+                const int slot = ((lo + STEP * step + 16 * t) & slots) + c;
+                const char* k = static_cast<const char*>(a.p.keys) + block;
+                f[t].codes = load_words<HD / 32>(k + slot * (HD / 2) + g * (HD / 8));
+                f[t].scale = (uint8_t)k[(HD / 2 << a.p.page_shift) + slot * (HD / 32) + g * HD / 128];
+            } else {
             const C* k = keys + paged_offset(a.p, max(page[t], 0), kvh, (lo + STEP * step + 16 * t) & slots) + (size_t)c * HD + R::KE * g;
 #pragma unroll
-            for (int i = 0; i < NK; i++) f[t][i] = *reinterpret_cast<const u4*>(k + i * R::KD);
+            for (int i = 0; i < NK; i++) f[t].f[i] = *reinterpret_cast<const u4*>(k + i * R::KD);
+            }
         }
     };
     int page[NT], next_page[NT] = {};
-    const auto step_on = [&](int step, u4 (&kc)[NT][NK], u4 (&kn)[NT][NK]) {
+    const auto step_on = [&](int step, Key (&kc)[NT], Key (&kn)[NT]) {
         // values of this step, keys of the next (the next step's values too
         // measured the same or, with a wavefront per SIMD fewer, slower)
         typename R::Value vr[NT][4];
+        MxValues<HD> vx[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
+            if constexpr (R::MX) {
+                const size_t block = ((size_t)max(page[t], 0) * a.p.n_kv + kvh) * paged_mx_block(a.p);
+                const int slot = ((lo + STEP * step + 16 * t) & slots) + 4 * g;
+                vx[t].load(static_cast<const char*>(a.p.values) + block, slot, HD / 2 << a.p.page_shift, c);
+                continue;
+            }
             const C* v = values + paged_offset(a.p, max(page[t], 0), kvh, ((lo + STEP * step + 16 * t) & slots) + 4 * g) + (size_t)c * NJ;
 #pragma unroll
             for (int i = 0; i < 4; i++) vr[t][i] = load_words<R::VW>(v + (size_t)i * HD);
@@ -755,7 +831,23 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
             load_keys(step + W, next_page, kn);
         }
         float s[NT][4];
-        r.scores(kc, s);
+        if constexpr (R::MX) {
+            u4 kw[NT][NK];
+#pragma unroll
+            for (int t = 0; t < NT; t++) kc[t].widen(kw[t]);
+            r.scores(kw, s);
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) vx[t].widen(i, vr[t][i].w, c);
+        } else {
+            u4 kw[NT][NK];
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < NK; i++) kw[t][i] = kc[t].f[i];
+            r.scores(kw, s);
+        }
         const int p0 = lo + STEP * step;
         bool edge = p0 + STEP > min(least, hi), odd = false;
 #pragma unroll
@@ -887,6 +979,43 @@ __global__ __launch_bounds__(64 * kTileWaves, HD == 128 ? 2 : 4) void k_paged_at
     const auto pages_from = [&](int at) { return at < hi ? paged_page(set.pages[at >> a.p.page_shift], a.p.n_pages) : -1; };
     constexpr int S = POS / 16;
     int page_reg = pages_from(lo + 16 * lane), next_reg = page_reg;
+    // MXFP4: a thread's pieces (8 elements) of a tile, codes in registers while
+    // the tile before is computed, bf16 in LDS from then on
+    constexpr int MP = R::MX ? 2 * POS * PIECES / (64 * kTileWaves) : 1;
+    uint32_t codes[MP], scale[MP];
+    const auto mx_place = [&](int n, bool* key, int* row, int* pc) {
+        const int i = 64 * kTileWaves * n + tid, j = i % (POS * PIECES);
+        *key = i < POS * PIECES;
+        *row = j / PIECES;
+        *pc = j % PIECES;
+    };
+    const auto mx_fetch = [&](int t, int reg) {
+#pragma unroll
+        for (int n = 0; n < MP; n++) {
+            bool key;
+            int row, pc;
+            mx_place(n, &key, &row, &pc);
+            // (a wavefront's pieces lie in one stretch of 16 positions)
+            const int page = __builtin_amdgcn_readlane(reg, (t % (64 / S)) * S + __builtin_amdgcn_readfirstlane(row) / 16);
+            const char* block = static_cast<const char*>(key ? a.p.keys : a.p.values) + ((size_t)max(page, 0) * a.p.n_kv + kvh) * paged_mx_block(a.p);
+            const int slot = (lo + POS * t + row) & slots;
+            codes[n] = *reinterpret_cast<const uint32_t*>(block + slot * (HD / 2) + 4 * pc);
+            scale[n] = (uint8_t)block[(HD / 2 << a.p.page_shift) + slot * (HD / 32) + pc / 4];
+        }
+    };
+    const auto mx_store = [&](int buffer) {
+#pragma unroll
+        for (int n = 0; n < MP; n++) {
+            bool key;
+            int row, pc;
+            mx_place(n, &key, &row, &pc);
+            const int r16 = row & 15;
+            const uint32_t at = row * RB + 16 * (pc ^ (key ? (r16 / PER) & SWZ : 2 * ((r16 / PER) & VSWZ)));
+            const float unit = mx_unit(scale[n]);
+            *reinterpret_cast<u4*>(&lds[buffer][key ? 0 : 1][at]) =
+                u4{mx_pair<0>(codes[n], unit), mx_pair<1>(codes[n], unit), mx_pair<2>(codes[n], unit), mx_pair<3>(codes[n], unit)};
+        }
+    };
     // Brings a tile's keys and values into a buffer: RB bytes per position, 1024 per instruction.
     const int prow = lane / PIECES, piece = lane % PIECES;
     constexpr int PI = 1024 / RB, N = POS / PI;                // positions per instruction, instructions
@@ -916,14 +1045,20 @@ __global__ __launch_bounds__(64 * kTileWaves, HD == 128 ? 2 : 4) void k_paged_at
     const int v_row = 4 * g + c / 4, v_swz = (v_row / PER) & VSWZ;
 #pragma unroll
     for (int j = 0; j < NJ; j++) v_at[j] = v_row * RB + 32 * (j ^ v_swz) + 8 * (c & 3);
-    fetch(0, page_reg, 0);
+    if constexpr (R::MX) {
+        mx_fetch(0, page_reg);
+        mx_store(0);
+    } else {
+        fetch(0, page_reg, 0);
+    }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     lds_barrier();
     for (int t = 0; t < tiles; t++) {
         const int buffer = t & 1;
         if (t + 1 < tiles) {
             next_reg = (t + 1) % (64 / S) ? page_reg : pages_from(lo + POS * (t + 1) + 16 * lane);
-            fetch(t + 1, next_reg, buffer ^ 1);
+            if constexpr (R::MX) mx_fetch(t + 1, next_reg);
+            else fetch(t + 1, next_reg, buffer ^ 1);
         }
         const char* kt = lds[buffer][0];
         const char* vt = lds[buffer][1];
@@ -971,6 +1106,9 @@ __global__ __launch_bounds__(64 * kTileWaves, HD == 128 ? 2 : 4) void k_paged_at
             }
         }
         page_reg = next_reg;
+        if constexpr (R::MX) {
+            if (t + 1 < tiles) mx_store(buffer ^ 1);
+        }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // the next tile is there
         lds_barrier();
     }
@@ -1333,8 +1471,9 @@ yl_status yl_paged_attention(float* out, size_t out_ld, const float* q, size_t q
     hipStream_t s = (hipStream_t)stream;
     float* space = static_cast<float*>(workspace);
     const hipError_t e = cache->dtype == YL_T_F32   ? launch_all<float>(a, plan, space, s)
-                         : cache->dtype == YL_T_F16 ? launch_all<_Float16>(a, plan, space, s)
-                                                    : launch_all<__bf16>(a, plan, space, s);
+                         : cache->dtype == YL_T_F16  ? launch_all<_Float16>(a, plan, space, s)
+                         : cache->dtype == YL_T_BF16 ? launch_all<__bf16>(a, plan, space, s)
+                                                     : launch_all<Mx4>(a, plan, space, s);
     if (e == hipSuccess) return YL_OK;
     set_error(std::string("paged_attention launch: ") + hipGetErrorString(e));
     return YL_ERR_HIP;

@@ -14,6 +14,7 @@ Ops for programs that serve many conversations from one pool of cache pages
 include/yallma3.h say what they hold):
   rope_table        the (cos, sin) tables that paged_append rotates by
   paged_append      rows' keys and values into pages, rotated on the way
+  paged_gather      keys and values back out of their pages
   paged_attention   causal attention over pages, a shared prefix read once
   token_logprobs    log probabilities of tokens, entropy, top alternatives
 """
@@ -155,13 +156,18 @@ class PagedBatch:
 
 def _pool(keys, values):
     """Device copies and the descriptor of pages [n_pages][kv_heads][page_size][head_size]
-    (float32, float16, or bf16 bits as uint16)."""
+    (float32, float16, or bf16 bits as uint16); uint8: MXFP4 bytes, 17 / 32 of
+    head_size in the last dimension (codes and scales stand as yl_paged_cache says)."""
     keys, values = np.ascontiguousarray(keys), np.ascontiguousarray(values)
-    if keys.ndim != 4 or keys.shape != values.shape or keys.dtype != values.dtype or keys.dtype not in _DTYPE_OF:
-        raise ValueError("keys and values: [pages][kv_heads][page_size][head_size] of float32, float16 or uint16 (bf16 bits)")
-    dk, dv = DeviceBuffer.from_numpy(keys), DeviceBuffer.from_numpy(values)
+    if keys.ndim != 4 or keys.shape != values.shape or keys.dtype != values.dtype or keys.dtype not in (*_DTYPE_OF, np.uint8):
+        raise ValueError("keys and values: [pages][kv_heads][page_size][head_size] of float32, float16, uint16 (bf16 bits) or uint8 (MXFP4)")
     n_pages, kvh, page, hd = keys.shape
-    return dk, dv, PagedCacheDesc(dk.ptr, dv.ptr, DTYPES[_DTYPE_OF[keys.dtype]], n_pages, page, kvh, hd)
+    if keys.dtype == np.uint8:
+        if hd % 17:
+            raise ValueError("MXFP4 pages take 17 bytes for 32 elements")
+        hd = hd // 17 * 32
+    dk, dv = DeviceBuffer.from_numpy(keys), DeviceBuffer.from_numpy(values)
+    return dk, dv, PagedCacheDesc(dk.ptr, dv.ptr, DTYPES[_DTYPE_OF.get(keys.dtype, "mxfp4")], n_pages, page, kvh, hd)
 
 
 def _rows(x):
@@ -198,6 +204,19 @@ def paged_append(keys, values, batch: PagedBatch, q, k, v, n_heads: int, pairs: 
                                 bc.ptr if bc else None, bs.ptr if bs else None, len(cos) if cos is not None else 0, None))
     check(lib().yl_synchronize())
     return bq.numpy() if bq else None, dk.numpy(), dv.numpy()
+
+
+def paged_gather(keys, values, batch: PagedBatch, rows: int, fill: float = 0.0):
+    """yl_paged_gather of `rows` rows -> (keys, values) [rows][kv_heads *
+    head_size]; rows whose position nothing holds come back as `fill`."""
+    dk, dv, cache = _pool(keys, values)
+    batch.check_prefix(cache.page_size)
+    desc, held = batch.upload(rows)
+    kv = cache.n_kv_heads * cache.head_size
+    out = [DeviceBuffer.from_numpy(np.full((rows, kv), fill, np.float32)) for _ in range(2)]
+    check(lib().yl_paged_gather(C.byref(cache), C.byref(desc), out[0].ptr, kv, out[1].ptr, kv, None))
+    check(lib().yl_synchronize())
+    return out[0].numpy(), out[1].numpy()
 
 
 def paged_attention(keys, values, batch: PagedBatch, q, n_heads: int, attn_scale: float) -> np.ndarray:
