@@ -340,6 +340,68 @@ yl_status yl_paged_attention(float *out, size_t out_ld, const float *q, size_t q
                              const yl_paged_batch *batch, uint32_t n_heads, float attn_scale, void *workspace,
                              size_t workspace_bytes, void *stream);
 
+/* Which pages of a pool are in use, for the operations below.  Every layer of a
+ * model has its own yl_paged_cache; one set of tables names the pages of all of
+ * them.  page_table, kv_len, prefix_len and prefix_pages as in yl_paged_batch
+ * (every row of the table is a sequence, or free: entries -1).  refs[p]: how
+ * many entries of page_table and prefix_pages name page p; 0 or less: free.
+ * page_size and n_pages are those of the pools; n_seqs at most 2^22, n_seqs *
+ * max_pages below 2^31.
+ *
+ * The operations enqueue on `stream` like those above.  Results are defined to
+ * the bit: free pages are taken in rising order, by the entries of a call in
+ * their order.  Operations on the same tables have to follow each other.
+ * workspace: yl_paged_tables_workspace bytes, 16-byte aligned, for `n` forks at
+ * most; it serves any of the operations on tables no larger.  `lacking` (device,
+ * nullable) receives a count and is 0 when all was done. */
+typedef struct {
+    uint32_t n_seqs, max_pages, n_pages, page_size;
+    int32_t *page_table;         /* device [n_seqs][max_pages] */
+    uint32_t *kv_len;            /* device [n_seqs] */
+    int32_t *refs;               /* device [n_pages] */
+    uint32_t prefix_len;
+    int32_t *prefix_pages;       /* device [ceil(prefix_len / page_size)]; unused without a prefix */
+} yl_paged_tables;
+
+size_t yl_paged_tables_workspace(const yl_paged_tables *tables, uint32_t n);
+
+/* Gives every sequence pages for its positions below want_len[s] (device,
+ * [n_seqs]): entries there that name no page get a free one, sequence by
+ * sequence.  kv_len stays.  *lacking: entries that got none, the pool being
+ * used up (the first ones are served), and sequences whose table is too short. */
+yl_status yl_paged_reserve(const yl_paged_tables *tables, const uint32_t *want_len, uint32_t *lacking, void *workspace,
+                           size_t workspace_bytes, void *stream);
+
+/* Makes sequence children[i] a branch of parents[i] (device, n each): it names
+ * its parent's filled pages (one more reference each), and a page that the
+ * parent has filled in part is copied, its filled slots in all layers, to a free
+ * one; the rest of its table row becomes -1, its kv_len the parent's.  A child's
+ * row is overwritten: it should be empty.  No sequence may be a child twice, or
+ * both a child and a parent, in one call; pairs that name no sequence, or the
+ * same one twice, are passed over.  *lacking: children that the pool had no page
+ * for; their rows are -1, their kv_len 0. */
+yl_status yl_paged_fork(const yl_paged_tables *tables, const yl_paged_cache *layers, uint32_t n_layers, const uint32_t *parents,
+                        const uint32_t *children, uint32_t n, uint32_t *lacking, void *workspace, size_t workspace_bytes,
+                        void *stream);
+
+/* Ends sequences (seqs: device, n ids; one may be there twice, ids that are none
+ * are passed over): every page they name has one reference less, their rows
+ * become -1, their kv_len 0. */
+yl_status yl_paged_release(const yl_paged_tables *tables, const uint32_t *seqs, uint32_t n, void *stream);
+
+/* Moves the pages in use to ids 0 .. *used - 1 (device): the free ids below take
+ * the pages from there on, both in rising order, in all layers; tables,
+ * prefix_pages and refs follow.  Entries that name a free page stay. */
+yl_status yl_paged_compact(const yl_paged_tables *tables, const yl_paged_cache *layers, uint32_t n_layers, uint32_t *used,
+                           void *workspace, size_t workspace_bytes, void *stream);
+
+/* Copies page src_pages[i] of every layer of `src` to dst_pages[i] of the same
+ * layer of `dst` (device ids, n each; pairs of which one names no page are
+ * passed over): pools of one type, page size and heads, or the same pools.  No
+ * page may be written twice, or written and read, in one call. */
+yl_status yl_paged_copy(const yl_paged_cache *dst, const yl_paged_cache *src, uint32_t n_layers, const int32_t *dst_pages,
+                        const int32_t *src_pages, uint32_t n, void *stream);
+
 /* Scores rows of logits [rows][vocab] of `dtype` (device, ld elements apart):
  *   logprob[r] = x[tokens[r]] - log sum_i exp(x[i])  (-inf for an id that is
  *                not below vocab); tokens and logprob both NULL: not wanted
@@ -355,6 +417,36 @@ size_t yl_token_logprobs_workspace(size_t rows, size_t vocab, uint32_t top);
 yl_status yl_token_logprobs(const void *logits, int32_t dtype, size_t rows, size_t vocab, size_t ld,
                             const uint32_t *tokens, float *logprob, float *entropy, uint32_t top, uint32_t *top_ids,
                             float *top_logprobs, void *workspace, size_t workspace_bytes, void *stream);
+
+/* What rows of logits are subject to (all device; NULL: not wanted).  Lists of
+ * rows: row r has the entries start[r] .. start[r + 1] - 1 (the starts ascend). */
+typedef struct {
+    const uint32_t *tokens, *token_start;   /* tokens that are there already; token_start [rows + 1] */
+    const uint32_t *n_prompt;               /* [rows]: how many of the row's tokens, the first ones, are its prompt's (NULL: none) */
+    uint32_t n_tokens;                      /* entries of tokens */
+    const float *repetition, *presence, *frequency;   /* [rows] each: above 0; any; any (NULL: 1, 0, 0) */
+    const uint32_t *bias_ids;
+    const float *bias;
+    const uint32_t *bias_start;             /* [rows + 1] */
+    uint32_t n_biases;                      /* entries of bias_ids and bias */
+    const uint32_t *mask;                   /* [mask_rows] grammars, mask_ld words apart: bit id % 32 of word id / 32: allowed */
+    size_t mask_ld;
+    uint32_t mask_rows;
+    const int32_t *mask_of;                 /* [rows]: row r's grammar, negative: none, not below mask_rows: nothing is
+                                               allowed; NULL: grammar r */
+} yl_logit_rules;
+
+/* Applies rules to rows of logits [rows][vocab] of `dtype` (device, ld elements
+ * apart) into out (out_ld apart; may be logits, with ld, but not overlap them
+ * otherwise).  For the logit x of an id, each step rounded to f32, the result
+ * once to `dtype`:
+ *   among the row's tokens:                       x > 0 ? x / repetition : x * repetition
+ *   n > 0 times among those after its prompt:     x - frequency n - presence
+ *   biased:                                       x + bias (of an id's several in a list, the last)
+ *   not allowed by the row's grammar:             -inf
+ * Ids that are not below vocab count for nothing.  NaN stays NaN where it is allowed. */
+yl_status yl_adjust_logits(void *out, size_t out_ld, const void *logits, size_t ld, int32_t dtype, size_t rows, size_t vocab,
+                           const yl_logit_rules *rules, void *stream);
 
 /* --------------------------------------------------- model and session */
 

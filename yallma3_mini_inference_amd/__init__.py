@@ -14,7 +14,8 @@ reference's API over it:
                                                        reference does not have
   synth                                                seeded GGUF models
 """
-from ._lib import DTYPES, LIB_PATH, ROPE_PAIRS, PagedBatchDesc, PagedCacheDesc, YlError, check, lib
+from ._lib import (DTYPES, LIB_PATH, ROPE_PAIRS, LogitRules, PagedBatchDesc, PagedCacheDesc, PagedTablesDesc, YlError, check,
+                   lib)
 from .device import DeviceBuffer, device_count
 from .tokenizer import Sampler, Tokenizer, pretokenize
 from .transformer import (InferenceSession, Transformer, TransformerLlamaGguf, infer_ffi, infer_reset,
@@ -26,4 +27,5 @@ __all__ = [
     "TransformerLlamaGguf", "infer_ffi", "load_transformer", "load_transformer_ffi", "QuantizedWeight",
     "WeightFormat", "matmul", "matmul_device", "quantize", "quantize_device", "Sampler", "Tokenizer", "pretokenize",
     "infer_reset", "infer_set_max_tokens", "DTYPES", "ROPE_PAIRS", "PagedBatchDesc", "PagedCacheDesc",
+    "PagedTablesDesc", "LogitRules",
 ]

@@ -33,7 +33,8 @@ EXPORTS = [
     "yl_tokenize", "yl_detokenize", "yl_chat_template", "yl_chat_prompt", "yl_pretokenize", "yl_sampler_new",
     "yl_sampler_sample", "yl_sampler_free", "yl_generate_text", "yl_weight_upload_f16", "yl_matmul_f32",
     "yl_rope_table", "yl_paged_append", "yl_paged_gather", "yl_paged_attention_workspace", "yl_paged_attention",
-    "yl_token_logprobs_workspace", "yl_token_logprobs",
+    "yl_token_logprobs_workspace", "yl_token_logprobs", "yl_paged_tables_workspace", "yl_paged_reserve", "yl_paged_fork",
+    "yl_paged_release", "yl_paged_compact", "yl_paged_copy", "yl_adjust_logits",
 ]
 
 # yl_dtype, and which elements of a head a rotation turns together (YL_ROPE_*)
@@ -75,6 +76,21 @@ class PagedBatchDesc(C.Structure):
     _fields_ = [("n_seqs", C.c_uint32), ("n_rows", C.c_uint32), ("max_pages", C.c_uint32), ("max_len", C.c_uint32),
                 ("page_table", C.c_void_p), ("kv_len", C.c_void_p), ("row_start", C.c_void_p),
                 ("prefix_len", C.c_uint32), ("prefix_pages", C.c_void_p)]
+
+
+class PagedTablesDesc(C.Structure):
+    """yl_paged_tables: which pages of a pool are in use (device arrays)."""
+    _fields_ = [("n_seqs", C.c_uint32), ("max_pages", C.c_uint32), ("n_pages", C.c_uint32), ("page_size", C.c_uint32),
+                ("page_table", C.c_void_p), ("kv_len", C.c_void_p), ("refs", C.c_void_p), ("prefix_len", C.c_uint32),
+                ("prefix_pages", C.c_void_p)]
+
+
+class LogitRules(C.Structure):
+    """yl_logit_rules: what rows of logits are subject to (device arrays)."""
+    _fields_ = [("tokens", C.c_void_p), ("token_start", C.c_void_p), ("n_prompt", C.c_void_p), ("n_tokens", C.c_uint32),
+                ("repetition", C.c_void_p), ("presence", C.c_void_p), ("frequency", C.c_void_p), ("bias_ids", C.c_void_p),
+                ("bias", C.c_void_p), ("bias_start", C.c_void_p), ("n_biases", C.c_uint32), ("mask", C.c_void_p),
+                ("mask_ld", C.c_size_t), ("mask_rows", C.c_uint32), ("mask_of", C.c_void_p)]
 
 
 class SynthConfig(C.Structure):
@@ -189,6 +205,13 @@ def lib():
                                     sz, vp]),
         "yl_token_logprobs_workspace": (sz, [sz, sz, u32]),
         "yl_token_logprobs": (st, [vp, st, sz, sz, sz, vp, vp, vp, u32, vp, vp, vp, sz, vp]),
+        "yl_paged_tables_workspace": (sz, [C.POINTER(PagedTablesDesc), u32]),
+        "yl_paged_reserve": (st, [C.POINTER(PagedTablesDesc), vp, vp, vp, sz, vp]),
+        "yl_paged_fork": (st, [C.POINTER(PagedTablesDesc), C.POINTER(PagedCacheDesc), u32, vp, vp, u32, vp, vp, sz, vp]),
+        "yl_paged_release": (st, [C.POINTER(PagedTablesDesc), vp, u32, vp]),
+        "yl_paged_compact": (st, [C.POINTER(PagedTablesDesc), C.POINTER(PagedCacheDesc), u32, vp, vp, sz, vp]),
+        "yl_paged_copy": (st, [C.POINTER(PagedCacheDesc), C.POINTER(PagedCacheDesc), u32, vp, vp, u32, vp]),
+        "yl_adjust_logits": (st, [vp, sz, vp, sz, st, sz, sz, C.POINTER(LogitRules), vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

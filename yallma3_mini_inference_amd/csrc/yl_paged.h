@@ -95,7 +95,46 @@ YL_HD bool paged_place(const PagedArgs& a, int s, int64_t pos, int* page, int* s
     return *page >= 0;
 }
 
+// The tables of a pool as the page operations see them (yl_paged_tables).
+struct TableArgs {
+    int n_seqs, max_pages, n_pages, page_shift;
+    int32_t* table; uint32_t* kv_len; int32_t* refs;
+    int prefix_len, prefix_entries;
+    int32_t* prefix_pages;
+};
+
+// Positions of its own that a length stands for.
+YL_HD int64_t table_own(const TableArgs& t, uint32_t len) {
+    return (int64_t)len > t.prefix_len ? (int64_t)len - t.prefix_len : 0;
+}
+// Whole pages of its own that a sequence of that length has filled, within its
+// table, and the filled slots of the next entry (0: there is none).
+YL_HD void table_filled(const TableArgs& t, uint32_t len, int* full, int* slots) {
+    const int64_t own = table_own(t, len), pages = own >> t.page_shift;
+    *full = (int)(pages < t.max_pages ? pages : t.max_pages);
+    *slots = pages < t.max_pages ? (int)(own & ((1 << t.page_shift) - 1)) : 0;
+}
+// Entries that positions below `len` take, within the table; *past: whether it is too short.
+YL_HD int table_entries(const TableArgs& t, uint32_t len, bool* past) {
+    const int64_t n = (table_own(t, len) + (1 << t.page_shift) - 1) >> t.page_shift;
+    *past = n > t.max_pages;
+    return (int)(*past ? t.max_pages : n);
+}
+
+// Pages that one workgroup looks through, and how many workgroups that takes (at most 1024).
+constexpr int kPagesPerStep = 1024;
+YL_HD int pages_per_group(int n_pages) {
+    const int64_t steps = ((int64_t)n_pages + kPagesPerStep - 1) / kPagesPerStep;
+    return (int)((steps + 1023) / 1024) * kPagesPerStep;
+}
+YL_HD int page_groups(int n_pages) {
+    const int64_t per = pages_per_group(n_pages);
+    return (int)(((int64_t)n_pages + per - 1) / per);
+}
+
 #if defined(YALLMA3_H)
+// YL_OK if the pool's description is one that the kernels take, or the refusal.
+yl_status paged_cache_ok(const yl_paged_cache* c);
 // The kernels' arguments from a caller's descriptions; YL_OK, or the refusal.
 yl_status paged_args(const yl_paged_cache* c, const yl_paged_batch* b, uint32_t n_heads, PagedArgs* a);
 #endif

@@ -217,18 +217,24 @@ yl_status refuse(const char* what, yl_status st = YL_ERR_ARG) {
 
 }  // namespace
 
-yl_status paged_args(const yl_paged_cache* c, const yl_paged_batch* b, uint32_t n_heads, PagedArgs* a) {
-    if (!c || !b) return refuse("paged: no cache or no batch");
+yl_status paged_cache_ok(const yl_paged_cache* c) {
     if (c->dtype != YL_T_F32 && c->dtype != YL_T_F16 && c->dtype != YL_T_BF16 && c->dtype != YL_T_MXFP4)
         return refuse("paged: the cache's type is f32, f16, bf16 or MXFP4", YL_ERR_FORMAT);
     if (c->head_size != 32 && c->head_size != 64 && c->head_size != 128) return refuse("paged: head size 32, 64 or 128");
     if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128 && c->page_size != 256)
         return refuse("paged: page size 16, 32, 64, 128 or 256");
     if (!c->n_pages || (uint64_t)c->n_pages * c->page_size >= (1ull << 31)) return refuse("paged: n_pages * page_size from 1 page to below 2^31");
-    if (!c->n_kv_heads || !n_heads || n_heads % c->n_kv_heads || n_heads > 1024)
-        return refuse("paged: n_heads (at most 1024) is a multiple of n_kv_heads");
     if (!c->keys || !c->values || ((uintptr_t)c->keys | (uintptr_t)c->values) % 16)
         return refuse("paged: keys and values have to be there, 16-byte aligned");
+    if (!c->n_kv_heads || c->n_kv_heads > 1024) return refuse("paged: n_kv_heads from 1 to 1024");
+    return YL_OK;
+}
+
+yl_status paged_args(const yl_paged_cache* c, const yl_paged_batch* b, uint32_t n_heads, PagedArgs* a) {
+    if (!c || !b) return refuse("paged: no cache or no batch");
+    const yl_status st = paged_cache_ok(c);
+    if (st != YL_OK) return st;
+    if (!n_heads || n_heads % c->n_kv_heads || n_heads > 1024) return refuse("paged: n_heads (at most 1024) is a multiple of n_kv_heads");
     if ((uint64_t)b->n_rows * n_heads >= (1ull << 24) || (uint64_t)b->n_seqs * n_heads >= (1ull << 22) ||
         (uint64_t)b->prefix_len + (uint64_t)b->max_pages * c->page_size >= (1ull << 30))
         return refuse("paged: n_rows * n_heads below 2^24, n_seqs * n_heads below 2^22, a sequence's capacity below 2^30", YL_ERR_RANGE);

@@ -16,6 +16,10 @@ include/yallma3.h say what they hold):
   paged_append      rows' keys and values into pages, rotated on the way
   paged_gather      keys and values back out of their pages
   paged_attention   causal attention over pages, a shared prefix read once
+  paged_reserve, paged_fork, paged_release, paged_compact, paged_copy
+                    the pages themselves: handed out, shared by branches of a
+                    conversation, given back, moved together, copied
+  adjust_logits     penalties for repeated tokens, biases, grammar masks
   token_logprobs    log probabilities of tokens, entropy, top alternatives
 """
 from __future__ import annotations
@@ -25,7 +29,7 @@ import dataclasses
 
 import numpy as np
 
-from ._lib import DTYPES, ROPE_PAIRS, PagedBatchDesc, PagedCacheDesc, RopeParams, check, lib
+from ._lib import DTYPES, ROPE_PAIRS, LogitRules, PagedBatchDesc, PagedCacheDesc, PagedTablesDesc, RopeParams, check, lib
 from .device import DeviceBuffer
 
 
@@ -234,6 +238,150 @@ def paged_attention(keys, values, batch: PagedBatch, q, n_heads: int, attn_scale
                                    need, None))
     check(lib().yl_synchronize())
     return out.numpy()
+
+
+@dataclasses.dataclass
+class PagedTables:
+    """yl_paged_tables on host arrays: page_table [seqs][entries], kv_len
+    [seqs], refs [pages].  The operations below update them in place."""
+    page_table: np.ndarray
+    kv_len: np.ndarray
+    refs: np.ndarray
+    page_size: int
+    prefix_len: int = 0
+    prefix_pages: np.ndarray | None = None
+
+    def __post_init__(self):
+        self.page_table = np.ascontiguousarray(self.page_table, np.int32)
+        self.kv_len = np.ascontiguousarray(self.kv_len, np.uint32)
+        self.refs = np.ascontiguousarray(self.refs, np.int32)
+        if self.page_table.ndim != 2 or self.page_table.shape[0] != self.kv_len.size:
+            raise ValueError("page_table holds a row of entries per sequence")
+        if self.prefix_pages is not None:
+            self.prefix_pages = np.ascontiguousarray(self.prefix_pages, np.int32)
+        if self.prefix_len and (self.prefix_pages is None or self.prefix_pages.size * self.page_size < self.prefix_len):
+            raise ValueError("prefix_pages does not reach prefix_len")
+
+    def _run(self, forks: int, call):
+        """call(descriptor, workspace pointer, its bytes) on device copies, which are read back."""
+        arrays = [self.page_table, self.kv_len, self.refs] + ([self.prefix_pages] if self.prefix_len else [])
+        held = [DeviceBuffer.from_numpy(a) for a in arrays]
+        desc = PagedTablesDesc(*self.page_table.shape, self.refs.size, self.page_size, held[0].ptr, held[1].ptr, held[2].ptr,
+                               self.prefix_len, held[3].ptr if self.prefix_len else None)
+        need = lib().yl_paged_tables_workspace(C.byref(desc), forks)
+        space = DeviceBuffer(need)
+        check(call(C.byref(desc), space.ptr, need))
+        check(lib().yl_synchronize())
+        for a, b in zip(arrays, held):
+            a[...] = b.numpy()
+
+
+def _layer_pools(layers):
+    """Device copies and descriptors of [(keys, values), ...]."""
+    pools = [_pool(k, v) for k, v in layers]
+    return pools, (PagedCacheDesc * max(1, len(pools)))(*[p[2] for p in pools])
+
+
+def _pools_back(pools):
+    return [(p[0].numpy(), p[1].numpy()) for p in pools]
+
+
+def _ids(x, dtype=np.uint32):
+    x = np.ascontiguousarray(x, dtype)
+    if x.ndim != 1:
+        raise ValueError("ids: one dimension")
+    return x, DeviceBuffer.from_numpy(x)
+
+
+def paged_reserve(tables: PagedTables, want_len) -> int:
+    """yl_paged_reserve -> entries that got no page."""
+    want, dw = _ids(want_len)
+    if want.size != tables.kv_len.size:
+        raise ValueError("want_len: one per sequence")
+    lacking = DeviceBuffer.zeros(1, np.uint32)
+    tables._run(0, lambda t, w, n: lib().yl_paged_reserve(t, dw.ptr, lacking.ptr, w, n, None))
+    return int(lacking.numpy()[0])
+
+
+def paged_fork(tables: PagedTables, layers, parents, children):
+    """yl_paged_fork of layers [(keys, values), ...] -> (children that got no page, layers)."""
+    (p, dp), (c, dc) = _ids(parents), _ids(children)
+    if p.size != c.size:
+        raise ValueError("a child for every parent")
+    pools, descs = _layer_pools(layers)
+    lacking = DeviceBuffer.zeros(1, np.uint32)
+    tables._run(p.size, lambda t, w, n: lib().yl_paged_fork(t, descs, len(pools), dp.ptr, dc.ptr, p.size, lacking.ptr, w, n, None))
+    return int(lacking.numpy()[0]), _pools_back(pools)
+
+
+def paged_release(tables: PagedTables, seqs) -> None:
+    """yl_paged_release."""
+    s, ds = _ids(seqs)
+    tables._run(0, lambda t, w, n: lib().yl_paged_release(t, ds.ptr, s.size, None))
+
+
+def paged_compact(tables: PagedTables, layers):
+    """yl_paged_compact of layers [(keys, values), ...] -> (pages in use, layers)."""
+    pools, descs = _layer_pools(layers)
+    used = DeviceBuffer.zeros(1, np.uint32)
+    tables._run(0, lambda t, w, n: lib().yl_paged_compact(t, descs, len(pools), used.ptr, w, n, None))
+    return int(used.numpy()[0]), _pools_back(pools)
+
+
+def paged_copy(dst_layers, src_layers, dst_pages, src_pages):
+    """yl_paged_copy from one set of layers [(keys, values), ...] to another (None: the same pools) -> the written ones."""
+    (d, dd), (s, ds) = _ids(dst_pages, np.int32), _ids(src_pages, np.int32)
+    if d.size != s.size or (src_layers is not None and len(src_layers) != len(dst_layers)):
+        raise ValueError("as many sources as destinations")
+    to, to_desc = _layer_pools(dst_layers)
+    src, src_desc = _layer_pools(src_layers) if src_layers is not None else (to, to_desc)
+    check(lib().yl_paged_copy(to_desc, src_desc, len(to), dd.ptr, ds.ptr, d.size, None))
+    check(lib().yl_synchronize())
+    return _pools_back(to)
+
+
+def _row_lists(lists, dtype):
+    """(entries of all rows, starts) of a list of arrays per row."""
+    rows = [np.ascontiguousarray(x, dtype).ravel() for x in lists]
+    return np.concatenate(rows + [np.empty(0, dtype)]), np.concatenate([[0], np.cumsum([r.size for r in rows])]).astype(np.uint32)
+
+
+def adjust_logits(logits, tokens=None, n_prompt=None, repetition=None, presence=None, frequency=None, biases=None, mask=None,
+                  mask_of=None) -> np.ndarray:
+    """yl_adjust_logits of logits [rows][vocab] (float32, float16, or bf16 bits
+    as uint16).  tokens: an array of ids per row; biases: (ids, values) per row;
+    mask: uint32 words [grammars][ceil(vocab / 32)]; the others one per row."""
+    x = np.ascontiguousarray(logits)
+    if x.ndim != 2 or x.dtype not in _DTYPE_OF:
+        raise ValueError("logits: [rows][vocab] of float32, float16 or uint16 (bf16 bits)")
+    rows, vocab = x.shape
+    per_row = dict(n_prompt=n_prompt, repetition=repetition, presence=presence, frequency=frequency, mask_of=mask_of, tokens=tokens, biases=biases)
+    for name, v in per_row.items():
+        if v is not None and len(v) != rows:
+            raise ValueError(name + ": one per row")
+    ids, starts = _row_lists(tokens, np.uint32) if tokens is not None else (None, None)
+    bias_ids, bias_start = _row_lists([b[0] for b in biases], np.uint32) if biases is not None else (None, None)
+    bias, ends = _row_lists([b[1] for b in biases], np.float32) if biases is not None else (None, None)
+    if biases is not None and not np.array_equal(bias_start, ends):
+        raise ValueError("biases: a value for every id")
+    if mask is not None and np.ndim(mask) != 2:
+        raise ValueError("mask: [grammars][words]")
+    held = []
+
+    def put(a, dtype):
+        if a is None:
+            return None
+        held.append(DeviceBuffer.from_numpy(np.ascontiguousarray(a, dtype)))
+        return held[-1].ptr
+
+    r = LogitRules(put(ids, np.uint32), put(starts, np.uint32), put(n_prompt, np.uint32), ids.size if ids is not None else 0,
+                   put(repetition, np.float32), put(presence, np.float32), put(frequency, np.float32), put(bias_ids, np.uint32),
+                   put(bias, np.float32), put(bias_start, np.uint32), bias.size if bias is not None else 0, put(mask, np.uint32),
+                   np.shape(mask)[1] if mask is not None else 0, np.shape(mask)[0] if mask is not None else 0, put(mask_of, np.int32))
+    dx = DeviceBuffer.from_numpy(x)
+    check(lib().yl_adjust_logits(dx.ptr, vocab, dx.ptr, vocab, DTYPES[_DTYPE_OF[x.dtype]], rows, vocab, C.byref(r), None))
+    check(lib().yl_synchronize())
+    return dx.numpy()
 
 
 def token_logprobs(logits, tokens=None, top: int = 0):
