@@ -78,7 +78,7 @@ template <> struct Type<_Float16> {
     static __device__ __forceinline__ vf4 mul(u4 a, u4 b, vf4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
     }
-    // two values -> their parts, packed
+    // two values -> their parts, packed (part[1] is not settled: see below)
     static __device__ __forceinline__ void cut(float a, float b, uint32_t part[2]) {
         const h2 hi = __builtin_convertvector(vf2{a, b}, h2);
         part[0] = __builtin_bit_cast(uint32_t, hi);
@@ -86,6 +86,10 @@ template <> struct Type<_Float16> {
         asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]\n\tv_fma_mixhi_f16 %0, %1, -1.0, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
             : "=&v"(part[1]) : "v"(part[0]), "v"(a), "v"(b));
     }
+    // A matrix instruction has to be two wait states behind the write of its
+    // operand, and the compiler does not look into the assembly above.
+    template <typename V>
+    static __device__ __forceinline__ void settle(V* part) { asm volatile("s_nop 1" : "+v"(part[1])); }
     // the power of two that brings a row of q to [2^13, 2^14): its elements keep
     // 22 bits down to 2^-15 of the largest, and are right to 2^-38 of it below
     static __device__ __forceinline__ int exponent(float amax) {
@@ -115,6 +119,7 @@ template <> struct Type<__bf16> {
             b -= __uint_as_float(part[p] & 0xffff0000u);
         }
     }
+    template <typename V> static __device__ __forceinline__ void settle(V*) {}
     static __device__ __forceinline__ int exponent(float) { return 0; }
     static __device__ __forceinline__ uint32_t not_finite(uint32_t two) {
         return ((two & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((two & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
@@ -552,6 +557,7 @@ struct Tile {
 #pragma unroll
             for (int p = 0; p < NP; p++) pf[p][d] = part[p];
         }
+        T::settle(pf);
 #pragma unroll
         for (int p = NP - 1; p >= 0; p--) {
             if constexpr (TR) ones = T::mul(u4{T::kOnes, T::kOnes, T::kOnes, T::kOnes}, pf[p], ones);
