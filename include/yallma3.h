@@ -326,6 +326,11 @@ yl_status yl_paged_gather(const yl_paged_cache *cache, const yl_paged_batch *bat
  * f32 but over f16 caches: there an element of q has 22 bits (below 2^-15 of its
  * head's largest: right to 2^-38 of that) and so has the largest weight e_j of
  * 32 or 64 positions taken together (the others: right to 2^-23 of that at least).
+ * Over MXFP4 pages the values that the codes stand for count, with a batch of one
+ * row per sequence (row_start NULL) and up to four query heads per kv head as over
+ * f16 caches, and then blocks of a key below 2^-35 of its largest, and of the
+ * values below 2^-35 of the largest value of the sequence, may count as zero; else
+ * as over bf16 caches.
  * q, out: [n_rows] rows of n_heads * head_size floats (device), q_ld and out_ld
  * floats apart; out may be q (with q_ld) but not overlap it otherwise.  A prefix
  * is read once for all sequences.  workspace (device, 16-byte aligned):

@@ -386,3 +386,119 @@ def test_serving_steps(gpu, heads, kvh, prefix):
                 row += 1
         sc.q = call.q.numpy().reshape(sc.total, -1)
         _check(sc, out)
+
+
+# ---------------------------- one row per sequence, up to four heads per kv head
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(4, 2, 32), (8, 2, 64), (6, 2, 64), (2, 2, 128), (8, 2, 128)])
+@pytest.mark.parametrize("prefix", [0, 37])
+@pytest.mark.parametrize("kind", ["few_long", "many_long", "many_short"])
+def test_single_rows(gpu, heads, kvh, hd, prefix, kind):
+    """Units of four wavefronts and of one, split and whole (128 and 1600 sequences times kv heads, 640 positions), ends
+    inside every quad of positions, and entries, lengths and sequences of nothing."""
+    rng = np.random.default_rng(heads + hd)
+    lens = {"few_long": [1500, 1, 701, 64, 65, 66, 67, 0, 130], "many_long": [1100, 900] + list(range(68)),
+            "many_short": [int(x) for x in rng.integers(0, 70, 810)]}[kind]
+    lens = [prefix + n for n in lens]
+    assert len(lens) * kvh >= {"few_long": 1, "many_long": 128, "many_short": 1600}[kind]
+    sc = MxScene([1] * len(lens), lens, heads, kvh, hd, 16, spread=1.0, prefix=prefix, seed=hd, extra_entries=1)
+    sc.table[0, 2] = -1
+    sc.table[2, 0] = sc.n_pages
+    if kind == "few_long":
+        sc.lens[3] = prefix + 16 * sc.table.shape[1] + 500      # past its table (this one fills its pages)
+    _check(sc, _attend(sc, single=True, max_len=0 if kind == "few_long" else max(lens)))
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("seqs", [3, 70])
+@pytest.mark.parametrize("slope", [0.3, -0.3, 2.0])
+def test_values_that_grow(gpu, hd, seqs, slope):
+    """Values of position p are 2^(slope p / 8) times the first ones (up to 2^120): the exponent that they are held against
+    follows; the bound is that of the largest value."""
+    sc = MxScene([1] * seqs, [700] + [90] * (seqs - 1), 4, 2, hd, 16, seed=5)
+    for s in range(min(seqs, 3)):
+        for p, (page, slot) in enumerate(sc.places(s, sc.lens[s])):
+            sc.v32[page, :, slot] *= np.float32(2.0 ** np.clip(slope * p / 8, -60, 100))
+    sc.settle()
+    _check(sc, _attend(sc, single=True))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("seqs", [3, 70])
+@pytest.mark.parametrize("power", [12, 40])
+def test_keys_of_unlike_blocks(gpu, hd, seqs, power):
+    """A block of a key that is 2^12 or 2^40 times the others, in a few positions and with queries that bring it back."""
+    sc = MxScene([1] * seqs, [700] + [90] * (seqs - 1), 4, 2, hd, 16, seed=6)
+    sc.k32[:, :, ::3, 32:] *= np.float32(2.0 ** power)
+    q = sc.q.reshape(seqs, 4, hd)
+    q[..., 32:] *= np.float32(2.0 ** -power)
+    sc.settle()
+    _check(sc, _attend(sc, single=True))
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 2, 64), (8, 2, 128), (4, 4, 32)])
+@pytest.mark.parametrize("seqs", [3, 70])
+@pytest.mark.parametrize("size", [2.0, 5.0, 12.0])
+def test_scores_far_apart(gpu, heads, kvh, hd, seqs, size):
+    """As over f16 pages: what the weights are taken against rises and falls; the RMS error stays that of an f32 evaluation."""
+    sc = MxScene([1] * seqs, [1500, 700] + [80] * (seqs - 2), heads, kvh, hd, 16, seed=int(size))
+    sc.q *= np.float32(size)
+    for at in (5, 130, 131, 400):
+        page, slot = sc.places(0, 600)[at]
+        sc.k32[page, :, slot] *= 2.5
+    sc.settle()
+    plain = sc.plain()
+    at = P.sample(plain, 150)
+    ref = P.exact(plain, at)
+    out = _attend(sc, single=True).reshape(sc.total, sc.heads, sc.hd)
+    err = P.rms(np.array([out[a] for a in at]) - ref)
+    assert err <= P.allowed(plain, at, ref), f"{err / P.allowed(plain, at, ref):.3g} of what is allowed"
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("seqs", [3, 70])
+def test_no_numbers_in_single_rows(gpu, hd, seqs):
+    """A NaN block of a value spoils its 32 components of that sequence, a NaN key its row; no other sequence feels it."""
+    sc = MxScene([1] * seqs, [700] + [90] * (seqs - 1), 4, 2, hd, 16, seed=7)
+    page, slot = sc.places(0, 700)[333]
+    sc.v32[page, :, slot, :32] = np.nan
+    page1, slot1 = sc.places(1, 90)[17]
+    sc.k32[page1, :, slot1, -5] = np.inf
+    sc.settle()
+    out = _attend(sc, single=True).reshape(seqs, 4, hd)
+    sc.v32[page, :, slot, :32] = 0.0
+    ref, bound = (x.reshape(seqs, 4, hd) for x in sc.plain().attention())
+    assert np.isnan(out[0, :, :32]).all() and np.isnan(out[1]).all()
+    assert (np.abs(out[0] - ref[0])[:, 32:] <= bound[0][:, 32:]).all()
+    assert (np.abs(out[2:] - ref[2:]) <= bound[2:]).all()
+
+
+def test_no_queries(gpu):
+    """Queries of zero weigh all positions alike; queries that are no numbers spoil their own row and head alone."""
+    sc = MxScene([1] * 4, [700, 90, 5, 64], 8, 2, 64, 16, seed=8)
+    sc.q[0] = 0.0
+    sc.q[1, 64 + 3] = np.nan
+    sc.q[3, 7 * 64] = np.inf
+    out = _attend(sc, single=True).reshape(4, 8, 64)
+    sc.q[1, 64 + 3] = sc.q[3, 7 * 64] = 0.0
+    ref, bound = (x.reshape(4, 8, 64) for x in sc.attention())
+    fine = np.ones((4, 8), bool)
+    fine[1, 1] = fine[3, 7] = False
+    assert np.isnan(out[1, 1]).all()
+    assert (np.abs(out - ref)[fine] <= bound[fine]).all()
+
+
+def test_single_rows_same_bits(gpu):
+    """No sum's order depends on which workgroup ends first; alone or among others, in place or not."""
+    sc = MxScene([1] * 70, [3000, 900] + [60] * 68, 8, 2, 64, 16, seed=12)
+    call = Call(gpu, sc, single=True)
+    outs = []
+    for _ in range(4):
+        call.out.upload(np.zeros(call.out.shape, np.float32))
+        call()
+        outs.append(call.result()[0].copy())
+    assert all(np.array_equal(outs[0], o) for o in outs[1:])
+    call(in_place=True)
+    assert np.array_equal(call.result(call.q)[0], outs[0])
+    _check(sc, outs[0])

@@ -1,11 +1,13 @@
 """What the entry points refuse of MXFP4 pages and of gathering, and the pages' byte arithmetic on the host (no GPU)."""
 import ctypes as C
 import os
+import random
 import subprocess
 
 import numpy as np
 import pytest
 
+from test_paged_workspaces import LAYOUTS
 from test_paged_refusals import ARG, BAD_BATCH, BAD_CACHE, FORMAT, RANGE, ROOT, P, _append, _attention, _batch, _cache
 
 MX = 4
@@ -57,6 +59,34 @@ def test_wrapper_refuses(yl):
     for shape in ((2, 1, 16, 32), (2, 16, 34)):
         with pytest.raises(ValueError):
             ops._pool(np.zeros(shape, np.uint8), np.zeros(shape, np.uint8))
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_a_workspace_serves_smaller_batches(yl, layout):
+    """As test_paged_workspaces.py has it for the other types: no more sequences, rows, entries, positions and prefix."""
+    heads, kvh, hd = layout
+
+    def need_of(seqs, rows, pages, max_len, starts, prefix):
+        cache = yl.PagedCacheDesc(P, P, MX, 1 << 20, 16, kvh, hd)
+        batch = yl.PagedBatchDesc(seqs, rows, pages, max_len, P, P, P if starts else None, prefix, P if prefix else None)
+        return yl.lib().yl_paged_attention_workspace(C.byref(cache), C.byref(batch), heads)
+
+    r = random.Random(f"mx{layout}")
+    ln = lambda hi: int(round(hi ** r.random()))  # noqa: E731
+    for _ in range(60):
+        seqs, rows, pages, prefix = ln(3000), ln(12000), ln(3000), r.choice([0, 0, ln(9000)])
+        max_len = r.choice([0, ln(60000)])
+        most = need_of(seqs, rows, pages, max_len, True, prefix)
+        for _ in range(150):
+            edge = lambda hi, *at: min(hi, r.choice([hi, ln(hi), *at]))  # noqa: E731
+            n, q = edge(seqs, 1, 16, 17, 32, 200, 511, 512, 513), edge(rows, 1, 16, 128, 512, 600, 2400)
+            p, e = edge(prefix) if prefix and r.random() < 0.8 else 0, edge(pages, 40, 41, 128, 129)
+            ml = edge(max_len, 640, 641, 2048, 2049) if max_len else r.choice([0, ln(60000)])
+            starts = r.random() < 0.4
+            if not starts:
+                n = q = min(n, q)
+            need = need_of(n, q, e, ml, starts, p)
+            assert need <= most, (seqs, rows, pages, max_len, prefix, "|", n, q, e, ml, p, starts, need, most)
 
 
 HARNESS = r"""

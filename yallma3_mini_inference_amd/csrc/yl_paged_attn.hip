@@ -606,21 +606,6 @@ struct Tile {
     }
 };
 
-// A lane's part of 16 keys: its pieces, or of an MXFP4 row HD / 4 codes and their scale byte.
-template <int NK> struct KeyPieces { u4 f[NK]; };
-template <int HD> struct KeyCodes {
-    Words<HD / 32> codes;
-    uint32_t scale;
-    __device__ __forceinline__ void widen(u4 k[HD / 32]) const {
-        const float unit = mx_unit(scale);
-#pragma unroll
-        for (int i = 0; i < HD / 32; i++)
-            k[i] = u4{mx_pair<0>(codes.w[i], unit), mx_pair<1>(codes.w[i], unit), mx_pair<2>(codes.w[i], unit), mx_pair<3>(codes.w[i], unit)};
-    }
-};
-template <typename C, int HD> struct KeyOf { typedef KeyPieces<HD * sizeof(C) / 64> type; };
-template <int HD> struct KeyOf<Mx4, HD> { typedef KeyCodes<HD> type; };
-
 // A lane's part of four neighbouring positions' values in MXFP4: HD / 16 codes of
 // each, and the scale bytes of all.
 template <int HD> struct MxValues {
@@ -646,6 +631,22 @@ template <int HD> struct MxValues {
         }
     }
 };
+
+// A lane's part of 16 positions that is loaded a step ahead: its pieces of the
+// keys; of MXFP4 pages HD / 4 codes of a key and their scale byte, and the values.
+template <int HD> struct KeyCodes {
+    Words<HD / 32> codes;
+    uint32_t scale;
+    MxValues<HD> values;
+    __device__ __forceinline__ void widen(u4 k[HD / 32]) const {
+        const float unit = mx_unit(scale);
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++)
+            k[i] = u4{mx_pair<0>(codes.w[i], unit), mx_pair<1>(codes.w[i], unit), mx_pair<2>(codes.w[i], unit), mx_pair<3>(codes.w[i], unit)};
+    }
+};
+template <typename C, int HD> struct KeyOf { typedef u4 type[HD * sizeof(C) / 64]; };
+template <int HD> struct KeyOf<Mx4, HD> { typedef KeyCodes<HD> type; };
 
 // Clears values that are not there, and among positions that not every row
 // attends to those that are no numbers; true if there was one of the latter.
@@ -804,10 +805,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
                 const char* k = static_cast<const char*>(a.p.keys) + block;
                 f[t].codes = load_words<HD / 32>(k + slot * (HD / 2) + g * (HD / 8));
                 f[t].scale = (uint8_t)k[(HD / 2 << a.p.page_shift) + slot * (HD / 32) + g * HD / 128];
+                f[t].values.load(static_cast<const char*>(a.p.values) + block, slot - c + 4 * g, HD / 2 << a.p.page_shift, c);
             } else {
             const C* k = keys + paged_offset(a.p, max(page[t], 0), kvh, (lo + STEP * step + 16 * t) & slots) + (size_t)c * HD + R::KE * g;
 #pragma unroll
-            for (int i = 0; i < NK; i++) f[t].f[i] = *reinterpret_cast<const u4*>(k + i * R::KD);
+            for (int i = 0; i < NK; i++) f[t][i] = *reinterpret_cast<const u4*>(k + i * R::KD);
             }
         }
     };
@@ -816,15 +818,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
         // values of this step, keys of the next (the next step's values too
         // measured the same or, with a wavefront per SIMD fewer, slower)
         typename R::Value vr[NT][4];
-        MxValues<HD> vx[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            if constexpr (R::MX) {
-                const size_t block = ((size_t)max(page[t], 0) * a.p.n_kv + kvh) * paged_mx_block(a.p);
-                const int slot = ((lo + STEP * step + 16 * t) & slots) + 4 * g;
-                vx[t].load(static_cast<const char*>(a.p.values) + block, slot, HD / 2 << a.p.page_shift, c);
-                continue;
-            }
+            if constexpr (R::MX) continue;
             const C* v = values + paged_offset(a.p, max(page[t], 0), kvh, ((lo + STEP * step + 16 * t) & slots) + 4 * g) + (size_t)c * NJ;
 #pragma unroll
             for (int i = 0; i < 4; i++) vr[t][i] = load_words<R::VW>(v + (size_t)i * HD);
@@ -845,14 +841,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) vx[t].widen(i, vr[t][i].w, c);
+                for (int i = 0; i < 4; i++) kc[t].values.widen(i, vr[t][i].w, c);
         } else {
-            u4 kw[NT][NK];
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int i = 0; i < NK; i++) kw[t][i] = kc[t].f[i];
-            r.scores(kw, s);
+            r.scores(kc, s);
         }
         const int p0 = lo + STEP * step;
         bool edge = p0 + STEP > min(least, hi), odd = false;
@@ -912,6 +903,370 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
         for (int k = 0; k < NJ; k++) dst[k] = o[k];
         // (NaN scores alone leave the reference at -inf: 0 marks the part as there)
         if ((tid & 15) == 0) a.pml[at] = make_float2(M == -INFINITY && L != 0.0f ? 0.0f : M, L);
+    }
+}
+
+// One row per sequence and up to four query heads per kv head over MXFP4 pages:
+// 4 x 4 x 4 products, of which a wavefront computes 16 at once.  16 x 16 tiles are
+// three quarters empty here, and pages of 4 bits are read so fast that the
+// instructions count: of the scores of 64 positions a lane has 4, not 16, and all of
+// a key, or of a quarter of four values, stands in one lane.  Lane (block b, n):
+//   scores: key of position 4b + n (A) times q's dimensions of row n (B) -> row n,
+//           positions 4b .. 4b + 3;
+//   output: quarter n of the values of positions 4b .. 4b + 3 (A) times row n's
+//           weights (B, the scores' registers) -> row n, dimensions i HD / 4 + j; the 16
+//           blocks are added up once, at the end.
+// f16 parts of q and the weights as over f16 caches.  The codes are widened to f16
+// against an exponent: of a key, its own largest scale, which goes back into its
+// score; of the values, one that the wavefront raises when scales pass it, the sums
+// following.  What is below 2^-35 of the largest is lost by that: of a key's other
+// blocks, of the values of the other positions.
+// Bound by vector instructions (some 220 for 64 positions of hd 64, 380 of hd 128,
+// and as many again in a unit's first and last part) and the latency of its few
+// steps: two rows at 128,000 positions, 32 heads on 8, hd 64: 32 us, 4.4 TB/s of 17/32
+// byte an element (the row kernel's 16-row tiles 47); 64 rows at 100 .. 8000, hd 128:
+// 46 us, 3.7 TB/s (52).  Measured and dropped: q's parts in registers (spills), one
+// buffer of keys and values for the two (hd 64 168 registers or 128, 44 us), even
+// shares of all positions that cross sequences (67 us: each takes a unit's first and
+// last part in turn).
+template <int HD> struct FewStep {
+    static constexpr int NB = HD / 32;                    // blocks of a head
+    Words<HD / 8> k;
+    uint32_t ke;                                          // the key's scale bytes
+    Words<HD / 32> v[4];
+    Words<HD / 32> ve;                                    // the four values'
+    // page: of the lane's position, its first's where there is none; slot: its slot
+    static __device__ __forceinline__ size_t block_of(const PagedArgs& p, int page, int kvh) {
+        // (a page's bytes fit 32 bits: one multiplication)
+        const uint32_t head = (uint32_t)paged_mx_block(p);
+        return (uint64_t)(uint32_t)max(page, 0) * (head * (uint32_t)p.n_kv) + (uint64_t)head * (uint32_t)kvh;
+    }
+    __device__ __forceinline__ void load_key(const PagedArgs& p, size_t block, int slot) {
+        const char* kb = static_cast<const char*>(p.keys) + block;
+        k = load_words<HD / 8>(kb + slot * (HD / 2));
+        const char* e = kb + (HD / 2 << p.page_shift) + slot * NB;
+        if constexpr (NB == 1) ke = (uint8_t)*e;
+        else if constexpr (NB == 2) ke = *reinterpret_cast<const uint16_t*>(e);
+        else ke = *reinterpret_cast<const uint32_t*>(e);
+    }
+    __device__ __forceinline__ void load_values(const PagedArgs& p, size_t block, int slot, int n) {
+        const char* vb = static_cast<const char*>(p.values) + block;
+        const int first = slot & ~3;
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = load_words<HD / 32>(vb + (first + i) * (HD / 2) + n * (HD / 8));
+        ve = load_words<HD / 32>(vb + (HD / 2 << p.page_shift) + first * NB);
+    }
+    __device__ __forceinline__ uint32_t key_scale(int b) const { return (ke >> (8 * b)) & 255u; }
+    // scale byte of position i, at the bits of an exponent
+    __device__ __forceinline__ int value_unit(int i, int n) const {
+        const uint32_t at = 8 * (i * NB % 4) + 8 * (n * NB / 4);
+        return (int)(((ve.w[i * NB / 4] >> at) & 255u) << 23);
+    }
+};
+
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ vf4 mul4(u2 a, u2 b, vf4 c) {
+    return __builtin_amdgcn_mfma_f32_4x4x4f16(__builtin_bit_cast(h4, a), __builtin_bit_cast(h4, b), c, 0, 0, 0);
+}
+// Byte I's two elements as packed f16.
+template <int I>
+__device__ __forceinline__ uint32_t half_pair(uint32_t codes, float unit) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, unit, I));
+}
+// over the 16 lanes of one n
+__device__ __forceinline__ float few_max(float v) {
+    v = fmaxf(v, dpp_mov<0x124>(v));                      // row_ror:4
+    v = fmaxf(v, dpp_mov<0x128>(v));                      // row_ror:8
+    return group_max16(v);
+}
+__device__ __forceinline__ float few_sum(float v) {
+    v += dpp_mov<0x124>(v);
+    v += dpp_mov<0x128>(v);
+    return group_sum16(v);
+}
+
+// W wavefronts deal the steps of a unit among themselves.
+template <int HD, int W>
+__global__ __launch_bounds__(64 * W, HD == 128 ? 2 : 3) void k_paged_attn_few(PagedAttn a) {
+    using T = Type<_Float16>;
+    constexpr int STEP = 64, K4 = HD / 4, NB = HD / 32;
+    constexpr int LD = HD + 4;
+    __shared__ __align__(16) float so[W][4][LD];
+    __shared__ float sm[W][4], sl[W][4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 3, b = lane >> 2;
+    const int kvh = blockIdx.x % a.p.n_kv, slot = blockIdx.x / a.p.n_kv;
+    Unit u{slot, 0, 0, 1, 0, slot};
+    if (a.wanted) {
+        if (!unit_of(a, slot, &u)) return;
+        if (a.joined && slot == u.first && kvh == 0 && tid == 0) a.units[u.seq] = make_int4(u.first, u.splits, 0, 0);
+    }
+    const RowSet set = set_of_seq(a.p, u.seq);
+    const int row = set.first;
+    const bool direct = a.direct && u.splits == 1;
+    const int64_t held = (int64_t)set.entries << a.p.page_shift;
+    const int begin = (int)min((int64_t)u.split * u.chunk, held);
+    // The table's entry of a position, as it is (looking at it now would wait for
+    // everything in flight), of the last position where there is none.
+    const auto entry_at = [&](int pos, int end) { return end > 0 ? set.pages[min(pos, end - 1) >> a.p.page_shift] : -1; };
+    // (the first steps' before the length is known: one round trip less)
+    int entry = entry_at(begin + STEP * wave + lane, (int)held), entry1 = entry_at(begin + STEP * (wave + W) + lane, (int)held);
+    // q in parts, a piece of row n per lane at a time; every wavefront needs its exponent
+    __shared__ __align__(16) u4 sq[K4][4];
+    int ex;
+    {
+        constexpr int P = (K4 + 15) / 16;
+        const float* qr = a.q + (size_t)row * a.q_ld + (size_t)(kvh * a.group + (n < a.group ? n : 0)) * HD;
+        f4u x[P];
+        float amax = 0.0f;
+#pragma unroll
+        for (int k = 0; k < P; k++) {
+            x[k] = f4u{0.0f, 0.0f, 0.0f, 0.0f};
+            if (n < a.group && 16 * k + b < K4) x[k] = *reinterpret_cast<const f4u*>(qr + 4 * (16 * k + b));
+#pragma unroll
+            for (int i = 0; i < 4; i++) amax = fmaxf(amax, fabsf(x[k][i]));
+        }
+        ex = T::exponent(few_max(amax) * fabsf(a.scale));
+#pragma unroll
+        for (int k = 0; k < P; k++) {
+            uint32_t part[2][2];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                T::cut(__builtin_amdgcn_ldexpf(x[k][2 * h] * a.scale, ex), __builtin_amdgcn_ldexpf(x[k][2 * h + 1] * a.scale, ex), part[h]);
+            if (wave == 0 && 16 * k + b < K4) sq[16 * k + b][n] = u4{part[0][0], part[1][0], part[0][1], part[1][1]};
+        }
+    }
+    __syncthreads();
+    constexpr int kKeyBits = 12;                          // a key's largest unit in f16: 6 * 2^12
+    const float unscale = __builtin_amdgcn_ldexpf(1.0f, min(max(a.scale_exp - ex - kKeyBits, -126), 127));
+    const int lim = (int)min((int64_t)limit_of_row(a, set, row), held);
+    const int lo = min(begin, lim), hi = u.splits > 1 && lim - lo > u.chunk ? lo + u.chunk : lim;
+    const size_t part0 = ((size_t)slot * a.p.n_kv + kvh) * kRowTile;
+    if (lo >= hi && !direct) {
+        if (tid < a.group) a.pml[part0 + tid] = make_float2(-INFINITY, 0.0f);
+        return;
+    }
+    const int steps = (hi - lo + STEP - 1) / STEP, slots = (1 << a.p.page_shift) - 1;
+
+    vf4 acc[K4];
+#pragma unroll
+    for (int j = 0; j < K4; j++) acc[j] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    int vref = 0, vlimit = -1;                            // the values' exponent; scales above the limit raise it
+    const auto position = [&](int step) { return lo + STEP * step + lane; };
+    const int end = (hi + 3) & ~3;                        // four positions stand together: of one page, looked at by four lanes
+    FewStep<HD> x, y;                                     // this step's, the next one's
+    int page = -1;
+    float s[4];
+    int vu[4];
+    int then_page = -1;
+    // Scores of a step, the next one's keys and values on their way; whether
+    // a weight, or a value's scale, is out of its range.
+    const auto score = [&](int step, bool more) {
+        if (more) {
+            // (the entry after next before the next step's loads: what waits for it does not wait for them)
+            const int pos = position(step + W), later = entry_at(pos + STEP * W, end);
+            then_page = pos < end ? paged_page(entry1, a.p.n_pages) : -1;
+            entry1 = later;
+            const size_t block = FewStep<HD>::block_of(a.p, then_page, kvh);
+            y.load_key(a.p, block, pos & slots);
+            y.load_values(a.p, block, pos & slots, n);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        uint32_t top = x.key_scale(0);
+#pragma unroll
+        for (int k = 1; k < NB; k++) top = max(top, x.key_scale(k));
+        vf4 dh{0.0f, 0.0f, 0.0f, 0.0f}, dl = dh;
+        float unit[NB];
+#pragma unroll
+        for (int k = 0; k < NB; k++) unit[k] = mx_unit((uint32_t)max((int)x.key_scale(k) - (int)top + 127 + kKeyBits, 0));
+#pragma unroll
+        for (int w = 0; w < HD / 8; w++) {
+            const float un = unit[w / 4];
+            const u2 lower{half_pair<0>(x.k.w[w], un), half_pair<1>(x.k.w[w], un)}, upper{half_pair<2>(x.k.w[w], un), half_pair<3>(x.k.w[w], un)};
+            const u4 q0 = sq[2 * w][n], q1 = sq[2 * w + 1][n];
+            dl = mul4(lower, u2{q0[2], q0[3]}, dl);
+            dh = mul4(lower, u2{q0[0], q0[1]}, dh);
+            dl = mul4(upper, u2{q1[2], q1[3]}, dl);
+            dh = mul4(upper, u2{q1[0], q1[1]}, dh);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // (a scale of 255 is NaN)
+        const float factor = __uint_as_float(top == 255u ? 0x7fc00000u : top << 23);
+        s[0] = (dh[0] + dl[0]) * (dpp_mov<0x00>(factor) * unscale);
+        s[1] = (dh[1] + dl[1]) * (dpp_mov<0x55>(factor) * unscale);
+        s[2] = (dh[2] + dl[2]) * (dpp_mov<0xAA>(factor) * unscale);
+        s[3] = (dh[3] + dl[3]) * (dpp_mov<0xFF>(factor) * unscale);
+#pragma unroll
+        for (int i = 0; i < 4; i++) vu[i] = x.value_unit(i, n);
+        // what is not there: no weight, and values of zero (a garbage scale may be NaN)
+        const int p0 = lo + STEP * step;
+        if (p0 + STEP > hi || __ballot(page < 0)) {
+            const int left = hi - p0 - 4 * b;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (i >= left || page < 0) { s[i] = -INFINITY; vu[i] = 0; }
+        }
+        const float above = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])) - m;
+        return __ballot(!(above >= T::kLeast && above <= T::kMost) || max(max(vu[0], vu[1]), max(vu[2], vu[3])) > vlimit) != 0;
+    };
+    // Brings them into it: the weights' reference as in Tile::weigh, the values' exponent.
+    const auto adjust = [&] {
+            const float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+            const float high = few_max(mx);
+            float to = fmaxf(m, high - T::kBias);
+            if (high - to > T::kMost) to = high;
+            const int room = max(T::kRoom - __builtin_amdgcn_frexp_expf(few_sum(l)), 0);
+            if (high - m < T::kLeast && high > -INFINITY && fabsf(m) < 0x1p20f) to = fmaxf(high - T::kFall, m - (float)room);
+            float alpha = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+            l *= alpha;
+            m = to;
+            int e = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) e = max(e, vu[i] == 0x7f800000 ? 0 : vu[i] >> 23);
+            e = max16(e);
+            e = max(e, __shfl_xor(e, 16, 64));
+            e = __builtin_amdgcn_readfirstlane(max(e, __shfl_xor(e, 32, 64)));
+            const int vto = (e << 23) > max(vlimit, 0) ? e - 8 : vref;
+            alpha *= __builtin_amdgcn_ldexpf(1.0f, max(vref - vto, -126));      // (before the first values: of zeros)
+            vlimit = vto != vref || vlimit >= 0 || e > 0 ? min(vto + 13, 254) << 23 : -1;
+            vref = vto;
+#pragma unroll
+            for (int j = 0; j < K4; j++) acc[j] *= alpha;
+#pragma unroll
+            for (int i = 0; i < 4; i++) vu[i] = (int)((uint32_t)vu[i] + (vu[i] == 0x7f800000 ? (uint32_t)(vref - 127) << 23 : 0u));
+    };
+    // Adds the weighted values.
+    const auto add = [&](bool more) {
+        {
+            const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                s[i] = __builtin_amdgcn_exp2f(s[i] - ref);
+                l += s[i];
+            }
+        }
+        float uf[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) uf[i] = __int_as_float(max((int)((uint32_t)vu[i] - ((uint32_t)(vref - 127) << 23)), 0));
+        uint32_t lowp[2], highp[2];
+        {
+            uint32_t part[2];
+            T::cut(s[0], s[1], part);
+            lowp[0] = part[1]; highp[0] = part[0];
+            T::cut(s[2], s[3], part);
+            lowp[1] = part[1]; highp[1] = part[0];
+        }
+        const u2 ph{highp[0], highp[1]};
+        u2 parts[2]{ph, u2{lowp[0], lowp[1]}};
+        T::settle(parts);
+        const u2 pl = parts[1];
+        const auto two = [&](int j, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) {
+            const u2 even{__builtin_amdgcn_perm(v1, v0, 0x05040100), __builtin_amdgcn_perm(v3, v2, 0x05040100)};
+            const u2 odd{__builtin_amdgcn_perm(v1, v0, 0x07060302), __builtin_amdgcn_perm(v3, v2, 0x07060302)};
+            // (as assembly, so that the sums stay in their registers: left to itself the
+            // compiler copies them in every step.  Waits: two states behind the operands'
+            // writes, two between products of one sum; nothing else reads or
+            // writes the sums within a step.)
+            asm("s_nop 1\n\t"
+                "v_mfma_f32_4x4x4_16b_f16 %0, %2, %4, %0\n\t"
+                "v_mfma_f32_4x4x4_16b_f16 %1, %3, %4, %1\n\t"
+                "s_nop 0\n\t"
+                "v_mfma_f32_4x4x4_16b_f16 %0, %2, %5, %0\n\t"
+                "v_mfma_f32_4x4x4_16b_f16 %1, %3, %5, %1"
+                : "+v"(acc[j]), "+v"(acc[j + 1])
+                : "v"(even), "v"(odd), "v"(pl), "v"(ph));
+        };
+#pragma unroll
+        for (int w = 0; w < HD / 32; w++) {
+            two(8 * w, half_pair<0>(x.v[0].w[w], uf[0]), half_pair<0>(x.v[1].w[w], uf[1]), half_pair<0>(x.v[2].w[w], uf[2]), half_pair<0>(x.v[3].w[w], uf[3]));
+            two(8 * w + 2, half_pair<1>(x.v[0].w[w], uf[0]), half_pair<1>(x.v[1].w[w], uf[1]), half_pair<1>(x.v[2].w[w], uf[2]), half_pair<1>(x.v[3].w[w], uf[3]));
+            two(8 * w + 4, half_pair<2>(x.v[0].w[w], uf[0]), half_pair<2>(x.v[1].w[w], uf[1]), half_pair<2>(x.v[2].w[w], uf[2]), half_pair<2>(x.v[3].w[w], uf[3]));
+            two(8 * w + 6, half_pair<3>(x.v[0].w[w], uf[0]), half_pair<3>(x.v[1].w[w], uf[1]), half_pair<3>(x.v[2].w[w], uf[2]), half_pair<3>(x.v[3].w[w], uf[3]));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) {
+            x = y;
+            page = then_page;
+        }
+    };
+    if (wave < steps) {
+        const int pos = position(wave);
+        page = pos < end ? paged_page(entry, a.p.n_pages) : -1;
+        const size_t block = FewStep<HD>::block_of(a.p, page, kvh);
+        x.load_key(a.p, block, pos & slots);
+        x.load_values(a.p, block, pos & slots, n);
+        // (a loop of the steps that need no adjustment inside one of those that do:
+        // as a branch in one loop, the compiler copies all sums in every step)
+        int step = wave;
+        bool out = score(step, step + W < steps);
+        for (;;) {
+            if (out) adjust();
+            do {
+                add(step + W < steps);
+                step += W;
+                if (step >= steps) break;
+                out = score(step, step + W < steps);
+            } while (!out);
+            if (step >= steps) break;
+        }
+    }
+
+    // (the last products are written)
+    asm volatile("s_nop 7\n\ts_nop 7" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < K4; j++) asm volatile("" : "+v"(acc[j]));
+    // the blocks' sums together: halves of the wavefront, then pairs of 16 lanes
+    // exchange half of their registers, so that 16 lanes have a quarter of the dimensions
+    float r[HD / 4];
+    {
+        float x[HD];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < K4; j++) x[i * K4 + j] = acc[j][i];
+#pragma unroll
+        for (int i = 0; i < HD / 2; i++) {
+            const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[i]), __float_as_uint(x[i + HD / 2]), false, false);
+            x[i] = __uint_as_float(t[0]) + __uint_as_float(t[1]);
+        }
+#pragma unroll
+        for (int i = 0; i < HD / 4; i++) {
+            const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[i]), __float_as_uint(x[i + HD / 4]), false, false);
+            float v = __uint_as_float(t[0]) + __uint_as_float(t[1]);
+            v += dpp_mov<0x124>(v);
+            v += dpp_mov<0x128>(v);
+            r[i] = v;
+        }
+    }
+    l = few_sum(l);
+    {
+        const int rr = lane >> 4, q = b & 3;              // which quarter of the dimensions; which part of it to write
+        const int at = (rr & 1) * (HD / 4) + (rr >> 1) * (HD / 2);
+#pragma unroll
+        for (int i = 0; i < HD / 4; i++)
+            if (i / (HD / 16) == q) so[wave][n][at + i] = __builtin_amdgcn_ldexpf(r[i], vref - 127);
+        if (lane < 4) { sm[wave][n] = m; sl[wave][n] = l; }
+    }
+    __syncthreads();
+    for (int i = tid; i < a.group * HD; i += 64 * W) {
+        const int tr = i / HD, e = i % HD;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < W; w++) M = fmaxf(M, sm[w][tr]);
+        float L = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            const float f = sm[w][tr] == M ? 1.0f : __builtin_amdgcn_exp2f(sm[w][tr] - M);
+            L = fmaf(sl[w][tr], f, L);
+            o = fmaf(so[w][tr][e], f, o);
+        }
+        if (direct) {
+            a.out[(size_t)row * a.out_ld + (size_t)(kvh * a.group + tr) * HD + e] = o * (L != 0.0f ? 1.0f / L : 0.0f);
+        } else {
+            a.po[(part0 + tr) * HD + e] = o;
+            if (e == 0) a.pml[part0 + tr] = make_float2(M == -INFINITY && L != 0.0f ? 0.0f : M, L);
+        }
     }
 }
 
@@ -1233,6 +1588,7 @@ struct AttnPlan {
     int per = 1, wanted = 0, max_units = 0;          // row kernel, own pages (PagedAttn)
     float finer = 0.0f;
     bool split = false, join_rows = false, both = false;
+    int few = 0;                                     // wavefronts of k_paged_attn_few (0: the row kernel)
     int per_seq = 0;                                 // joining only what the row kernel took: rows of a sequence
     int tile_groups = 0;                             // tile kernel, own pages (not split): row tiles
     Launch prefix;
@@ -1285,6 +1641,26 @@ size_t bytes_of(const PagedArgs& p, size_t row_units, size_t all_units) {
     return bytes ? ((bytes + 15) & ~(size_t)15) + (size_t)p.n_seqs * sizeof(int4) : 0;
 }
 
+// One row per sequence over MXFP4 pages (k_paged_attn_few): sequences times kv
+// heads from which on a wavefront takes a unit alone, where positions are split.
+// 32 heads on 8, in us, row kernel | four wavefronts a unit | one:
+//   2 sequences of 128,000, hd 64                 50 |  39 |  47
+//   16 of 100 .. 8000, hd 128                     26 |  29 |  23
+//   64 of them, hd 64 (hd 128)            39 (57)    |  34 (55) |  29 (51)
+//   200 of them, hd 64                            80 |  74 |  67
+//   500 of 100 .. 3000, hd 128                   217 | 204 | 147
+// Where they are not split: four wavefronts below kFewShort, the row kernel
+// (whose steps are half as long) below kFewMany, one wavefront from there on; four
+// for more than kDivided sequences that may be long (600 of 200 .. 8000: 233 | 186 | 244).
+//   one of 600, hd 64                            8.4 | 7.8 | 14.2
+//   30 of 100 .. 600, hd 64                      8.6 | 8.0 | 14.6
+//   100 of 20 .. 600, hd 64                     10.4 | 11.9 | 15.1
+//   300 of them, hd 128                           41 |  43 |  34
+//   1500 of them, hd 64                           81 |  94 |  52
+constexpr int kFewAlone = 128, kFewShort = 256, kFewMany = 1600;
+// Units wanted of them (hd 64, 64 sequences of 100 .. 8000 in 1024 | 2048 | 3072: 41 | 33 | 29 us; 16 of them, hd 128: 24 | 26 | 31).
+constexpr int kFewLeast = 1024, kFewMost = 3072;
+
 // Workgroups of the tile kernel that run at once (their registers).
 int tile_resident(const PagedArgs& p) { return p.hd == 128 ? 256 : 512; }
 
@@ -1315,13 +1691,23 @@ AttnPlan plan_attention(const PagedArgs& p, int dtype, uint32_t max_len) {
     const int64_t tiles = !p.row_start          ? (int64_t)p.n_seqs * r.per
                           : r.both && !search ? std::min<int64_t>((int64_t)p.n_seqs * (kRowKernelRows / kRowTile), slots)
                                               : slots;
-    r.wanted = r.split ? std::max(1, 512 / p.n_kv) : p.row_start && !search ? 1 : 0;
+    // one row per sequence over MXFP4 pages: how many wavefronts share a unit
+    const int64_t few_units = (int64_t)p.n_seqs * p.n_kv;
+    if (dtype == YL_T_MXFP4 && !p.row_start && group <= 4)
+        r.few = r.split                                  ? (few_units < kFewAlone ? 4 : 1)
+                : own > kUnsplit                         ? 4
+                : few_units < kFewShort                  ? 4
+                : few_units < kFewMany                   ? 0
+                                                         : 1;
+    const int workgroups = r.few == 1 ? (int)std::clamp<int64_t>(8 * few_units, kFewLeast, kFewMost) : 512;
+    r.wanted = r.split ? std::max(1, workgroups / p.n_kv) : p.row_start && !search ? 1 : 0;
     // One row per sequence: lengths differ, tiles of more than half the mean are
     // split (64 sequences of 100 .. 8000 139 -> 134 us; 128, hd 64, 98 against 102
     // for those above the mean), those above the mean where there are workgroups
     // enough (512 sequences 380 -> 373, of 100 .. 3000 232 -> 210).  Rows of
     // prompts: tiles of one length, which stay whole where there are many.
     r.finer = p.row_start ? 0.95f : tiles * p.n_kv >= kEnough ? 1.0f : 2.0f;
+    if (r.few) r.finer = 2.0f;
     r.max_units = (int)(tiles + std::max<int64_t>(r.wanted, r.split ? (int64_t)std::ceil(r.finer * (float)tiles) + 1 : 0));
     r.join_rows = r.split || p.prefix_len;
     if (r.both) r.tile_groups = (int)(stacked / R) + p.n_seqs;
@@ -1365,6 +1751,7 @@ size_t bytes_at_most(const PagedArgs& p, int dtype, uint32_t max_len) {
         const int64_t single = std::min<int64_t>(seqs, p.n_rows) * ((group + kRowTile - 1) / kRowTile);
         const int64_t few = std::min<int64_t>(single, (kEnough - 1) / p.n_kv);
         units = std::max({units, single + std::max(wanted, finer(1.0f, single)), few + finer(2.0f, few)});
+        if (dtype == YL_T_MXFP4) units = std::max(units, single + std::max<int64_t>(kFewMost / p.n_kv, finer(2.0f, single)));
     }
     size_t all = 0;
     if (p.prefix_len) {
@@ -1414,7 +1801,17 @@ hipError_t launch_all(PagedAttn a, const AttnPlan& plan, float* space, hipStream
     a.direct = !a.p.prefix_len;
     a.joined = plan.join_rows;
     a.chunk = plan.split ? kLeastChunk : 1 << 30;
-    hipError_t e = launch_attn<C>(a, dim3((unsigned)plan.max_units * a.p.n_kv), false, false, s);
+    hipError_t e = hipSuccess;
+    if (kMx<C> && plan.few) {
+        const bool one = plan.few == 1;
+        auto k = a.p.hd == 32   ? (one ? k_paged_attn_few<32, 1> : k_paged_attn_few<32, 4>)
+                 : a.p.hd == 64 ? (one ? k_paged_attn_few<64, 1> : k_paged_attn_few<64, 4>)
+                                : (one ? k_paged_attn_few<128, 1> : k_paged_attn_few<128, 4>);
+        hipLaunchKernelGGL(k, dim3((unsigned)plan.max_units * a.p.n_kv), dim3(one ? 64 : 256), 0, s, a);
+        e = hipGetLastError();
+    } else {
+        e = launch_attn<C>(a, dim3((unsigned)plan.max_units * a.p.n_kv), false, false, s);
+    }
     a.po = all_po; a.pml = all_ml;
     a.parts = plan.tile_parts + plan.prefix.splits;
     if (e == hipSuccess && plan.both) {
