@@ -375,3 +375,47 @@ def test_branches_attend_as_their_parents(gpu, dtype):
     assert used == len(set(t.page_table[t.page_table >= 0])) < base.n_pages and t.page_table.max() == used - 1
     again = ops.paged_attention(*moved[0], ops.PagedBatch(t.page_table[n:], want[n:]), q2, heads, base.scale)
     assert np.array_equal(again, out)
+
+
+@pytest.mark.parametrize("n_pages", [1, 1023, 1024, 1025, 4096, 4097, 16384, 16385, 40000])
+def test_forks_and_moves_in_pools_of_any_size(gpu, n_pages):
+    """Both sides of the sizes from which on pools are looked through in another way; the free pages scattered."""
+    from yallma3_mini_inference_amd import ops
+    rng = np.random.default_rng(n_pages)
+    used = rng.permutation(n_pages)[:n_pages // 2]
+    table = np.full((12, max(1, len(used) // 6)), -1)
+    lens = np.zeros(12, int)
+    refs = np.zeros(n_pages, int)
+    for s, pages in enumerate(np.array_split(used, 6)):
+        pages = pages[:table.shape[1]]
+        table[s, :len(pages)] = pages
+        refs[pages] = 1
+        lens[s] = max(0, 16 * len(pages) - s * 3)
+    layers = [(rng.integers(0, 1 << 15, (n_pages, 1, 16, 32)).astype(np.uint16).view(np.float16), rng.integers(0, 1 << 15, (n_pages, 1, 16, 32)).astype(np.uint16).view(np.float16))]
+    m = Pages(table, lens, refs, 16, layers)
+    parents, children = [0, 1, 2, 3, 4, 5], [6, 7, 8, 9, 10, 11]
+    t = _tables(ops, m)
+    lacking, got = ops.paged_fork(t, m.layers, parents, children)
+    assert lacking == m.fork(parents, children)
+    _same(t, m, got)
+    ops.paged_release(t, [1, 4, 9])
+    m.release([1, 4, 9])
+    used, got = ops.paged_compact(t, got)
+    assert used == m.compact()
+    _same(t, m, got)
+
+
+@pytest.mark.parametrize("n", [1, 1024, 1025, 5000])
+def test_many_forks(gpu, n):
+    """More children than threads look at one each; not pages enough for all."""
+    from yallma3_mini_inference_amd import ops
+    rng = np.random.default_rng(n)
+    n_pages = 3 * n // 2 + 3
+    layers = [tuple(_pool(rng, "f16", n_pages, 1, 16, 32) for _ in range(2))]
+    m = _made(rng, [16 * (1 + i % 3) + i % 16 for i in range(max(1, n // 5))], n // 5 + 1 + n, 4, n_pages, 16, layers)
+    parents = rng.integers(0, max(1, n // 5), n)
+    children = max(1, n // 5) + rng.permutation(n)
+    t = _tables(ops, m)
+    lacking, got = ops.paged_fork(t, m.layers, parents, children)
+    assert lacking == m.fork(parents, children)
+    _same(t, m, got)

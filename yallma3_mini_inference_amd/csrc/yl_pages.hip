@@ -167,6 +167,19 @@ __global__ __launch_bounds__(256) void k_pages_list(TableArgs t, Space sp, int n
     }
 }
 
+// Page p, which `before` used pages precede, where `used` are in use: the j-th used page
+// (from 0) moves if its id is not below `used`; the movers are the last kMoved of
+// the ranks, and meet the free ids below `used` in order.
+__device__ __forceinline__ void move_page(const Space& sp, int p, bool is, int before, int used) {
+    if (p == used) sp.meta[kMoved] = used - before;
+    if (p >= used) {
+        sp.rank[p] = is ? before : -1;
+        if (is) sp.list[before] = p;
+    } else if (!is) {
+        sp.holes[p - before] = p;
+    }
+}
+
 // ---------------------------------------------------------------- reserving
 
 // A wavefront per sequence fills the entries that name no page, in their order.
@@ -190,6 +203,106 @@ __global__ __launch_bounds__(256) void k_pages_reserve(TableArgs t, Space sp, co
         lacks += __builtin_popcountll(__ballot(missing && r >= free_pages));
     }
     if (lane == 0 && lacks && lacking) atomicAdd(lacking, (uint32_t)lacks);
+}
+
+// -------------------------------------------------------------- small pools
+
+// One workgroup looks through up to kSmall things, C neighbouring ones per thread,
+// all of their loads in flight: a launch less than counting and listing, two less
+// than reserving.
+constexpr int kSmallThreads = 1024, kSmallMost = 16, kSmall = kSmallThreads * kSmallMost;
+
+// Ranks, in rising order, of those of n things that `is` picks from their values: put(index, rank).  Returns how many there are.
+template <int C, typename Load, typename Is, typename Put>
+__device__ __forceinline__ int rank_all(int n, const Load& load, const Is& is, const Put& put) {
+    const int at = threadIdx.x * C;
+    int v[C], mine = 0;
+#pragma unroll
+    for (int i = 0; i < C; i++) v[i] = n > 0 ? load(min(at + i, n - 1)) : 0;
+#pragma unroll
+    for (int i = 0; i < C; i++) mine += at + i < n && is(at + i, v[i]);
+    int total, rank = scan_group<kSmallThreads / 64>(mine, &total);
+#pragma unroll
+    for (int i = 0; i < C; i++)
+        if (at + i < n) {
+            const bool yes = is(at + i, v[i]);
+            put(at + i, yes ? rank : -1, rank);
+            rank += yes;
+        }
+    return total;
+}
+
+// What k_pages_count and k_pages_list leave for a fork.
+template <int C>
+__global__ __launch_bounds__(kSmallThreads) void k_pages_list_small(TableArgs t, Space sp, int items, const uint32_t* parents, const uint32_t* children,
+                                                                    uint32_t* lacking) {
+    if (threadIdx.x == 0 && lacking) *lacking = 0;
+    const int free_pages = rank_all<C>(t.n_pages, [&](int i) { return t.refs[i]; }, [](int, int r) { return r <= 0; },
+                                       [&](int i, int r, int) { if (r >= 0) sp.list[r] = i; });
+    if (threadIdx.x == 0) sp.meta[kFree] = free_pages;
+    rank_all<C>(items,
+                [&](int i) {
+                    int p, c, f, s, last;
+                    return (int)(fork_pair(t, parents, children, i, &p, &c, &f, &s, &last) && last >= 0);
+                },
+                [](int, int need) { return need != 0; }, [&](int i, int, int before) { sp.first[i] = before; });
+}
+
+// yl_paged_reserve: the entries that name no page, in the table's order, get the free pages.
+template <int C>
+__global__ __launch_bounds__(kSmallThreads) void k_pages_reserve_small(TableArgs t, const uint32_t* want_len, uint32_t* lacking) {
+    __shared__ int list[kSmallThreads * C];
+    __shared__ int past;
+    if (threadIdx.x == 0) past = 0;
+    const int free_pages = rank_all<C>(t.n_pages, [&](int i) { return t.refs[i]; }, [](int, int r) { return r <= 0; },
+                                       [&](int i, int r, int) { if (r >= 0) list[r] = i; });
+    __syncthreads();
+    for (int s = threadIdx.x; s < t.n_seqs; s += kSmallThreads) {
+        bool p;
+        table_entries(t, want_len[s], &p);
+        if (p) atomicAdd(&past, 1);
+    }
+    // (1: wanted and not there)
+    const int missing = rank_all<C>(t.n_seqs * t.max_pages,
+                                    [&](int i) {
+                                        bool p;
+                                        const int s = i / t.max_pages;
+                                        return (int)(i - s * t.max_pages < table_entries(t, want_len[s], &p) && paged_page(t.table[i], t.n_pages) < 0);
+                                    },
+                                    [](int, int is) { return is != 0; },
+                                    [&](int i, int r, int) {
+                                        if (r < 0 || r >= free_pages) return;
+                                        t.table[i] = list[r];
+                                        t.refs[list[r]] = 1;
+                                    });
+    __syncthreads();
+    if (threadIdx.x == 0 && lacking) *lacking = (uint32_t)(max(missing - free_pages, 0) + past);
+}
+
+// What k_pages_count and k_pages_moves leave for moving.
+template <int C>
+__global__ __launch_bounds__(kSmallThreads) void k_pages_moves_small(TableArgs t, Space sp, uint32_t* used_out) {
+    int used = 0;
+    {
+        const int at = threadIdx.x * C;
+        int v[C], mine = 0;
+#pragma unroll
+        for (int i = 0; i < C; i++) v[i] = t.refs[min(at + i, t.n_pages - 1)];
+#pragma unroll
+        for (int i = 0; i < C; i++) mine += at + i < t.n_pages && v[i] > 0;
+        int before = scan_group<kSmallThreads / 64>(mine, &used);
+#pragma unroll
+        for (int i = 0; i < C; i++)
+            if (at + i < t.n_pages) {
+                move_page(sp, at + i, v[i] > 0, before, used);
+                before += v[i] > 0;
+            }
+    }
+    if (threadIdx.x == 0) {
+        sp.meta[kFree] = used;
+        *used_out = (uint32_t)used;
+        if (used == t.n_pages) sp.meta[kMoved] = 0;
+    }
 }
 
 // ------------------------------------------------------------------ copying
@@ -274,9 +387,7 @@ __global__ __launch_bounds__(256) void k_pages_release(TableArgs t, const uint32
 
 // --------------------------------------------------------------- compacting
 
-// With `used` pages in use, the j-th of them (from 0) moves if its id is not below
-// `used`; the movers are the last kMoved of the ranks, and meet the free ids
-// below `used` in order.  Ranks of pages that move, -1 of free ones.
+// Ranks of pages that move, -1 of free ones; where they go.
 __global__ __launch_bounds__(256) void k_pages_moves(TableArgs t, Space sp, uint32_t* used_out) {
     const int groups = page_groups(t.n_pages), per = pages_per_group(t.n_pages), tid = threadIdx.x;
     int used;
@@ -292,15 +403,7 @@ __global__ __launch_bounds__(256) void k_pages_moves(TableArgs t, Space sp, uint
         const bool is = p < end && t.refs[p] > 0;
         int total;
         const int before = rank + scan_group<4>(is, &total);
-        if (p < end) {
-            if (p == used) sp.meta[kMoved] = used - before;
-            if (p >= used) {
-                sp.rank[p] = is ? before : -1;
-                if (is) sp.list[before] = (int)p;
-            } else if (!is) {
-                sp.holes[p - before] = (int)p;
-            }
-        }
+        if (p < end) move_page(sp, (int)p, is, before, used);
         rank += total;
     }
 }
@@ -418,6 +521,13 @@ yl_status launched(const char* what) {
 
 constexpr uint32_t kGridY = 65535;
 
+// Launches one of a kernel's forms for 1, 4 or 16 things per thread of a workgroup.
+#define YL_SMALL(kernel, things, s, ...)                                                                           \
+    do {                                                                                                           \
+        auto k = (things) <= kSmallThreads ? kernel<1> : (things) <= 4 * kSmallThreads ? kernel<4> : kernel<16>;   \
+        hipLaunchKernelGGL(k, dim3(1), dim3(kSmallThreads), 0, s, __VA_ARGS__);                                    \
+    } while (0)
+
 }  // namespace
 }  // namespace yl
 
@@ -440,6 +550,11 @@ yl_status yl_paged_reserve(const yl_paged_tables* tables, const uint32_t* want_l
     if (t.n_seqs && !want_len) return refuse("paged_reserve: no want_len");
     const Space sp = space_of(workspace, t.n_pages, items_of(t, 0));
     const hipStream_t s = (hipStream_t)stream;
+    const int64_t things = std::max<int64_t>({t.n_pages, (int64_t)t.n_seqs * t.max_pages, 1});
+    if (things <= kSmall) {
+        YL_SMALL(k_pages_reserve_small, things, s, t, want_len, lacking);
+        return launched("paged_reserve launch");
+    }
     const int groups = page_groups(t.n_pages), by_seq = (t.n_seqs + 3) / 4;
     hipLaunchKernelGGL(k_pages_count, dim3(groups + by_seq), dim3(256), 0, s, t, sp, 0, want_len, lacking);
     if ((st = launched("paged_reserve launch")) != YL_OK || !t.n_seqs) return st;
@@ -461,9 +576,15 @@ yl_status yl_paged_fork(const yl_paged_tables* tables, const yl_paged_cache* lay
     const Space sp = space_of(workspace, t.n_pages, items_of(t, n));
     const hipStream_t s = (hipStream_t)stream;
     const int groups = page_groups(t.n_pages);
-    hipLaunchKernelGGL(k_pages_count, dim3(groups), dim3(256), 0, s, t, sp, 0, (const uint32_t*)nullptr, lacking);
-    if ((st = launched("paged_fork launch")) != YL_OK || !n) return st;
-    hipLaunchKernelGGL(k_pages_list, dim3(groups + 1), dim3(256), 0, s, t, sp, (int)std::min<uint32_t>(n, t.n_pages), (int)n, parents, children);
+    const int64_t things = std::max<int64_t>(t.n_pages, n);
+    if (things <= kSmall) {
+        YL_SMALL(k_pages_list_small, things, s, t, sp, (int)n, parents, children, lacking);
+        if ((st = launched("paged_fork launch")) != YL_OK || !n) return st;
+    } else {
+        hipLaunchKernelGGL(k_pages_count, dim3(groups), dim3(256), 0, s, t, sp, 0, (const uint32_t*)nullptr, lacking);
+        if ((st = launched("paged_fork launch")) != YL_OK || !n) return st;
+        hipLaunchKernelGGL(k_pages_list, dim3(groups + 1), dim3(256), 0, s, t, sp, (int)std::min<uint32_t>(n, t.n_pages), (int)n, parents, children);
+    }
     for (uint32_t c = 0; c < n && (st = launched("paged_fork launch")) == YL_OK; c += kGridY)
         hipLaunchKernelGGL(k_pages_fork, dim3(2 * pl.n + 1, std::min(n - c, kGridY)), dim3(256), 0, s, t, sp, pl, parents, children, (int)c, lacking);
     return st != YL_OK ? st : launched("paged_fork launch");
@@ -491,9 +612,13 @@ yl_status yl_paged_compact(const yl_paged_tables* tables, const yl_paged_cache* 
     const Space sp = space_of(workspace, t.n_pages, items_of(t, 0));
     const hipStream_t s = (hipStream_t)stream;
     const int groups = page_groups(t.n_pages);
-    hipLaunchKernelGGL(k_pages_count, dim3(groups), dim3(256), 0, s, t, sp, 1, (const uint32_t*)nullptr, (uint32_t*)nullptr);
-    if ((st = launched("paged_compact launch")) != YL_OK) return st;
-    hipLaunchKernelGGL(k_pages_moves, dim3(groups), dim3(256), 0, s, t, sp, used);
+    if (t.n_pages <= kSmall) {
+        YL_SMALL(k_pages_moves_small, t.n_pages, s, t, sp, used);
+    } else {
+        hipLaunchKernelGGL(k_pages_count, dim3(groups), dim3(256), 0, s, t, sp, 1, (const uint32_t*)nullptr, (uint32_t*)nullptr);
+        if ((st = launched("paged_compact launch")) != YL_OK) return st;
+        hipLaunchKernelGGL(k_pages_moves, dim3(groups), dim3(256), 0, s, t, sp, used);
+    }
     if ((st = launched("paged_compact launch")) != YL_OK) return st;
     // as many jobs at most as half of the pages move, in a grid that fills the GPU
     const int64_t jobs = std::max<int64_t>((int64_t)(t.n_pages / 2) * 2 * pl.n, 1);
