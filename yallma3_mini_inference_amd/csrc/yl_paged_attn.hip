@@ -1658,8 +1658,9 @@ size_t bytes_of(const PagedArgs& p, size_t row_units, size_t all_units) {
 //   300 of them, hd 128                           41 |  43 |  34
 //   1500 of them, hd 64                           81 |  94 |  52
 constexpr int kFewAlone = 128, kFewShort = 256, kFewMany = 1600;
-// Units wanted of them (hd 64, 64 sequences of 100 .. 8000 in 1024 | 2048 | 3072: 41 | 33 | 29 us; 16 of them, hd 128: 24 | 26 | 31).
-constexpr int kFewLeast = 1024, kFewMost = 3072;
+// Units wanted of them (hd 64, 64 sequences of 100 .. 8000 in one | two | three times
+// kFewLeast: 41 | 33 | 29 us; 16 of them, hd 128: 24 | 26 | 31).
+constexpr int kFewLeast = 1024, kFewMost = 3 * kFewLeast;
 
 // Workgroups of the tile kernel that run at once (their registers).
 int tile_resident(const PagedArgs& p) { return p.hd == 128 ? 256 : 512; }

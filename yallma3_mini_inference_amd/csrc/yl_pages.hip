@@ -627,9 +627,10 @@ yl_status yl_paged_compact(const yl_paged_tables* tables, const yl_paged_cache* 
         hipLaunchKernelGGL(k_pages_moves, dim3(groups), dim3(256), 0, s, t, sp, used);
     }
     if ((st = launched("paged_compact launch")) != YL_OK) return st;
-    // as many jobs at most as half of the pages move, in a grid that fills the GPU
-    const int64_t jobs = std::max<int64_t>((int64_t)(t.n_pages / 2) * 2 * pl.n, 1);
-    hipLaunchKernelGGL(k_pages_move, dim3((unsigned)std::min<int64_t>(jobs, 4096)), dim3(256), 0, s, t, sp, pl);
+    // as many copies at most as half of the pages move, or the entries, in a grid that fills the GPU
+    const int64_t copies = (int64_t)(t.n_pages / 2) * 2 * pl.n, entries = ((int64_t)t.n_seqs * t.max_pages + t.prefix_entries + 255) / 256;
+    const unsigned grid = (unsigned)std::clamp<int64_t>(std::max(copies, entries), 1, 4096);
+    hipLaunchKernelGGL(k_pages_move, dim3(grid), dim3(256), 0, s, t, sp, pl);
     return launched("paged_compact launch");
 }
 
