@@ -726,6 +726,10 @@ __device__ __forceinline__ size_t part_of(const PagedAttn& a, int row, int head,
 // at 100 .. 8000, bf16, hd 128: 122 us, 5.3 TB/s (units of unlike lengths).  A
 // single row at 600 positions 8 us: launch, three round trips, then what one CU
 // loads (57 GB/s); eight wavefronts for four, or values a step ahead, the same.
+// MXFP4 pages come in a step ahead as codes (a quarter of the registers that bf16
+// would take) and become bf16 as they are used: 64 rows at 100 .. 8000, 64 query heads
+// on 8, hd 64: 44 us, 2.0 TB/s, bound by
+// instructions.
 template <typename C, int HD>
 __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int prefix) {
     using R = Tile<C, HD, false>;
@@ -1281,6 +1285,13 @@ __global__ __launch_bounds__(64 * W, HD == 128 ? 2 : 3) void k_paged_attn_few(Pa
 // the time, vector instructions 49%, clock 2.05 GHz.  Measured and dropped: two
 // row tiles a wavefront (309 us), 4 wavefronts (281), 128 positions a tile
 // (262); at hd 128, 12 and 16 wavefronts spill (bf16 326 us -> 412 and 699).
+// MXFP4 pages: a thread loads codes while the tile before is computed, and writes them
+// to LDS as bf16, once for all eight wavefronts.  Four prompts of 600 .. 3000 tokens, 32
+// heads on 8, hd 64: 279 us (bf16 pages 293), 340 TFLOP/s, three times that in the
+// parts; hd 128 556 (585).  Measured and dropped: f16 against exponents, a key's
+// own and one of the values that all wavefronts raise together, which takes two parts for
+// three (291 and 696 us: a look at the exponent behind every barrier, registers);
+// parts cut by two-term products with -1 and 0 (v_dot2: 7 instructions for 11, 282 us).
 constexpr int kTileWaves = 8, kTileRows = kTileWaves * kRowTile;
 // Of 4 rows by 16 columns of halfwords, of which the 16 lanes of a row of the
 // wavefront point to four halfwords each, lane c gets column c.
