@@ -36,6 +36,24 @@ def test_as_many_heads_as_there_may_be(gpu, kvh, single):
     _check(sc, call.result()[0])
 
 
+@pytest.mark.parametrize("hd,power", [(64, 40), (64, -40), (128, 100), (128, -100)])
+@pytest.mark.parametrize("seqs", [3, 70])
+def test_large_keys_where_queries_are_zero(gpu, hd, power, seqs):
+    """Queries of 2^40 or 2^100, or so much smaller, in one half of a head, keys of 2^120 in the other and of zero in the first: all scores are
+    zero, whatever the scales multiply to."""
+    sc = MxScene([1] * seqs, [700] + [90] * (seqs - 1), 4, 2, hd, 16, seed=9)
+    q = sc.q.reshape(seqs, 4, hd)
+    q[..., :hd // 2] *= np.float32(2.0 ** power)
+    q[..., hd // 2:] = 0.0
+    sc.k32[..., :hd // 2] *= 0.0
+    sc.k32[..., hd // 2:] *= np.float32(2.0 ** 120)
+    sc.k32[~np.isfinite(sc.k32)] = np.nan                # (slots that nothing holds)
+    sc.settle()
+    call = Call(gpu, sc, single=True)
+    call()
+    _check(sc, call.result()[0])
+
+
 @pytest.mark.parametrize("prefix", [0, 40])
 def test_captured_calls_share_a_workspace(gpu, prefix):
     """Single rows and prompts in graphs of their own over the workspace of the larger one, replayed in turn."""

@@ -977,6 +977,11 @@ template <int I>
 __device__ __forceinline__ uint32_t half_pair(uint32_t codes, float unit) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, unit, I));
 }
+// of four neighbouring lanes, the one that the pattern names
+template <int P>
+__device__ __forceinline__ int quad(uint32_t v) {
+    return __builtin_amdgcn_update_dpp(0, (int)v, P, 0xF, 0xF, true);
+}
 // over the 16 lanes of one n
 __device__ __forceinline__ float few_max(float v) {
     v = fmaxf(v, dpp_mov<0x124>(v));                      // row_ror:4
@@ -1042,7 +1047,7 @@ __global__ __launch_bounds__(64 * W, HD == 128 ? 2 : 3) void k_paged_attn_few(Pa
     }
     __syncthreads();
     constexpr int kKeyBits = 12;                          // a key's largest unit in f16: 6 * 2^12
-    const float unscale = __builtin_amdgcn_ldexpf(1.0f, min(max(a.scale_exp - ex - kKeyBits, -126), 127));
+    const int unscale = a.scale_exp - ex - kKeyBits - 127;      // a score: its products times 2^(the key's scale byte + unscale)
     const int lim = (int)min((int64_t)limit_of_row(a, set, row), held);
     const int lo = min(begin, lim), hi = u.splits > 1 && lim - lo > u.chunk ? lo + u.chunk : lim;
     const size_t part0 = ((size_t)slot * a.p.n_kv + kvh) * kRowTile;
@@ -1095,12 +1100,18 @@ __global__ __launch_bounds__(64 * W, HD == 128 ? 2 : 3) void k_paged_attn_few(Pa
             dh = mul4(upper, u2{q1[0], q1[1]}, dh);
         }
         __builtin_amdgcn_sched_barrier(0);
-        // (a scale of 255 is NaN)
-        const float factor = __uint_as_float(top == 255u ? 0x7fc00000u : top << 23);
-        s[0] = (dh[0] + dl[0]) * (dpp_mov<0x00>(factor) * unscale);
-        s[1] = (dh[1] + dl[1]) * (dpp_mov<0x55>(factor) * unscale);
-        s[2] = (dh[2] + dl[2]) * (dpp_mov<0xAA>(factor) * unscale);
-        s[3] = (dh[3] + dl[3]) * (dpp_mov<0xFF>(factor) * unscale);
+        // (by exponents: a factor might be infinite where a sum is zero; a scale of 255 is NaN)
+        s[0] = __builtin_amdgcn_ldexpf(dh[0] + dl[0], quad<0x00>(top) + unscale);
+        s[1] = __builtin_amdgcn_ldexpf(dh[1] + dl[1], quad<0x55>(top) + unscale);
+        s[2] = __builtin_amdgcn_ldexpf(dh[2] + dl[2], quad<0xAA>(top) + unscale);
+        s[3] = __builtin_amdgcn_ldexpf(dh[3] + dl[3], quad<0xFF>(top) + unscale);
+        if (__ballot(top == 255u)) {
+            const float nan = __uint_as_float(0x7fc00000u);
+            if (quad<0x00>(top) == 255) s[0] = nan;
+            if (quad<0x55>(top) == 255) s[1] = nan;
+            if (quad<0xAA>(top) == 255) s[2] = nan;
+            if (quad<0xFF>(top) == 255) s[3] = nan;
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++) vu[i] = x.value_unit(i, n);
         // what is not there: no weight, and values of zero (a garbage scale may be NaN)
