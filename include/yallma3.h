@@ -330,7 +330,8 @@ yl_status yl_paged_gather(const yl_paged_cache *cache, const yl_paged_batch *bat
  * row per sequence (row_start NULL) and up to four query heads per kv head as over
  * f16 caches, and then blocks of a key below 2^-35 of its largest, and of the
  * values below 2^-35 of the largest value of the sequence, may count as zero; else
- * as over bf16 caches.
+ * as over bf16 caches.  (Weighted values are summed in f32 before they are divided by
+ * the weights' sum: from some 2^80 on they may pass it.)
  * q, out: [n_rows] rows of n_heads * head_size floats (device), q_ld and out_ld
  * floats apart; out may be q (with q_ld) but not overlap it otherwise.  A prefix
  * is read once for all sequences.  workspace (device, 16-byte aligned):
