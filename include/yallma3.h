@@ -358,8 +358,8 @@ yl_status yl_paged_attention(float *out, size_t out_ld, const float *q, size_t q
  * the bit: free pages are taken in rising order, by the entries of a call in
  * their order.  Operations on the same tables have to follow each other.
  * workspace: yl_paged_tables_workspace bytes, 16-byte aligned, for `n` forks at
- * most; it serves any of the operations on tables no larger.  `lacking` (device,
- * nullable) receives a count and is 0 when all was done. */
+ * most; it serves any of the operations on tables no larger, one at a time.
+ * `lacking` (device, nullable) receives a count and is 0 when all was done. */
 typedef struct {
     uint32_t n_seqs, max_pages, n_pages, page_size;
     int32_t *page_table;         /* device [n_seqs][max_pages] */

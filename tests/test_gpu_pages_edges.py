@@ -97,6 +97,30 @@ def test_compact_of_tables_wider_than_their_pool(gpu, refs):
     _same(t, m, got)
 
 
+def test_pools_whose_workgroups_look_through_more_pages(gpu):
+    """Beyond 2^20 pages a workgroup has more than one stretch of them; used pages in all parts of the pool."""
+    from yallma3_mini_inference_amd import ops
+    rng = np.random.default_rng(5)
+    n_pages = 1100000
+    pool = rng.integers(0, 256, (n_pages, 1, 16, 17)).astype(np.uint8)
+    used = rng.choice(n_pages, 400, replace=False)
+    table, refs = np.full((20, 40), -1), np.zeros(n_pages, int)
+    table[:10] = used.reshape(10, 40)
+    refs[used] = 1
+    lens = np.where(np.arange(20) < 10, 640 - 7 * np.arange(20), 0)
+    m = Pages(table, lens, refs, 16, [(pool, pool[::-1])])
+    parents, children = np.arange(10), 10 + rng.permutation(10)
+    t = _tables(ops, m)
+    lacking, got = ops.paged_fork(t, m.layers, parents, children)
+    assert lacking == m.fork(parents, children) == 0
+    _same(t, m, got)
+    ops.paged_release(t, [3, 8, 14])
+    m.release([3, 8, 14])
+    count, got = ops.paged_compact(t, got)
+    assert count == m.compact()
+    _same(t, m, got)
+
+
 @pytest.mark.parametrize("rows,entries", [(0, 4), (3, 0), (0, 0)])
 def test_tables_of_nothing(gpu, rows, entries):
     """No sequences, or no entries: ids name nothing, lengths are within the prefix or lack."""
