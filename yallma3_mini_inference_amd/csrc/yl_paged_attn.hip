@@ -927,9 +927,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_rows(PagedAttn a, int pre
 // blocks, of the values of the other positions.
 // Bound by vector instructions (some 220 for 64 positions of hd 64, 380 of hd 128,
 // and as many again in a unit's first and last part) and the latency of its few
-// steps: two rows at 128,000 positions, 32 heads on 8, hd 64: 32 us, 4.4 TB/s of 17/32
+// steps: two rows at 128,000 positions, 32 heads on 8, hd 64: 36 us, 3.9 TB/s of 17/32
 // byte an element (the row kernel's 16-row tiles 47); 64 rows at 100 .. 8000, hd 128:
-// 46 us, 3.7 TB/s (52).  Measured and dropped: q's parts in registers (spills), one
+// 48 us, 3.6 TB/s (52).  Measured and dropped: q's parts in registers (spills), one
 // buffer of keys and values for the two (hd 64 168 registers or 128, 44 us), even
 // shares of all positions that cross sequences (67 us: each takes a unit's first and
 // last part in turn).
